@@ -482,6 +482,37 @@ typedef struct {
 } ktb_attn_args;
 int ktb_launch_attention_fwd(ktb_ctx* ctx, const ktb_attn_args* args);
 
+/* ---- rotary positions -------------------------------------------------------------------
+ * Pairs (x, y) of a head turned by an angle of the token's position p: x cos[p, j] - y sin[p, j] and
+ * y cos[p, j] + x sin[p, j], products and sums in f32 one by one, rounded once to the tensors' type; `inverse` takes -sin.
+ * What a KTIR program does that loads a row of both tables through an index tensor (ktir_cpu/ops/memory_ops.py:867-915),
+ * multiplies, adds and stores (ktir_cpu/dialects/arith_ops.py:49-59).  An item holds `tokens` tokens of every tensor:
+ * its entry of the item table is the offset of its first position (idx_dtype units), then per tensor the offsets, in and
+ * out, of the first element of its first pair.  Element j of a pair's first half is at j * pair_stride, its partner
+ * in_partner / out_partner (> 0) behind; `rest` elements from in_rest on are copied to out_rest.  Outputs and inputs are
+ * apart, or the same elements.  A position whose row is past a table's end (cos_end, sin_end: elements of the arena)
+ * reads zeros there; a negative one is recorded in the status word. */
+#define KTB_ROTARY_TENSORS 4
+typedef struct {
+    int32_t heads, rest;
+    int64_t in_token, in_head, out_token, out_head;      /* element strides */
+    int64_t in_partner, out_partner, in_rest, out_rest;  /* element distances from a head's first pair */
+} ktb_rotary_tensor;
+typedef struct {
+    void* arena;
+    const int64_t* dev_item_offsets;          /* [n_items][1 + 2 * n_tensors] */
+    int64_t n_items;
+    int32_t tokens, pairs;                    /* per item; per head */
+    int32_t dtype, idx_dtype;                 /* KTB_F16 / KTB_F32; KTB_I32 / KTB_I64 */
+    int32_t n_tensors, inverse;
+    int64_t pos_stride, pair_stride;
+    int64_t table_stride, cos_off, sin_off;   /* f32 elements: from row to row, first rows */
+    int64_t cos_end, sin_end;
+    int32_t align, reserved;                  /* a power of two that divides the tensors' offsets in the item table */
+    ktb_rotary_tensor t[KTB_ROTARY_TENSORS];
+} ktb_rotary_args;
+int ktb_launch_rotary(ktb_ctx* ctx, const ktb_rotary_args* args);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1351,3 +1351,335 @@ def layernorm_blocked(n_rows: int = 64, n_cols: int = 1024, block: int = 256, co
           f"        %y = arith.addf %xw, %b : {tb}\n        ktdp.store %y, %ya : {tb}, {at}\n"
           "        scf.yield\n      }\n      scf.yield\n    }\n    return\n  }\n}\n")
     return s
+
+
+def rotary(tokens: int = 64, heads: int = 8, kv_heads: int = 2, head_dim: int = 128, rotary_dim: int | None = None,
+           table_rows: int = 4096, layout: str = "half", inverse: bool = False, dtype: str = "f16",
+           block: int | None = None) -> str:
+    """Rotary positions for the queries [tokens, heads, head_dim] and keys [tokens, kv_heads, head_dim] of packed
+    sequences (the reference's generator of such a kernel: notebooks/demo_gen_mlir.py:471-569).
+
+    Token t has the position ``positions[t]`` (i32), which picks row p of the f32 tables ``cos`` and ``sin``
+    [table_rows, rotary_dim / 2].  Pair j of a head's first ``rotary_dim`` elements is turned by that angle,
+    (a, b) -> (a cos - b sin, b cos + a sin), in f32, rounded once; the elements behind are copied.  ``layout`` says which
+    elements are pair j: "half" j and j + rotary_dim / 2, "interleaved" 2j and 2j + 1.  ``inverse`` turns back: the
+    gradient of the rotation.  ``kv_heads = 0`` leaves the keys out.  The tables hold whatever frequencies a model uses
+    (``rotary_tables``).  A core owns ``block`` tokens, a divisor of ``tokens``."""
+    rot = head_dim if rotary_dim is None else rotary_dim
+    assert layout in ("half", "interleaved") and dtype in ("f16", "f32") and 0 < rot <= head_dim and rot % 2 == 0
+    n, T = rot // 2, tokens
+    if block is None:
+        most = max(1, 16384 // (max(heads, kv_heads) * n))
+        block = max(b for b in range(1, min(most, T) + 1) if T % b == 0)
+    assert T % block == 0
+    bt = block
+    tensors = [("query", heads)] + ([("key", kv_heads)] if kv_heads else [])
+    ptrs = [f"%{x}_out_ptr" for x, _ in tensors] + [f"%{x}_ptr" for x, _ in tensors] + ["%positions_ptr", "%cos_ptr", "%sin_ptr"]
+    s = (f"module {{\n  func.func @rotary_kernel({', '.join(p + ': index' for p in ptrs)}) attributes {{grid = [{T // bt}]}} {{\n"
+         f"    %pid = ktdp.get_compute_tile_id : index\n"
+         f"    %c0 = arith.constant 0 : index\n    %c1 = arith.constant 1 : index\n"
+         f"    %c_half = arith.constant {n} : index\n    %c_rot = arith.constant {rot} : index\n"
+         f"    %c_bt = arith.constant {bt} : index\n    %t0 = arith.muli %pid, %c_bt : index\n")
+    s += view("positions", "positions_ptr", [T], "i32")
+    tc, at_c = f"tensor<{bt}x{n}xf32>", f"!ktdp.access_tile<{bt}x{n}xindex>"
+    for x in ("cos", "sin"):
+        s += view(f"{x}_table", f"{x}_ptr", [table_rows, n], "f32")
+        s += (f"    %{x}_tile = ktdp.construct_indirect_access_tile\n"
+              f"        intermediate_variables(%d0, %d1)\n"
+              f"        %{x}_table[ind(%positions[%t0 + %d0]), (%d1)] {{\n"
+              f"      variables_space_set = {_box([bt, n])},\n      variables_space_order = {_ident(2)}\n"
+              f"    }} : memref<{table_rows}x{n}xf32>, memref<{T}xi32> -> {at_c}\n"
+              f"    %{x} = ktdp.load %{x}_tile : {at_c} -> {tc}\n")
+    for x, H in tensors:
+        t3, t3s = f"tensor<{_xs([bt, H, n], 'f32')}>", f"tensor<{_xs([bt, H, n], dtype)}>"
+        if layout == "half":
+            vs, ts, st = [T, H, head_dim], [bt, H, n], None
+            at = [["%t0", "%c0", "%c0"], ["%t0", "%c0", "%c_half"]]
+        else:
+            vs, ts, st = [T, H, n, 2], [bt, H, n, 1], [H * head_dim, head_dim, 2, 1]
+            at = [["%t0", "%c0", "%c0", "%c0"], ["%t0", "%c0", "%c0", "%c1"]]
+        tt, att = f"tensor<{_xs(ts, dtype)}>", f"!ktdp.access_tile<{_xs(ts, 'index')}>"
+        s += view(f"{x}_in", f"{x}_ptr", vs, dtype, st) + view(f"{x}_res", f"{x}_out_ptr", vs, dtype, st)
+        for a, where in zip("ab", at):
+            v = f"{x}_{a}"
+            steps = [f"ktdp.load %{v}_tile : {att} -> {tt}"]
+            if layout != "half":
+                steps.append(f"tensor.collapse_shape %{v}_0 [[0], [1], [2, 3]] : {tt} into {t3s}")
+            if dtype == "f16":
+                steps.append(f"arith.extf %{v}_{len(steps) - 1} : {t3s} to {t3}")
+            s += tile(f"{v}_tile", f"{x}_in", where, ts, vs, dtype)
+            s += "".join(f"    %{v}_{k} = {line}\n" for k, line in enumerate(steps[:-1])) + f"    %{v} = {steps[-1]}\n"
+        for f in ("cos", "sin"):
+            s += (f"    %{x}_{f}_e = tensor.empty() : {t3}\n"
+                  f"    %{x}_{f} = linalg.broadcast ins(%{f} : {tc}) outs(%{x}_{f}_e : {t3}) dimensions = [1]\n")
+        first, second = ("addf", "subf") if inverse else ("subf", "addf")
+        s += (f"    %{x}_ac = arith.mulf %{x}_a, %{x}_cos : {t3}\n    %{x}_bs = arith.mulf %{x}_b, %{x}_sin : {t3}\n"
+              f"    %{x}_bc = arith.mulf %{x}_b, %{x}_cos : {t3}\n    %{x}_as = arith.mulf %{x}_a, %{x}_sin : {t3}\n"
+              f"    %{x}_ya = arith.{first} %{x}_ac, %{x}_bs : {t3}\n    %{x}_yb = arith.{second} %{x}_bc, %{x}_as : {t3}\n")
+        for a, where in zip("ab", at):
+            v = f"{x}_y{a}"
+            out = v
+            if dtype == "f16":
+                out = f"{v}_r"
+                s += f"    %{out} = arith.truncf %{v} : {t3} to {t3s}\n"
+            if layout != "half":
+                s += (f"    %{v}_x = tensor.expand_shape %{out} [[0], [1], [2, 3]] output_shape [{bt}, {H}, {n}, 1] : "
+                      f"{t3s} into {tt}\n")
+                out = f"{v}_x"
+            s += tile(f"{v}_tile", f"{x}_res", where, ts, vs, dtype) + f"    ktdp.store %{out}, %{v}_tile : {tt}, {att}\n"
+        if rot < head_dim:
+            rest = [bt, H, head_dim - rot]
+            tr, atr = f"tensor<{_xs(rest, dtype)}>", f"!ktdp.access_tile<{_xs(rest, 'index')}>"
+            for io, ptr in (("in", f"{x}_ptr"), ("res", f"{x}_out_ptr")):
+                s += view(f"{x}_{io}_whole", ptr, [T, H, head_dim], dtype)
+                s += tile(f"{x}_{io}_rest", f"{x}_{io}_whole", ["%t0", "%c0", "%c_rot"], rest, [T, H, head_dim], dtype)
+            s += (f"    %{x}_rest = ktdp.load %{x}_in_rest : {atr} -> {tr}\n"
+                  f"    ktdp.store %{x}_rest, %{x}_res_rest : {tr}, {atr}\n")
+    return s + "    return\n  }\n}\n"
+
+
+def rotary_tables(table_rows: int, rotary_dim: int, base: float = 10000.0, stretch: float = 1.0, rescale_base: bool = False):
+    """(cos, sin), f32 [table_rows, rotary_dim / 2]: the angles p / stretch * base^(-2 j / rotary_dim), taken in 64 bits (in
+    32 the angle of position 10^6 is off by up to 0.03).  ``stretch`` > 1 is a context that much longer than the trained
+    one: positions are squeezed into the trained range, or, with ``rescale_base``, the base grows so that the slowest pair
+    is slowed down by ``stretch`` and the fastest not at all."""
+    import numpy as np
+    assert rotary_dim % 2 == 0 and table_rows > 0 and stretch > 0
+    pos = np.arange(table_rows, dtype=np.float64)
+    if rescale_base:
+        if rotary_dim > 2:
+            base = base * stretch ** (rotary_dim / (rotary_dim - 2))
+    else:
+        pos = pos / stretch
+    angle = pos[:, None] * base ** (-np.arange(0, rotary_dim, 2, dtype=np.float64) / rotary_dim)
+    return np.cos(angle).astype(np.float32), np.sin(angle).astype(np.float32)
+
+
+def _attention_tiles(q_len, kv_len, heads, kv_heads, block_q, block_kv):
+    """(queries per tile, query heads per key head, rows per tile, keys per tile) of the attention generators below."""
+    assert q_len > 0 and kv_len > 0 and kv_heads > 0 and heads % kv_heads == 0
+    grp = heads // kv_heads
+    bq = min(q_len, max(1, 128 // grp)) if block_q is None else block_q
+    return bq, grp, bq * grp, min(kv_len, 128) if block_kv is None else block_kv
+
+
+def _attention_scores(p, q, k, q0, k0, dims, causal, kv_len, ind):
+    """Scaled scores of a tile of query rows (position-major, ``grp`` heads each) and a tile of keys; %{p}hidden says what
+    stands where a query does not see a key: ``None`` returned as its condition if it sees all."""
+    bm, bn, hd, grp = dims
+    f = lambda shp, dt="f32": f"tensor<{_xs(shp, dt)}>"   # noqa: E731
+    s = (f"{ind}%{p}kt_e = tensor.empty() : {f([hd, bn], 'f16')}\n"
+         f"{ind}%{p}kt16 = linalg.transpose ins(%{k}16 : {f([bn, hd], 'f16')}) outs(%{p}kt_e : {f([hd, bn], 'f16')}) permutation = [1, 0]\n"
+         f"{ind}%{p}kt = arith.extf %{p}kt16 : {f([hd, bn], 'f16')} to {f([hd, bn])}\n"
+         f"{ind}%{p}s_zero = tensor.splat %zero : {f([bm, bn])}\n"
+         f"{ind}%{p}qk = linalg.matmul ins(%{q}, %{p}kt : {f([bm, hd])}, {f([hd, bn])}) outs(%{p}s_zero : {f([bm, bn])}) -> {f([bm, bn])}\n"
+         f"{ind}%{p}scale = tensor.splat %scale : {f([bm, bn])}\n"
+         f"{ind}%{p}sc = arith.mulf %{p}scale, %{p}qk : {f([bm, bn])}\n")
+    lines = ["%c = linalg.index 1 : index", f"%k_pos = arith.addi %{k0}, %c : index"]
+    if causal:
+        lines += ["%r = linalg.index 0 : index", "%in_tile = arith.divui %r, %c_grp : index",
+                  f"%q_pos = arith.addi %{q0}, %in_tile : index", "%keep = arith.cmpi sle, %k_pos, %q_pos : index"]
+    elif kv_len % bn:
+        lines += ["%keep = arith.cmpi slt, %k_pos, %c_kv : index"]
+    else:
+        lines = None
+    return s, lines
+
+
+def attention_forward(q_len: int = 256, kv_len: int = 256, heads: int = 8, kv_heads: int = 8, head_dim: int = 128,
+                      causal: bool = True, block_q: int | None = None, block_kv: int | None = None) -> str:
+    """Attention of a training step or a prefill: O = softmax(scale Q K^T) V and, for the backward pass, the log-sum-exp
+    of every row's scaled scores.
+
+    Queries and output are [q_len, heads, head_dim] f16, keys and values [kv_len, kv_heads, head_dim] f16 (a batch folds
+    into the heads), ``lse`` is [q_len, heads] f32.  ``causal``: query i sees the keys up to i + kv_len - q_len; a row that
+    sees none gives 0 and -inf.  Core (i, h) owns ``block_q`` positions of the query heads that share key head h and walks
+    the keys ``block_kv`` at a time with a running maximum, sum and accumulator in f32, as ``paged_attention`` does.  The
+    last tiles run past the end of the tensors: what they read there is zero, what they store is dropped
+    (ktir_cpu/memory.py:217-306)."""
+    bq, grp, bm, bn = _attention_tiles(q_len, kv_len, heads, kv_heads, block_q, block_kv)
+    hd = head_dim
+    qv, kvv, lv = [q_len, heads, hd], [kv_len, kv_heads, hd], [q_len, heads]
+    f = lambda shp, dt="f32": f"tensor<{_xs(shp, dt)}>"   # noqa: E731
+    at = lambda shp: f"!ktdp.access_tile<{_xs(shp, 'index')}>"   # noqa: E731
+    q3, k3, l2 = [bq, grp, hd], [bn, 1, hd], [bq, grp]
+    s = (f"module {{\n  func.func @attention_forward_kernel(%output_ptr: index, %lse_ptr: index, %query_ptr: index, %key_ptr: index,\n"
+         f"      %value_ptr: index, %scale: f32) attributes {{grid = [{-(-q_len // bq)}, {kv_heads}]}} {{\n"
+         f"    %pid0, %pid1 = ktdp.get_compute_tile_id : index, index\n"
+         f"    %c0 = arith.constant 0 : index\n    %c1 = arith.constant 1 : index\n"
+         f"    %c_bq = arith.constant {bq} : index\n    %c_grp = arith.constant {grp} : index\n    %c_bn = arith.constant {bn} : index\n"
+         f"    %c_kv = arith.constant {kv_len} : index\n    %c_before = arith.constant {kv_len - q_len} : index\n"
+         f"    %n_tiles = arith.constant {-(-kv_len // bn)} : index\n"
+         f"    %q_row0 = arith.muli %pid0, %c_bq : index\n    %q_head0 = arith.muli %pid1, %c_grp : index\n"
+         f"    %q_abs0 = arith.addi %q_row0, %c_before : index\n"
+         f"    %ninf_bits = arith.constant 0xFF800000 : i32\n    %ninf = arith.bitcast %ninf_bits : i32 to f32\n"
+         f"    %zero = arith.constant 0.0 : f32\n    %low = arith.constant -1.0e30 : f32\n    %tiny = arith.constant 1.0e-30 : f32\n")
+    s += view("query", "query_ptr", qv, "f16") + view("output", "output_ptr", qv, "f16") + view("lse", "lse_ptr", lv, "f32")
+    s += view("key", "key_ptr", kvv, "f16") + view("value", "value_ptr", kvv, "f16")
+    s += tile("q_tile", "query", ["%q_row0", "%q_head0", "%c0"], q3, qv, "f16")
+    s += (f"    %q3 = ktdp.load %q_tile : {at(q3)} -> {f(q3, 'f16')}\n"
+          f"    %q16 = tensor.collapse_shape %q3 [[0, 1], [2]] : {f(q3, 'f16')} into {f([bm, hd], 'f16')}\n"
+          f"    %q = arith.extf %q16 : {f([bm, hd], 'f16')} to {f([bm, hd])}\n"
+          f"    %m_init = tensor.splat %low : {f([bm])}\n    %l_init = tensor.splat %zero : {f([bm])}\n"
+          f"    %acc_init = tensor.splat %zero : {f([bm, hd])}\n"
+          f"    %m_fin, %l_fin, %acc_fin = scf.for %j = %c0 to %n_tiles step %c1\n"
+          f"        iter_args(%m_run = %m_init, %l_run = %l_init, %acc = %acc_init)\n"
+          f"        -> ({f([bm])}, {f([bm])}, {f([bm, hd])}) {{\n"
+          f"      %k_row0 = arith.muli %j, %c_bn : index\n")
+    for x in ("k", "v"):
+        s += tile(f"{x}_tile", "key" if x == "k" else "value", ["%k_row0", "%pid1", "%c0"], k3, kvv, "f16", "      ")
+        s += (f"      %{x}3 = ktdp.load %{x}_tile : {at(k3)} -> {f(k3, 'f16')}\n"
+              f"      %{x}16 = tensor.collapse_shape %{x}3 [[0, 1], [2]] : {f(k3, 'f16')} into {f([bn, hd], 'f16')}\n")
+    s += f"      %v = arith.extf %v16 : {f([bn, hd], 'f16')} to {f([bn, hd])}\n"
+    text, keep = _attention_scores("", "q", "k", "q_abs0", "k_row0", (bm, bn, hd, grp), causal, kv_len, "      ")
+    s += text
+    masked = "sc"
+    if keep:
+        masked = "masked"
+        s += _generic("masked", [("sc", [bm, bn])], [bm, bn], ["s_val"],
+                      keep + ["%sel = arith.select %keep, %s_val, %ninf : f32", "sel"])
+    s += (f"      %rmax_init = tensor.splat %ninf : {f([bm])}\n"
+          f"      %rmax = linalg.reduce {{ arith.maximumf }} ins(%{masked} : {f([bm, bn])}) outs(%rmax_init : {f([bm])}) dimensions = [1]\n"
+          f"      %m_new = arith.maximumf %m_run, %rmax : {f([bm])}\n"
+          f"      %m_e = tensor.empty() : {f([bm, bn])}\n"
+          f"      %m_b = linalg.broadcast ins(%m_new : {f([bm])}) outs(%m_e : {f([bm, bn])}) dimensions = [1]\n"
+          f"      %shift = arith.subf %{masked}, %m_b : {f([bm, bn])}\n"
+          f"      %p = math.exp %shift : {f([bm, bn])}\n"
+          f"      %lsum_init = tensor.splat %zero : {f([bm])}\n"
+          f"      %lsum = linalg.reduce {{ arith.addf }} ins(%p : {f([bm, bn])}) outs(%lsum_init : {f([bm])}) dimensions = [1]\n"
+          f"      %dm = arith.subf %m_run, %m_new : {f([bm])}\n"
+          f"      %alpha = math.exp %dm : {f([bm])}\n"
+          f"      %a_e = tensor.empty() : {f([bm, hd])}\n"
+          f"      %alpha_b = linalg.broadcast ins(%alpha : {f([bm])}) outs(%a_e : {f([bm, hd])}) dimensions = [1]\n"
+          f"      %acc_scaled = arith.mulf %acc, %alpha_b : {f([bm, hd])}\n"
+          f"      %acc_new = linalg.matmul ins(%p, %v : {f([bm, bn])}, {f([bn, hd])}) "
+          f"outs(%acc_scaled : {f([bm, hd])}) -> {f([bm, hd])}\n"
+          f"      %l_scaled = arith.mulf %l_run, %alpha : {f([bm])}\n"
+          f"      %l_new = arith.addf %l_scaled, %lsum : {f([bm])}\n"
+          f"      scf.yield %m_new, %l_new, %acc_new : {f([bm])}, {f([bm])}, {f([bm, hd])}\n"
+          f"    }}\n"
+          f"    %tiny_t = tensor.splat %tiny : {f([bm])}\n"
+          f"    %l_safe = arith.maximumf %l_fin, %tiny_t : {f([bm])}\n"
+          f"    %l_e = tensor.empty() : {f([bm, hd])}\n"
+          f"    %l_b = linalg.broadcast ins(%l_safe : {f([bm])}) outs(%l_e : {f([bm, hd])}) dimensions = [1]\n"
+          f"    %o32 = arith.divf %acc_fin, %l_b : {f([bm, hd])}\n"
+          f"    %o16 = arith.truncf %o32 : {f([bm, hd])} to {f([bm, hd], 'f16')}\n"
+          f"    %o3 = tensor.expand_shape %o16 [[0, 1], [2]] output_shape [{bq}, {grp}, {hd}] : {f([bm, hd], 'f16')} into {f(q3, 'f16')}\n"
+          f"    %l_log = math.log %l_fin : {f([bm])}\n"
+          f"    %lse1 = arith.addf %m_fin, %l_log : {f([bm])}\n"
+          f"    %lse2 = tensor.expand_shape %lse1 [[0, 1]] output_shape [{bq}, {grp}] : {f([bm])} into {f(l2)}\n")
+    s += tile("o_tile", "output", ["%q_row0", "%q_head0", "%c0"], q3, qv, "f16")
+    s += tile("l_tile", "lse", ["%q_row0", "%q_head0"], l2, lv, "f32")
+    return s + (f"    ktdp.store %o3, %o_tile : {f(q3, 'f16')}, {at(q3)}\n"
+                f"    ktdp.store %lse2, %l_tile : {f(l2)}, {at(l2)}\n    return\n  }}\n}}\n")
+
+
+def attention_backward(q_len: int = 256, kv_len: int = 256, heads: int = 8, kv_heads: int = 8, head_dim: int = 128,
+                       causal: bool = True, block_q: int | None = None, block_kv: int | None = None) -> str:
+    """Gradients of ``attention_forward``: from Q, K, V, its results O and ``lse`` and the gradient dO of O,
+
+        P = exp(scale Q K^T - lse) where a query sees a key, 0 elsewhere     D = rowsum(dO * O)
+        dS = P * (dO V^T - D)     dQ = scale dS K     dK = scale dS^T Q     dV = P^T dO
+
+    in f32 with f16 results; the probabilities are computed again instead of kept.  dK and dV are the sums over the query
+    heads that share a key head.  Shapes, mask and ragged ends are those of ``attention_forward``.  The first cores own
+    tiles of queries and walk the keys for dQ, the others own tiles of keys and walk the queries for dK and dV."""
+    bq, grp, bm, bn = _attention_tiles(q_len, kv_len, heads, kv_heads, block_q, block_kv)
+    hd = head_dim
+    nq, nk = -(-q_len // bq), -(-kv_len // bn)
+    qv, kvv, lv = [q_len, heads, hd], [kv_len, kv_heads, hd], [q_len, heads]
+    f = lambda shp, dt="f32": f"tensor<{_xs(shp, dt)}>"   # noqa: E731
+    at = lambda shp: f"!ktdp.access_tile<{_xs(shp, 'index')}>"   # noqa: E731
+    q3, k3, l2 = [bq, grp, hd], [bn, 1, hd], [bq, grp]
+    names = ("query_grad", "key_grad", "value_grad", "query", "key", "value", "output", "lse", "output_grad")
+    s = (f"module {{\n  func.func @attention_backward_kernel({', '.join(f'%{x}_ptr: index' for x in names)},\n"
+         f"      %scale: f32) attributes {{grid = [{nq + nk}, {kv_heads}]}} {{\n"
+         f"    %pid0, %pid1 = ktdp.get_compute_tile_id : index, index\n"
+         f"    %c0 = arith.constant 0 : index\n    %c1 = arith.constant 1 : index\n"
+         f"    %c_bq = arith.constant {bq} : index\n    %c_grp = arith.constant {grp} : index\n    %c_bn = arith.constant {bn} : index\n"
+         f"    %c_kv = arith.constant {kv_len} : index\n    %c_before = arith.constant {kv_len - q_len} : index\n"
+         f"    %n_q = arith.constant {nq} : index\n    %n_k = arith.constant {nk} : index\n"
+         f"    %q_head0 = arith.muli %pid1, %c_grp : index\n"
+         f"    %zero = arith.constant 0.0 : f32\n")
+    for x in names:
+        s += view(x, f"{x}_ptr", qv if x in ("query", "query_grad", "output", "output_grad") else lv if x == "lse" else kvv,
+                  "f32" if x == "lse" else "f16")
+
+    def query_side(p, row0, ind):
+        """A tile of query rows: %{p}q, %{p}do, %{p}lse and %{p}d = rowsum(dO * O)."""
+        t = ""
+        for x, src in (("q", "query"), ("do", "output_grad"), ("o", "output")):
+            t += tile(f"{p}{x}_tile", src, [f"%{row0}", "%q_head0", "%c0"], q3, qv, "f16", ind)
+            t += (f"{ind}%{p}{x}3 = ktdp.load %{p}{x}_tile : {at(q3)} -> {f(q3, 'f16')}\n"
+                  f"{ind}%{p}{x}16 = tensor.collapse_shape %{p}{x}3 [[0, 1], [2]] : {f(q3, 'f16')} into {f([bm, hd], 'f16')}\n"
+                  f"{ind}%{p}{x} = arith.extf %{p}{x}16 : {f([bm, hd], 'f16')} to {f([bm, hd])}\n")
+        t += tile(f"{p}lse_tile", "lse", [f"%{row0}", "%q_head0"], l2, lv, "f32", ind)
+        return t + (f"{ind}%{p}lse2 = ktdp.load %{p}lse_tile : {at(l2)} -> {f(l2)}\n"
+                    f"{ind}%{p}lse = tensor.collapse_shape %{p}lse2 [[0, 1]] : {f(l2)} into {f([bm])}\n"
+                    f"{ind}%{p}doo = arith.mulf %{p}do, %{p}o : {f([bm, hd])}\n"
+                    f"{ind}%{p}d_init = tensor.splat %zero : {f([bm])}\n"
+                    f"{ind}%{p}d = linalg.reduce {{ arith.addf }} ins(%{p}doo : {f([bm, hd])}) outs(%{p}d_init : {f([bm])}) dimensions = [1]\n")
+
+    def key_side(p, row0, ind):
+        t = ""
+        for x, src in (("k", "key"), ("v", "value")):
+            t += tile(f"{p}{x}_tile", src, [f"%{row0}", "%pid1", "%c0"], k3, kvv, "f16", ind)
+            t += (f"{ind}%{p}{x}3 = ktdp.load %{p}{x}_tile : {at(k3)} -> {f(k3, 'f16')}\n"
+                  f"{ind}%{p}{x}16 = tensor.collapse_shape %{p}{x}3 [[0, 1], [2]] : {f(k3, 'f16')} into {f([bn, hd], 'f16')}\n")
+        return t
+
+    def probabilities(p, q0, k0, ind):
+        """%{p}p and %{p}ds of a tile of query rows and a tile of keys."""
+        t, keep = _attention_scores(p, f"{p}q", f"{p}k", q0, k0, (bm, bn, hd, grp), causal, kv_len, ind)
+        lines = [f"%shift = arith.subf %s_val, %l_val : f32", "%e = math.exp %shift : f32"]
+        t += _generic(f"{p}p", [(f"{p}sc", [bm, bn]), (f"{p}lse", [bm])], [bm, bn], ["s_val", "l_val"],
+                      lines + (keep + ["%sel = arith.select %keep, %e, %zero : f32", "sel"] if keep else ["e"]), ind)
+        return t + (f"{ind}%{p}vt_e = tensor.empty() : {f([hd, bn], 'f16')}\n"
+                    f"{ind}%{p}vt16 = linalg.transpose ins(%{p}v16 : {f([bn, hd], 'f16')}) outs(%{p}vt_e : {f([hd, bn], 'f16')}) permutation = [1, 0]\n"
+                    f"{ind}%{p}vt = arith.extf %{p}vt16 : {f([hd, bn], 'f16')} to {f([hd, bn])}\n"
+                    f"{ind}%{p}dp_zero = tensor.splat %zero : {f([bm, bn])}\n"
+                    f"{ind}%{p}dp = linalg.matmul ins(%{p}do, %{p}vt : {f([bm, hd])}, {f([hd, bn])}) outs(%{p}dp_zero : {f([bm, bn])}) -> {f([bm, bn])}\n"
+                    f"{ind}%{p}d_e = tensor.empty() : {f([bm, bn])}\n"
+                    f"{ind}%{p}d_b = linalg.broadcast ins(%{p}d : {f([bm])}) outs(%{p}d_e : {f([bm, bn])}) dimensions = [1]\n"
+                    f"{ind}%{p}dpd = arith.subf %{p}dp, %{p}d_b : {f([bm, bn])}\n"
+                    f"{ind}%{p}ds = arith.mulf %{p}p, %{p}dpd : {f([bm, bn])}\n")
+
+    def finish(p, src, shp, t3, dst, row0, head0, vshp, scaled):
+        """Store the accumulator %{src} as f16, times the score scale where the gradient passes through the scores."""
+        t, x = "", src
+        if scaled:
+            x = f"{src}_s"
+            t += (f"      %{src}_sc = tensor.splat %scale : {f(shp)}\n      %{x} = arith.mulf %{src}, %{src}_sc : {f(shp)}\n")
+        t += (f"      %{src}_h = arith.truncf %{x} : {f(shp)} to {f(shp, 'f16')}\n"
+              f"      %{src}_3 = tensor.expand_shape %{src}_h [[0, 1], [2]] output_shape {list(t3)} : {f(shp, 'f16')} into {f(t3, 'f16')}\n")
+        t += tile(f"{src}_tile", dst, [f"%{row0}", f"%{head0}", "%c0"], t3, vshp, "f16", "      ")
+        return t + f"      ktdp.store %{src}_3, %{src}_tile : {f(t3, 'f16')}, {at(t3)}\n"
+
+    i1, i2 = "      ", "        "
+    s += "    %of_queries = arith.cmpi slt, %pid0, %n_q : index\n    scf.if %of_queries {\n"
+    s += f"{i1}%a_row0 = arith.muli %pid0, %c_bq : index\n{i1}%a_abs0 = arith.addi %a_row0, %c_before : index\n"
+    s += query_side("a_", "a_row0", i1)
+    s += (f"{i1}%dq_init = tensor.splat %zero : {f([bm, hd])}\n"
+          f"{i1}%dq = scf.for %j = %c0 to %n_k step %c1 iter_args(%dq_acc = %dq_init) -> ({f([bm, hd])}) {{\n"
+          f"{i2}%a_k0 = arith.muli %j, %c_bn : index\n")
+    s += key_side("a_", "a_k0", i2) + probabilities("a_", "a_abs0", "a_k0", i2)
+    s += (f"{i2}%a_k = arith.extf %a_k16 : {f([bn, hd], 'f16')} to {f([bn, hd])}\n"
+          f"{i2}%dq_new = linalg.matmul ins(%a_ds, %a_k : {f([bm, bn])}, {f([bn, hd])}) outs(%dq_acc : {f([bm, hd])}) -> {f([bm, hd])}\n"
+          f"{i2}scf.yield %dq_new : {f([bm, hd])}\n{i1}}}\n")
+    s += finish("a_", "dq", [bm, hd], q3, "query_grad", "a_row0", "q_head0", qv, True)
+    s += "    } else {\n"
+    s += f"{i1}%b_tile0 = arith.subi %pid0, %n_q : index\n{i1}%b_k0 = arith.muli %b_tile0, %c_bn : index\n"
+    s += key_side("b_", "b_k0", i1)
+    s += (f"{i1}%dk_init = tensor.splat %zero : {f([bn, hd])}\n{i1}%dv_init = tensor.splat %zero : {f([bn, hd])}\n"
+          f"{i1}%dk, %dv = scf.for %i = %c0 to %n_q step %c1 iter_args(%dk_acc = %dk_init, %dv_acc = %dv_init)\n"
+          f"{i1}    -> ({f([bn, hd])}, {f([bn, hd])}) {{\n"
+          f"{i2}%b_row0 = arith.muli %i, %c_bq : index\n{i2}%b_abs0 = arith.addi %b_row0, %c_before : index\n")
+    s += query_side("b_", "b_row0", i2) + probabilities("b_", "b_abs0", "b_k0", i2)
+    for x, left, right in (("dv", "b_p", "b_do"), ("dk", "b_ds", "b_q")):
+        s += (f"{i2}%{x}_e = tensor.empty() : {f([bn, bm])}\n"
+              f"{i2}%{x}_t = linalg.transpose ins(%{left} : {f([bm, bn])}) outs(%{x}_e : {f([bn, bm])}) permutation = [1, 0]\n"
+              f"{i2}%{x}_new = linalg.matmul ins(%{x}_t, %{right} : {f([bn, bm])}, {f([bm, hd])}) outs(%{x}_acc : {f([bn, hd])}) -> {f([bn, hd])}\n")
+    s += f"{i2}scf.yield %dk_new, %dv_new : {f([bn, hd])}, {f([bn, hd])}\n{i1}}}\n"
+    s += finish("b_", "dk", [bn, hd], k3, "key_grad", "b_k0", "pid1", kvv, True)
+    s += finish("b_", "dv", [bn, hd], k3, "value_grad", "b_k0", "pid1", kvv, False)
+    return s + "    }\n    return\n  }\n}\n"

@@ -934,6 +934,12 @@ def _fused_statement(dev, st: Store, arena: ArenaMap, sid: int, row_shard):
     return stmt
 
 
+def _fused_stores(dev, stores: List[Store], arena: ArenaMap, sid: int):
+    """A fused kernel that runs several of the next stores: (statement, how many), or None."""
+    from .lower_rotary import try_lower_rotary
+    return try_lower_rotary(dev, stores, arena, sid)
+
+
 # A statement that stores one value per row made of its neighbour's row reductions joins that neighbour's launch.
 # (Switch for tests that want the stand-alone per-row statements.)
 FUSE_ROW_RESULTS = True
@@ -952,8 +958,20 @@ def lower(dev: R.Device, stores: List[Store], arena: ArenaMap, row_shard=None, f
     def per_row_program(s) -> bool:
         return s.kind == "row_program" and bool(s.args.out_per_row) and len(s.stores) == 1
 
-    for st in stores:
+    joined = 0                              # stores that a statement over several of them runs
+    for k, st in enumerate(stores):
+        if joined:
+            joined -= 1
+            continue
         sid = len(plan.statements)
+        if fused and merge and row_shard is None:
+            many = _fused_stores(dev, stores[k:], arena, sid)
+            if many is not None:
+                many[0].origin = st.origin
+                plan.statements.append(many[0])
+                groups.append(stores[k:k + many[1]])
+                joined = many[1] - 1
+                continue
         last = plan.statements[-1] if plan.statements else None
         if FUSE_ROW_RESULTS and last is not None and last.kind == "row_program" and not last.args.out_per_row and \
                 last.try_absorb(st):

@@ -134,6 +134,23 @@ class AttnArgs(C.Structure):
                 ("steps", C.c_int32), ("reserved", C.c_int32), ("scratch_bytes", C.c_int64)]
 
 
+ROTARY_TENSORS = 4
+
+
+class RotaryTensor(C.Structure):
+    _fields_ = [("heads", C.c_int32), ("rest", C.c_int32), ("in_token", C.c_int64), ("in_head", C.c_int64),
+                ("out_token", C.c_int64), ("out_head", C.c_int64), ("in_partner", C.c_int64), ("out_partner", C.c_int64),
+                ("in_rest", C.c_int64), ("out_rest", C.c_int64)]
+
+
+class RotaryArgs(C.Structure):
+    _fields_ = [("arena", C.c_void_p), ("dev_item_offsets", C.c_void_p), ("n_items", C.c_int64),
+                ("tokens", C.c_int32), ("pairs", C.c_int32), ("dtype", C.c_int32), ("idx_dtype", C.c_int32),
+                ("n_tensors", C.c_int32), ("inverse", C.c_int32), ("pos_stride", C.c_int64), ("pair_stride", C.c_int64),
+                ("table_stride", C.c_int64), ("cos_off", C.c_int64), ("sin_off", C.c_int64), ("cos_end", C.c_int64),
+                ("sin_end", C.c_int64), ("align", C.c_int32), ("reserved", C.c_int32), ("t", RotaryTensor * ROTARY_TENSORS)]
+
+
 G_MAXDIM = 6
 G_KINDS = {k: i for i, k in enumerate(["load", "addr", "idxadd", "gather", "constv", "fill", "param", "iota", "map",
                                        "ew", "redl", "matmul", "store", "scatter", "ringred", "table", "concat"])}
@@ -213,6 +230,7 @@ SYMBOLS = {
     "ktb_launch_generic": (C.c_int, [C.c_void_p, C.POINTER(GenOpArgs)]),
     "ktb_launch_gemm_f16": (C.c_int, [C.c_void_p, C.POINTER(GemmArgs)]),
     "ktb_launch_attention_fwd": (C.c_int, [C.c_void_p, C.POINTER(AttnArgs)]),
+    "ktb_launch_rotary": (C.c_int, [C.c_void_p, C.POINTER(RotaryArgs)]),
 }
 
 
