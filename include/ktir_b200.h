@@ -482,6 +482,52 @@ typedef struct {
 } ktb_attn_args;
 int ktb_launch_attention_fwd(ktb_ctx* ctx, const ktb_attn_args* args);
 
+/* ---- attention over whole sequences --------------------------------------------------------
+ * O = softmax(scale Q K^T) V over the keys that query i sees (all, or j <= i + causal_delta) and lse = log(sum(exp)) of its
+ * scaled scores, in f32; a row that sees none gives 0 and -inf.  The loop of ktb_launch_attention_fwd (running maximum, sum and
+ * accumulator per tile of keys, P rounded to f16) over keys and values that are tensors [kv_len][heads / kv_group][head_dim],
+ * of any length, instead of pages.  Offsets and strides in elements (f16: multiples of 8; lse f32 [queries][heads],
+ * lse_off < 0: not stored); head_dim 64 or 128. */
+typedef struct {
+    void* arena;
+    int64_t q_off, k_off, v_off, o_off, lse_off;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, lse_row, lse_head;
+    int32_t q_len, kv_len, heads, kv_group, head_dim;
+    int32_t causal, causal_delta;
+    float scale;
+} ktb_attn_dense_args;
+int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_args* args);
+
+/* ---- gradients of attention ---------------------------------------------------------------
+ * With S = scale Q K^T, P = exp(S - lse) where query i sees key j (all, or j <= i + causal_delta), 0 elsewhere, and
+ * D = rowsum(dO * O):  dS = P (dO V^T - D),  dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO, summed over the kv_group
+ * query heads that share a key head.  What a KTIR program computes that walks tiles of keys and of queries with
+ * linalg.matmul, exp and linalg.reduce (ktir_cpu/ops/arith_ops.py:323-340, ktir_cpu/dialects/linalg_ops.py:136-347).
+ * Tensors are [positions][heads][head_dim] f16 (lse f32 [queries][heads]) in the arena, by offset and strides in elements,
+ * the f16 ones multiples of 8; head_dim 64 or 128.  lse is the forward pass's (ktb_launch_attention_dense); where it is -inf
+ * the row has no probabilities.  P and dS are rounded to f16 before they are multiplied; the order of every sum is fixed.
+ * `want` says which gradients are stored; the dq_* ranges are of query rows and query heads, the dk_* ranges of key rows and
+ * key heads, and the rest of the outputs is left as it is.  dev_scratch (256-byte boundary) holds
+ * ktb_attention_bwd_scratch_bytes(args) bytes; launches that share it must be ordered. */
+enum { KTB_ATTN_DQ = 1, KTB_ATTN_DK = 2, KTB_ATTN_DV = 4 };
+typedef struct {
+    void* arena;
+    int64_t q_off, k_off, v_off, o_off, do_off, lse_off, dq_off, dk_off, dv_off;
+    int64_t q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head, do_row, do_head, lse_row, lse_head;
+    int64_t dq_row, dq_head, dk_row, dk_head, dv_row, dv_head;
+    int32_t q_len, kv_len, heads, kv_group, head_dim;
+    int32_t causal, causal_delta;
+    float scale;
+    int32_t want;
+    int32_t dq_row0, dq_rows, dq_head0, dq_heads;
+    int32_t dk_row0, dk_rows, dk_head0, dk_heads;
+    int32_t reserved;
+    void* dev_scratch;
+    int64_t scratch_bytes;
+} ktb_attn_bwd_args;
+int64_t ktb_attention_bwd_scratch_bytes(const ktb_attn_bwd_args* args);
+int ktb_launch_attention_bwd(ktb_ctx* ctx, const ktb_attn_bwd_args* args);
+
 /* ---- rotary positions -------------------------------------------------------------------
  * Pairs (x, y) of a head turned by an angle of the token's position p: x cos[p, j] - y sin[p, j] and
  * y cos[p, j] + x sin[p, j], products and sums in f32 one by one, rounded once to the tensors' type; `inverse` takes -sin.

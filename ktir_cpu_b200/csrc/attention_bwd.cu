@@ -1,0 +1,535 @@
+// Gradients of attention: with S = scale Q K^T, P = exp(S - lse) where a query sees a key, D = rowsum(dO * O),
+//   dS = P * (dO V^T - D),   dQ = scale dS K,   dK = scale dS^T Q,   dV = P^T dO.
+// It takes over the loops of a KTIR program that walks tiles of keys for dQ and tiles of queries for dK and dV
+// (linalg.matmul, exp, select and linalg.reduce per pair of tiles; ktir_cpu/ops/arith_ops.py:323-340,
+// ktir_cpu/dialects/linalg_ops.py:136-347).
+//
+// The tensor cores bound it: five products of 2 * 128 * 128 * head_dim operations per pair of 128-row tiles are needed.
+// Seven are made here: one kernel owns tiles of keys (S^T, dO V^T transposed, dV, dK), one tiles of queries (S, dO V^T, dQ),
+// so that every sum has one owner and one order, and no partial sum of dQ crosses HBM.
+//
+// Both kernels are the same loop.  A CTA holds two tiles of 128 rows X and Y (K and V, or Q and dO) in shared memory and
+// streams pairs of 64-row tiles X', Y' (Q and dO, or K and V) through a ring by TMA.  Per step one warp issues
+// S = X X'^T and T = Y Y'^T into one of two slots of TMEM (three for queries, which have one accumulator less); two threads
+// a row read them, 32 columns each, and write P and dS as f16 over the same columns; the next products take them from there
+// as their A operand: acc0 += dS X' and, for keys, acc1 += P Y'.  While one step is in the softmax, the tensor core has the
+// other slots'.
+//
+// f16 operands.  P is at most 1 but mostly near 1 / keys, dS is as small as the gradient: both are rounded to f16 (2^-12 of the
+// value on average, the only roundings before the results') after a shift by powers of two that keeps them in range:
+// P by 2^14, dS by 2^14 / B with B >= |dO V^T - D| a power of two from the norms of dO and V (per row for dQ, per key head
+// for dK, whose sums run over rows).  Sums, D and the statistics are f32.
+#include "tc_common.cuh"
+
+#define AB_M 128                   // rows that a CTA owns
+#define AB_N 64                    // rows of a step
+#define AB_SHIFT 14.f
+#define AB_LOG2E 1.4426950408889634f
+
+// ---- what the rows bring: 14 - lse / ln 2, D, |dO| per row, and the largest norms --------------------------------
+// One block takes 64 rows of one head, LANES = head_dim / 8 threads a row.  blockIdx.y counts blocks of queries, then of keys.
+struct ab_scratch {
+    float* neg_lse;                // [heads][padded queries]
+    float* d;
+    float* norm;
+    unsigned* most;                // [key heads][4]: bits of max |dO|, max |D|, max |V|
+    int64_t padded;
+};
+
+static __device__ __forceinline__ float ab_dot8(uint4 a, uint4 b) {
+    const __half2* x = reinterpret_cast<const __half2*>(&a);
+    const __half2* y = reinterpret_cast<const __half2*>(&b);
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 u = __half22float2(x[i]), v = __half22float2(y[i]);
+        s = fmaf(u.x, v.x, s);
+        s = fmaf(u.y, v.y, s);
+    }
+    return s;
+}
+
+template <int HD>
+__global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_bwd_args a, const ab_scratch w, int q_blocks) {
+    constexpr int LANES = HD / 8, ROWS = 256 / LANES;
+    const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
+    const int grp = a.kv_group;
+    const __half* base = reinterpret_cast<const __half*>(a.arena);
+    float most_a = 0.f, most_d = 0.f;
+    const bool keys = (int)blockIdx.y >= q_blocks;
+    const int64_t row0 = (int64_t)(keys ? blockIdx.y - q_blocks : blockIdx.y) * 64;
+    const int head = blockIdx.x;
+    if (keys && head >= a.heads / grp) return;
+#pragma unroll
+    for (int i = 0; i < 64; i += ROWS) {
+        const int64_t row = row0 + i + r0;
+        if (keys) {
+            float v2 = 0.f;
+            if (row < a.kv_len) {
+                const uint4 v = *reinterpret_cast<const uint4*>(base + a.v_off + row * a.v_row + (int64_t)head * a.v_head + lane * 8);
+                v2 = ab_dot8(v, v);
+            }
+#pragma unroll
+            for (int o = LANES / 2; o; o >>= 1) v2 += __shfl_xor_sync(0xffffffffu, v2, o);
+            if (v2 <= 3.0e38f) most_a = fmaxf(most_a, v2);              // (a row with an infinity has no say)
+            continue;
+        }
+        float d = 0.f, g2 = 0.f;
+        if (row < a.q_len) {
+            const uint4 g = *reinterpret_cast<const uint4*>(base + a.do_off + row * a.do_row + (int64_t)head * a.do_head + lane * 8);
+            const uint4 o = *reinterpret_cast<const uint4*>(base + a.o_off + row * a.o_row + (int64_t)head * a.o_head + lane * 8);
+            d = ab_dot8(g, o);
+            g2 = ab_dot8(g, g);
+        }
+#pragma unroll
+        for (int o = LANES / 2; o; o >>= 1) {
+            d += __shfl_xor_sync(0xffffffffu, d, o);
+            g2 += __shfl_xor_sync(0xffffffffu, g2, o);
+        }
+        if (lane == 0) {
+            float nl = -INFINITY;                                       // no probability: rows past the end, rows that see nothing
+            if (row < a.q_len) {
+                const float lse = (reinterpret_cast<const float*>(a.arena) + a.lse_off)[row * a.lse_row + (int64_t)head * a.lse_head];
+                if (lse != -INFINITY) nl = fmaf(-lse, AB_LOG2E, AB_SHIFT);
+            }
+            const int64_t at = (int64_t)head * w.padded + row;
+            w.neg_lse[at] = nl;
+            w.d[at] = d;
+            w.norm[at] = g2 <= 3.0e38f ? sqrtf(g2) : 0.f;
+        }
+        if (g2 <= 3.0e38f) most_a = fmaxf(most_a, g2);
+        if (fabsf(d) <= 3.0e38f) most_d = fmaxf(most_d, fabsf(d));
+    }
+    // largest of the block, one atomic each: a maximum does not depend on the order
+    __shared__ float sa[8], sd[8];
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        most_a = fmaxf(most_a, __shfl_xor_sync(0xffffffffu, most_a, o));
+        most_d = fmaxf(most_d, __shfl_xor_sync(0xffffffffu, most_d, o));
+    }
+    if ((threadIdx.x & 31) == 0) {
+        sa[threadIdx.x >> 5] = most_a;
+        sd[threadIdx.x >> 5] = most_d;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+        float m = 0.f;
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, threadIdx.x ? sd[i] : sa[i]);
+        unsigned* to = w.most + (keys ? head : head / grp) * 4;
+        if (threadIdx.x == 0) atomicMax(to + (keys ? 2 : 0), __float_as_uint(sqrtf(m)));
+        else if (!keys) atomicMax(to + 1, __float_as_uint(m));
+    }
+}
+
+// A power of two s with |x| s <= 1 for |x| <= bound.
+static __device__ __forceinline__ float ab_shrink(float bound) {
+    const int e = (int)((__float_as_uint(bound) >> 23) & 255) - 127;            // bound < 2^(e + 1)
+    if (!(bound > 0.f) || e < -120) return bound > 0.f ? 0x1p100f : 1.f;
+    return __uint_as_float((unsigned)(127 - (e + 1)) << 23);
+}
+
+// ---- the two kernels -----------------------------------------------------------------------------------------------
+template <int HD>
+struct ab_shape {
+    static constexpr int BLOCKS = HD / 64;                  // 64-column blocks of a tile (a 128-byte swizzled row each)
+    static constexpr int OWN = AB_M * HD * 2;               // bytes of X, of Y
+    static constexpr int STEP = AB_N * HD * 2;              // bytes of X', of Y'
+    static constexpr int STAGES = 4;
+    static constexpr size_t SMEM = 2 * OWN + STAGES * (2 * STEP + 2 * AB_N * 4) + 1024 + 256;
+};
+
+// Waits for a phase no matter what else has failed, so that no copy is under way into memory that the CTA gives up.
+static __device__ void ab_drain(uint64_t* bar, uint32_t parity) {
+    const long long start = clock64();
+    while (!tc_mbar_try_wait(bar, parity))
+        if (clock64() - start > 1000000000ll) return;
+}
+
+template <int HD, bool KEYS>
+__global__ void __launch_bounds__(384, 1)
+ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
+                         const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ys,
+                         const ktb_attn_bwd_args a, const ab_scratch w, int row_tiles, int heads_here, int by_head, ktb_status* st) {
+    typedef ab_shape<HD> Z;
+    constexpr int SLOTS = KEYS ? 2 : 3;                     // S and T, 64 columns of TMEM each
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sX = smem;
+    uint8_t* sY = sX + Z::OWN;
+    uint8_t* ring = sY + Z::OWN;                            // per stage X', then Y'
+    float* sRow = reinterpret_cast<float*>(ring + Z::STAGES * 2 * Z::STEP);     // KEYS: per stage 64 x (14 - lse / ln 2), 64 x D
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + Z::STAGES * 2 * AB_N);
+    uint64_t *full = bars, *empty = bars + Z::STAGES, *own = bars + 2 * Z::STAGES, *s_full = own + 1, *p_full = s_full + SLOTS, *done = p_full + SLOTS;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    const int grp = a.kv_group;
+
+    // The CTA's tile, longest walks first: of all heads (few tiles, so that the long ones do not come last), or head by head
+    // (so that the CTAs at work share their stream in L2).
+    const int tile_order = by_head ? blockIdx.x % row_tiles : blockIdx.x / heads_here;
+    const int head_here = by_head ? blockIdx.x / row_tiles : blockIdx.x % heads_here;
+    const int tile = KEYS ? tile_order : row_tiles - 1 - tile_order;            // causal: early keys, late queries
+    const int row0 = (KEYS ? a.dk_row0 : a.dq_row0) + tile * AB_M;
+    const int row_end = KEYS ? a.dk_row0 + a.dk_rows : a.dq_row0 + a.dq_rows;
+    const int head = (KEYS ? a.dk_head0 : a.dq_head0) + head_here;              // KEYS: key head; else query head
+    // steps: `per_head` tiles of 64 streamed rows from first * 64 on; for keys once for every query head of the group
+    int first = 0, per_head;
+    if (KEYS) {
+        per_head = (a.q_len + AB_N - 1) / AB_N;
+        if (a.causal) {
+            const long long q = (long long)row0 - a.causal_delta;               // the first query that sees key row0
+            first = q <= 0 ? 0 : q >= a.q_len ? per_head : (int)(q / AB_N);
+        }
+        per_head -= first;
+    } else {
+        per_head = (a.kv_len + AB_N - 1) / AB_N;
+        if (a.causal) {
+            const int last_row = row0 + AB_M - 1 < a.q_len - 1 ? row0 + AB_M - 1 : a.q_len - 1;
+            const long long k = (long long)last_row + a.causal_delta;           // the last key that the tile sees
+            const long long n = k < 0 ? 0 : k / AB_N + 1;
+            if (n < per_head) per_head = (int)n;
+        }
+    }
+    const int n = KEYS ? per_head * grp : per_head;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < Z::STAGES; ++i) {
+            tc_mbar_init(&full[i], 1);
+            tc_mbar_init(&empty[i], 1);
+        }
+        tc_mbar_init(own, 1);
+        for (int i = 0; i < SLOTS; ++i) {
+            tc_mbar_init(&s_full[i], 1);
+            tc_mbar_init(&p_full[i], 8);
+        }
+        tc_mbar_init(done, 1);
+        *abort_flag = 0;
+        tc_fence_barrier_init();
+    }
+    __syncthreads();
+    if (warp == 1) tc_tmem_alloc(tmem_slot, 512);
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+    const uint32_t t_acc0 = tmem, t_acc1 = tmem + 128, t_slot = tmem + (KEYS ? 256 : 128);      // slot i: S at 128 i, T at 128 i + 64
+
+    if (warp == 0) {
+        if (lane == 0 && n > 0) {
+            tc_prefetch_tmap(&map_x);
+            tc_prefetch_tmap(&map_xs);
+            tc_prefetch_tmap(&map_y);
+            tc_prefetch_tmap(&map_ys);
+            tc_mbar_expect_tx(own, 2 * Z::OWN);
+#pragma unroll
+            for (int b = 0; b < Z::BLOCKS; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    tc_tma_load_3d(sX + b * (AB_M * 128) + h * (AB_N * 128), &map_x, own, b * 64, head, row0 + h * AB_N);
+                    tc_tma_load_3d(sY + b * (AB_M * 128) + h * (AB_N * 128), &map_y, own, b * 64, head, row0 + h * AB_N);
+                }
+            int loaded = 0;
+            for (int i = 0; i < n; ++i) {
+                const int stage = i % Z::STAGES;
+                if (!tc_mbar_wait(&empty[stage], ((i / Z::STAGES) & 1) ^ 1, abort_flag, st, 61)) break;
+                const int sh = KEYS ? head * grp + i / per_head : head / grp;   // streamed head
+                const int r = (first + (KEYS ? i % per_head : i)) * AB_N;
+                uint8_t* to = ring + stage * 2 * Z::STEP;
+                tc_mbar_expect_tx(&full[stage], 2 * Z::STEP + (KEYS ? 2 * AB_N * 4 : 0));
+#pragma unroll
+                for (int b = 0; b < Z::BLOCKS; ++b) {
+                    tc_tma_load_3d(to + b * (AB_N * 128), &map_xs, &full[stage], b * 64, sh, r);
+                    tc_tma_load_3d(to + Z::STEP + b * (AB_N * 128), &map_ys, &full[stage], b * 64, sh, r);
+                }
+                if (KEYS) {
+                    float* rows = sRow + stage * 2 * AB_N;
+                    tc_bulk_load(rows, w.neg_lse + (int64_t)sh * w.padded + r, &full[stage], AB_N * 4);
+                    tc_bulk_load(rows + AB_N, w.d + (int64_t)sh * w.padded + r, &full[stage], AB_N * 4);
+                }
+                loaded = i + 1;
+            }
+            if (*abort_flag) {
+                ab_drain(own, 0);
+                for (int i = loaded > Z::STAGES ? loaded - Z::STAGES : 0; i < loaded; ++i) ab_drain(&full[i % Z::STAGES], (i / Z::STAGES) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        // the warp runs this converged; one elected lane issues the tcgen05 instructions
+        const uint32_t lead = tc_elect_one();
+        const uint32_t idesc_s = tc_idesc_f16(AB_M, AB_N, 0, 0), idesc_a = tc_idesc_f16(AB_M, HD, 0, 1);
+        const uint64_t xd = tc_smem_desc(tc_smem_u32(sX), 16, 1024), yd = tc_smem_desc(tc_smem_u32(sY), 16, 1024);
+        const uint32_t ring_at = tc_smem_u32(ring);
+        auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
+            const bool ok = __all_sync(0xffffffffu, tc_mbar_wait(bar, parity, abort_flag, st, site)) != 0;
+            tc_fence_after_sync();
+            return ok;
+        };
+        auto scores = [&](int i) {                              // S and T of step i
+            const uint32_t at = ring_at + (i % Z::STAGES) * 2 * Z::STEP, d = t_slot + (i % SLOTS) * 128;
+            const uint64_t xs = tc_smem_desc(at, 16, 1024), ys = tc_smem_desc(at + Z::STEP, 16, 1024);
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t ao = ((kk >> 2) * (AB_M * 128) + (kk & 3) * 32) >> 4, bo = ((kk >> 2) * (AB_N * 128) + (kk & 3) * 32) >> 4;
+                tc_mma_f16_p(d, xd + ao, xs + bo, idesc_s, kk != 0, lead);
+            }
+#pragma unroll
+            for (int kk = 0; kk < HD / 16; ++kk) {
+                const uint32_t ao = ((kk >> 2) * (AB_M * 128) + (kk & 3) * 32) >> 4, bo = ((kk >> 2) * (AB_N * 128) + (kk & 3) * 32) >> 4;
+                tc_mma_f16_p(d + 64, yd + ao, ys + bo, idesc_s, kk != 0, lead);
+            }
+            tc_mma_commit_p(&s_full[i % SLOTS], lead);
+        };
+        auto sums = [&](int i) {                                // the accumulators take step i; its stage is free then
+            const uint32_t at = ring_at + (i % Z::STAGES) * 2 * Z::STEP, p = t_slot + (i % SLOTS) * 128;
+            const uint64_t xs = tc_smem_desc(at, AB_N * 128, 1024), ys = tc_smem_desc(at + Z::STEP, AB_N * 128, 1024);
+            if (KEYS) {
+#pragma unroll
+                for (int kk = 0; kk < AB_N / 16; ++kk)
+                    tc_mma_f16_ts_p(t_acc1, p + (kk >> 1) * 32 + (kk & 1) * 8, ys + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u, lead);
+            }
+#pragma unroll
+            for (int kk = 0; kk < AB_N / 16; ++kk)
+                tc_mma_f16_ts_p(t_acc0, p + 64 + (kk >> 1) * 32 + (kk & 1) * 8, xs + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u, lead);
+            tc_mma_commit_p(&empty[i % Z::STAGES], lead);
+        };
+        bool ok = n > 0 && wait(own, 0, 62);
+        for (int i = 0; i < SLOTS && i < n && ok; ++i) {
+            ok = wait(&full[i % Z::STAGES], (i / Z::STAGES) & 1, 63);
+            if (ok) scores(i);
+        }
+        for (int i = 0; i < n && ok; ++i) {
+            ok = wait(&p_full[i % SLOTS], (i / SLOTS) & 1, 64);
+            if (!ok) break;
+            sums(i);
+            if (const int k = i + SLOTS; k < n) {
+                // (the tensor core runs one thread's products in their order: the slot has been read by then)
+                ok = wait(&full[k % Z::STAGES], (k / Z::STAGES) & 1, 65);
+                if (ok) scores(k);
+            }
+        }
+        if (ok) tc_mma_commit_p(done, lead);
+    } else if (warp >= 4) {
+        const int half = (warp - 4) >> 2;                       // which 32 columns of a step are this warpgroup's
+        const int r = (warp & 3) * 32 + lane;                   // row of the tile == TMEM lane
+        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t at0 = t_slot + lane_off + half * 32;
+        const int row = row0 + r;
+        const float sl = a.scale * AB_LOG2E;
+        const int kvh = KEYS ? head : head / grp;
+        const float most_v = __uint_as_float(w.most[kvh * 4 + 2]);
+        float shrink, row_nl = 0.f, row_d = 0.f;
+        if (KEYS) {
+            shrink = ab_shrink(__uint_as_float(w.most[kvh * 4]) * most_v + __uint_as_float(w.most[kvh * 4 + 1]));
+        } else {
+            const bool live = row < a.q_len;
+            const int64_t at_row = (int64_t)head * w.padded + row;
+            row_nl = live ? w.neg_lse[at_row] : -INFINITY;
+            row_d = live ? w.d[at_row] : 0.f;
+            shrink = ab_shrink((live ? w.norm[at_row] : 0.f) * most_v + fabsf(row_d));
+        }
+        const uint64_t sl2 = at_pack2(sl, sl), shrink2 = at_pack2(shrink, shrink);
+        const uint64_t row_nl2 = at_pack2(row_nl, row_nl), row_d2 = at_pack2(-row_d, -row_d);
+        bool ok = true;
+        for (int i = 0; i < n; ++i) {
+            const int slot = i % SLOTS;
+            const uint32_t at = at0 + slot * 128;
+            const int s0 = (first + (KEYS ? i % per_head : i)) * AB_N;          // first streamed row of the step
+            // columns [lo, hi) of this thread's are visible
+            int lo = 0, hi = 32;
+            bool masked = false;
+            if (KEYS) {
+                if (a.causal && (long long)row0 + AB_M - 1 > (long long)s0 + a.causal_delta) {
+                    const long long l = (long long)row - a.causal_delta - s0 - half * 32;
+                    lo = l < 0 ? 0 : l > 32 ? 32 : (int)l;
+                    masked = true;
+                }
+            } else {
+                if (s0 + AB_N > a.kv_len || (a.causal && (long long)s0 + AB_N - 1 > (long long)row0 + a.causal_delta)) {
+                    long long h = (long long)a.kv_len - s0;
+                    if (a.causal && (long long)row + a.causal_delta + 1 - s0 < h) h = (long long)row + a.causal_delta + 1 - s0;
+                    h -= half * 32;
+                    hi = h < 0 ? 0 : h > 32 ? 32 : (int)h;
+                    masked = true;
+                }
+            }
+            const float4* nl4 = reinterpret_cast<const float4*>(sRow + (i % Z::STAGES) * 2 * AB_N + half * 32);
+            const float4* d4 = nl4 + AB_N / 4;
+            bool there = tc_mbar_wait(&s_full[slot], (i / SLOTS) & 1, abort_flag, st, 66);
+            if (KEYS) there = there && tc_mbar_wait(&full[i % Z::STAGES], (i / Z::STAGES) & 1, abort_flag, st, 68);   // (the copies into sRow)
+            if (!__all_sync(0xffffffffu, there)) {
+                ok = false;
+                break;
+            }
+            tc_fence_after_sync();
+            uint32_t s[32], t[32];
+            tc_tmem_ld32(at, s);
+            tc_tmem_ld32(at + 64, t);
+            tc_tmem_ld_wait();
+            if (masked) {
+#pragma unroll
+                for (int j = 0; j < 32; ++j)
+                    if (j < lo || j >= hi) s[j] = 0xff800000u;                  // exp2 makes it a zero
+            }
+            uint32_t p16[16], s16[16];
+#pragma unroll
+            for (int j = 0; j < 32; j += 4) {
+                uint64_t nl2[2] = {row_nl2, row_nl2}, d2[2] = {row_d2, row_d2};
+                if (KEYS) {
+                    const float4 f = nl4[j >> 2], g = d4[j >> 2];
+                    nl2[0] = at_pack2(f.x, f.y), nl2[1] = at_pack2(f.z, f.w);
+                    d2[0] = at_pack2(-g.x, -g.y), d2[1] = at_pack2(-g.z, -g.w);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int k = j + 2 * e;
+                    float x0, x1, y0, y1;
+                    at_unpack2(at_fma2(at_pack2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), sl2, nl2[e]), x0, x1);
+                    const float p0 = at_ex2(x0), p1 = at_ex2(x1);
+                    const uint64_t diff = at_add2(at_pack2(__uint_as_float(t[k]), __uint_as_float(t[k + 1])), d2[e]);
+                    at_unpack2(at_mul2(at_mul2(diff, shrink2), at_pack2(p0, p1)), y0, y1);
+                    const __half2 hp = __floats2half2_rn(p0, p1), hs = __floats2half2_rn(y0, y1);
+                    p16[k >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
+                    s16[k >> 1] = *reinterpret_cast<const uint32_t*>(&hs);
+                }
+            }
+            // over the columns that this warpgroup has read: those of the other one may still be waited for
+            if (KEYS) tc_tmem_st16(at, p16);
+            tc_tmem_st16(at + 64, s16);
+            tc_tmem_st_wait();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) tc_mbar_arrive(&p_full[slot]);
+        }
+        if (ok && n > 0) ok = __all_sync(0xffffffffu, tc_mbar_wait(done, 0, abort_flag, st, 67)) != 0;
+        tc_fence_after_sync();
+        // results: keys: the first warpgroup dK, the second dV; queries: half of the columns of dQ each
+        const bool store = ok && row < row_end && *abort_flag == 0;
+        const float back = 0x1p-14f;
+        const bool of_v = KEYS && half == 1;
+        const int want = KEYS ? (of_v ? a.want & KTB_ATTN_DV : a.want & KTB_ATTN_DK) : a.want & KTB_ATTN_DQ;
+        const int64_t off = !KEYS ? a.dq_off + (int64_t)row * a.dq_row + (int64_t)head * a.dq_head
+                          : of_v  ? a.dv_off + (int64_t)row * a.dv_row + (int64_t)head * a.dv_head
+                                  : a.dk_off + (int64_t)row * a.dk_row + (int64_t)head * a.dk_head;
+        const float factor = of_v ? back : a.scale * (back / shrink);
+        constexpr int COLS = KEYS ? HD : HD / 2;
+        const int col0 = KEYS ? 0 : half * (HD / 2);
+        __half* dst = reinterpret_cast<__half*>(a.arena) + off + col0;
+        const uint32_t from = (of_v ? t_acc1 : t_acc0) + lane_off + col0;
+#pragma unroll
+        for (int c = 0; c < COLS; c += 32) {
+            uint32_t v[32];
+            if (n > 0 && ok) {                              // (the same for the whole warp)
+                tc_tmem_ld32(from + c, v);
+                tc_tmem_ld_wait();
+            } else {
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = 0;
+            }
+            if (store && want) {
+#pragma unroll
+                for (int j = 0; j < 32; j += 8) {
+                    uint4 o;
+                    __half2* h = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        h[e] = __floats2half2_rn(__uint_as_float(v[j + 2 * e]) * factor, __uint_as_float(v[j + 2 * e + 1]) * factor);
+                    *reinterpret_cast<uint4*>(dst + c + j) = o;
+                }
+            }
+        }
+        tc_fence_before_sync();
+    }
+    __syncthreads();
+    if (warp == 1) tc_tmem_dealloc(tmem, 512);
+}
+
+// Tensor [rows][heads][HD] in boxes of 64 rows x 64 columns of one head.
+static bool ab_map(CUtensorMap* m, const ktb_attn_bwd_args& a, int64_t off, int64_t rows, int64_t heads, int64_t row, int64_t head) {
+    const uint64_t dims[3] = {(uint64_t)a.head_dim, (uint64_t)heads, (uint64_t)rows};
+    const uint64_t str[2] = {(uint64_t)head * 2, (uint64_t)row * 2};
+    const uint32_t box[3] = {64, 1, AB_N};
+    return tc_make_map_f16(m, reinterpret_cast<__half*>(a.arena) + off, 3, dims, str, box);
+}
+
+static int64_t ab_padded(const ktb_attn_bwd_args& a) { return ((int64_t)a.q_len + AB_N - 1) / AB_N * AB_N; }
+
+extern "C" int64_t ktb_attention_bwd_scratch_bytes(const ktb_attn_bwd_args* args) {
+    if (!args || args->kv_group < 1 || args->heads < 1 || args->q_len < 1) return 0;
+    return (int64_t)(args->heads / args->kv_group) * 16 + 256 + 3 * 4 * (int64_t)args->heads * ab_padded(*args);
+}
+
+template <int HD, bool KEYS>
+static int ab_launch(ktb_ctx* ctx, const ktb_attn_bwd_args& a, const ab_scratch& w, const CUtensorMap& mq, const CUtensorMap& mk,
+                     const CUtensorMap& mv, const CUtensorMap& mg) {
+    const int rows = KEYS ? a.dk_rows : a.dq_rows, heads = KEYS ? a.dk_heads : a.dq_heads;
+    if (rows <= 0 || heads <= 0) return KTB_OK;
+    static bool attr_set[KTB_MAX_DEVICES] = {};     // the attribute is per device
+    if (!attr_set[ctx->device & (KTB_MAX_DEVICES - 1)]) {
+        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
+        attr_set[ctx->device & (KTB_MAX_DEVICES - 1)] = true;
+    }
+    const int tiles = (rows + AB_M - 1) / AB_M;
+    const long long items = (long long)tiles * heads;
+    if (items > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many tiles");
+    const int by_head = items >= 8ll * ctx->sm_count;
+    if (KEYS)
+        ktb_attention_bwd_kernel<HD, true><<<(int)items, 384, ab_shape<HD>::SMEM, ctx->stream>>>(mk, mv, mq, mg, a, w, tiles, heads, by_head, ctx->dev_status);
+    else
+        ktb_attention_bwd_kernel<HD, false><<<(int)items, 384, ab_shape<HD>::SMEM, ctx->stream>>>(mq, mg, mk, mv, a, w, tiles, heads, by_head, ctx->dev_status);
+    KTB_CHECK_LAUNCH(ctx, "ktb_attention_bwd_kernel");
+    return KTB_OK;
+}
+
+template <int HD>
+static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
+    const int kv_heads = a.heads / a.kv_group;
+    ab_scratch w;
+    w.padded = ab_padded(a);
+    w.most = reinterpret_cast<unsigned*>(a.dev_scratch);
+    w.neg_lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.dev_scratch) + ((int64_t)kv_heads * 16 + 255) / 256 * 256);
+    w.d = w.neg_lse + (int64_t)a.heads * w.padded;
+    w.norm = w.d + (int64_t)a.heads * w.padded;
+    CUtensorMap mq, mk, mv, mg;
+    if (!ab_map(&mq, a, a.q_off, a.q_len, a.heads, a.q_row, a.q_head) || !ab_map(&mg, a, a.do_off, a.q_len, a.heads, a.do_row, a.do_head) ||
+        !ab_map(&mk, a, a.k_off, a.kv_len, kv_heads, a.k_row, a.k_head) || !ab_map(&mv, a, a.v_off, a.kv_len, kv_heads, a.v_row, a.v_head))
+        return ktb_fail(ctx, KTB_E_CUDA, "attention_bwd", "cuTensorMapEncodeTiled failed");
+    KTB_CUDA(ctx, cudaMemsetAsync(w.most, 0, (size_t)kv_heads * 16, ctx->stream));
+    const int q_blocks = (a.q_len + 63) / 64, k_blocks = (a.kv_len + 63) / 64;
+    if (q_blocks + k_blocks > 65535) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "more than 2^21 positions");
+    ktb_attention_rows_kernel<HD><<<dim3(a.heads, q_blocks + k_blocks), 256, 0, ctx->stream>>>(a, w, q_blocks);
+    KTB_CHECK_LAUNCH(ctx, "ktb_attention_rows_kernel");
+    if (a.want & (KTB_ATTN_DK | KTB_ATTN_DV))
+        if (int rc = ab_launch<HD, true>(ctx, a, w, mq, mk, mv, mg)) return rc;
+    if (a.want & KTB_ATTN_DQ)
+        if (int rc = ab_launch<HD, false>(ctx, a, w, mq, mk, mv, mg)) return rc;
+    return KTB_OK;
+}
+
+extern "C" int ktb_launch_attention_bwd(ktb_ctx* ctx, const ktb_attn_bwd_args* args) {
+    if (!ctx || !args) return KTB_E_ARG;
+    const ktb_attn_bwd_args& a = *args;
+    const char* me = "attention_bwd";
+    if (a.head_dim != 64 && a.head_dim != 128) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "head_dim must be 64 or 128");
+    if (a.q_len < 0 || a.kv_len < 0 || a.heads < 0 || a.kv_group < 1 || a.heads % a.kv_group)
+        return ktb_fail(ctx, KTB_E_ARG, me, "lengths, heads or kv_group");
+    if ((a.want & ~7) || a.want == 0) return ktb_fail(ctx, KTB_E_ARG, me, "which gradients are wanted");
+    if (a.q_len == 0 || a.kv_len == 0 || a.heads == 0) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "no queries, keys or heads");
+    if (a.q_len > (1 << 30) || a.kv_len > (1 << 30) || a.heads > 65535 * 32) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "lengths or heads");
+    if (!(fabsf(a.scale) <= 3.0e38f)) return ktb_fail(ctx, KTB_E_ARG, me, "score scale must be finite");
+    const int kv_heads = a.heads / a.kv_group;
+    if (a.want & KTB_ATTN_DQ)
+        if (a.dq_row0 < 0 || a.dq_rows < 0 || a.dq_rows > a.q_len - a.dq_row0 || a.dq_head0 < 0 || a.dq_heads < 0 || a.dq_heads > a.heads - a.dq_head0)
+            return ktb_fail(ctx, KTB_E_ARG, me, "rows or heads of dQ outside the tensors");
+    if (a.want & (KTB_ATTN_DK | KTB_ATTN_DV))
+        if (a.dk_row0 < 0 || a.dk_rows < 0 || a.dk_rows > a.kv_len - a.dk_row0 || a.dk_head0 < 0 || a.dk_heads < 0 || a.dk_heads > kv_heads - a.dk_head0)
+            return ktb_fail(ctx, KTB_E_ARG, me, "rows or heads of dK and dV outside the tensors");
+    const int64_t all = a.q_off | a.k_off | a.v_off | a.o_off | a.do_off | a.q_row | a.q_head | a.k_row | a.k_head | a.v_row | a.v_head |
+                        a.o_row | a.o_head | a.do_row | a.do_head | ((a.want & KTB_ATTN_DQ) ? a.dq_off | a.dq_row | a.dq_head : 0) |
+                        ((a.want & KTB_ATTN_DK) ? a.dk_off | a.dk_row | a.dk_head : 0) | ((a.want & KTB_ATTN_DV) ? a.dv_off | a.dv_row | a.dv_head : 0);
+    if ((all & 7) || (reinterpret_cast<uintptr_t>(a.arena) & 15))
+        return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "strides and offsets must be multiples of 8 elements");
+    if (!a.dev_scratch || (reinterpret_cast<uintptr_t>(a.dev_scratch) & 255) || a.scratch_bytes < ktb_attention_bwd_scratch_bytes(args))
+        return ktb_fail(ctx, KTB_E_ARG, me, "scratch too small or not on a 256-byte boundary");
+    return a.head_dim == 64 ? ab_run<64>(ctx, a) : ab_run<128>(ctx, a);
+}

@@ -31,7 +31,6 @@
 
 #define AT_BM 128
 #define AT_D 128
-#define AT_Q_BYTES (AT_BM * AT_D * 2)
 #define AT_MAX_STAGES 8
 #define AT_RESCALE_GAP 8.0f
 
@@ -43,58 +42,11 @@ static __device__ __forceinline__ void at_tma_load_4d(void* smem_dst, const CUte
         : "memory");
 }
 
-static __device__ __forceinline__ float at_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 static __device__ __forceinline__ float at_max3(float a, float b, float c) {
     float r;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// two f32 lanes in one 64-bit register: Blackwell issues fma / add on such pairs as one instruction
-static __device__ __forceinline__ uint64_t at_pack2(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-static __device__ __forceinline__ void at_unpack2(uint64_t v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-static __device__ __forceinline__ uint64_t at_fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-static __device__ __forceinline__ uint64_t at_add2(uint64_t a, uint64_t b) {
-    uint64_t r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-
-// 2^x for two values at once on the FMA pipe (the exp unit is the busiest unit of the softmax):
-// x = r + f with r = round(x), 2^f by a cubic on [-0.5, 0.5] (relative error 7.5e-5, a sixth of
-// an f16 ulp), 2^r by an add into the exponent field.  x is clamped to >= -125 so that the
-// exponent stays positive (such a term is zero in f16 either way).
-static __device__ __forceinline__ void at_ex2_poly2(float x0, float x1, float& p0, float& p1) {
-    const float magic = 12582912.f;                     // 1.5 * 2^23: the sum keeps round(x) in the low mantissa bits
-    const uint64_t x2 = at_pack2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
-    const uint64_t t2 = at_add2(x2, at_pack2(magic, magic));
-    const uint64_t r2 = at_add2(t2, at_pack2(-magic, -magic));
-    const uint64_t f2 = at_fma2(r2, at_pack2(-1.f, -1.f), x2);
-    uint64_t q2 = at_fma2(at_pack2(0.05517164617776871f, 0.05517164617776871f), f2,
-                          at_pack2(0.2426111251115799f, 0.2426111251115799f));
-    q2 = at_fma2(q2, f2, at_pack2(0.6932609677314758f, 0.6932609677314758f));
-    q2 = at_fma2(q2, f2, at_pack2(0.9999280571937561f, 0.9999280571937561f));
-    float q0, q1, t0, t1;
-    at_unpack2(q2, q0, q1);
-    at_unpack2(t2, t0, t1);
-    p0 = __int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23));
-    p1 = __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23));
-}
-
 // Maximum of CW raw scores.
 template <int CW>
 static __device__ __forceinline__ float at_chunk_max(const uint32_t (&v)[CW], float mx) {
@@ -118,7 +70,7 @@ static __device__ __forceinline__ float at_chunk_max(const uint32_t (&v)[CW], fl
 // POLY of every 4 pairs take the polynomial instead of the exp unit.  A score of -inf (a masked
 // column) gives 0 on either path (the polynomial clamps it to 2^-125, which is 0 in f16 and
 // vanishes in the sum).
-template <int CW, int POLY>
+template <int CW, int POLY, bool FINE>
 static __device__ __forceinline__ void at_chunk_prob(const uint32_t (&v)[CW], float sl, float m, uint64_t& acc2,
                                                      uint32_t (&packed)[CW / 2]) {
     const uint64_t sl2 = at_pack2(sl, sl), nm2 = at_pack2(-m, -m);
@@ -128,7 +80,7 @@ static __device__ __forceinline__ void at_chunk_prob(const uint32_t (&v)[CW], fl
         at_unpack2(at_fma2(at_pack2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), sl2, nm2), x0, x1);
         float p0, p1;
         if (((i >> 1) & 3) < POLY) {
-            at_ex2_poly2(x0, x1, p0, p1);
+            at_ex2_poly2<FINE>(x0, x1, p0, p1);
         } else {
             p0 = at_ex2(x0);
             p1 = at_ex2(x1);
@@ -158,12 +110,22 @@ enum { B_QFULL = 0, B_QFREE = 2, B_KVFULL = 4, B_KVEMPTY = B_KVFULL + AT_MAX_STA
 // point of it: the Q tiles and first K/V pages of the next sub-item are fetched while the last steps
 // of the current one run, and its first scores are computed while the softmax warps normalise and
 // store the output, so a tile pair no longer pays a start-up and a drain of its own.
-template <int BN, int TPR, int POLY>
+//
+// DENSE: keys and values are rows of one tensor instead of pages, a.num_tiles groups of BN of them of which d.kv_len exist;
+// rows that see nothing give 0, and the log-sum-exp of every row is kept.
+struct at_dense {
+    float* lse;                 // null: not wanted
+    int64_t row, head;
+    int kv_len;
+};
+
+template <int BN, int TPR, int POLY, int HD, bool DENSE>
 __global__ void __launch_bounds__(128 + 256 * TPR, 1)
 ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                         const __grid_constant__ CUtensorMap map_v, const ktb_attn_args a, int q_pairs,
-                         int n_items, ktb_status* st) {
-    constexpr int KV_BYTES = BN * AT_D * 2;            // one K or V page in shared memory
+                         const __grid_constant__ CUtensorMap map_v, const ktb_attn_args a, const at_dense d,
+                         int q_pairs, int n_items, ktb_status* st) {
+    constexpr int Q_BYTES = AT_BM * HD * 2;
+    constexpr int KV_BYTES = BN * HD * 2;              // one K or V page in shared memory
     constexpr int AT_STAGES = BN == 128 ? 4 : 8;       // ring slots: 128 KB (64 KB for 32-row pages)
     constexpr int KV_BLK = BN * 128;                   // bytes of one [BN x 64] block
     constexpr int SB = BN > 64 ? 64 : BN;              // kv rows of one step (a page is NSUB steps)
@@ -171,7 +133,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sQ = smem;                                // 2 tiles x 2 blocks [128 x 64]
-    uint8_t* sKV = sQ + 2 * AT_Q_BYTES;                // ring of K / V pages
+    uint8_t* sKV = sQ + 2 * Q_BYTES;                // ring of K / V pages
     float* xbuf = reinterpret_cast<float*>(sKV + AT_STAGES * KV_BYTES);   // [2 tiles][2 parities][2 halves][128 rows]
     uint64_t* bars = reinterpret_cast<uint64_t*>(xbuf + 2 * 2 * 2 * AT_BM);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
@@ -184,7 +146,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // Sub-item s of this CTA: false when the CTA has run out of items.  n_of[i] = steps (SB kv rows each)
     // tile i can see (kv position p is visible to row R iff p <= R + delta), 0 for a tile that does
     // not exist; nmax = pages to stream.  An item whose two halves coincide has an empty second half.
-    auto sub_item = [&](int s, int& head, int& q0, int (&n_of)[2], int& nmax) -> bool {
+    auto sub_item = [&](int s, int& head, int& q0, int (&n_of)[2], int& nmax, bool& again) -> bool {
         const long long item64 = (long long)blockIdx.x + (long long)(s >> 1) * gridDim.x;
         if (item64 >= n_items) return false;
         const int item = (int)item64;
@@ -193,9 +155,10 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const int qp = (s & 1) ? r : q_pairs - 1 - r;
         q0 = qp * 2 * AT_BM;
         const bool empty = (s & 1) && r == q_pairs - 1 - r;
+        again = empty;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            int n = a.num_tiles * NSUB;
+            int n = DENSE ? (d.kv_len + SB - 1) / SB : a.num_tiles * NSUB;
             const long long last = (long long)q0 + i * AT_BM + AT_BM - 1 + a.causal_delta;
             const long long vis = last < 0 ? 0 : last / SB + 1;
             if (a.causal && vis < n) n = (int)vis;
@@ -254,7 +217,8 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             bool ok = true;
             for (int s = 0; ok; ++s) {
                 int head, q0, n_of[2], nmax;
-                if (!sub_item(s, head, q0, n_of, nmax)) break;
+            bool again;
+                if (!sub_item(s, head, q0, n_of, nmax, again)) break;
                 const int kv_head = head / kv_group;   // grouped-query attention: kv_group query heads per K/V head
                 for (int i = 0; i < 2 && ok; ++i) {
                     if (n_of[i] == 0) continue;
@@ -262,15 +226,15 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     if (q_loads[i] > 0) ok = tc_mbar_wait(&bars[B_QFREE + i], (q_loads[i] - 1) & 1, abort_flag, st, 12);
                     if (!ok) break;
                     ++q_loads[i];
-                    tc_mbar_expect_tx(&bars[B_QFULL + i], AT_Q_BYTES);
-                    tc_tma_load_3d(sQ + i * AT_Q_BYTES, &map_q, &bars[B_QFULL + i], 0, head, q0 + i * AT_BM);
-                    tc_tma_load_3d(sQ + i * AT_Q_BYTES + AT_BM * 128, &map_q, &bars[B_QFULL + i], 64, head, q0 + i * AT_BM);
+                    tc_mbar_expect_tx(&bars[B_QFULL + i], Q_BYTES);
+                    tc_tma_load_3d(sQ + i * Q_BYTES, &map_q, &bars[B_QFULL + i], 0, head, q0 + i * AT_BM);
+                    if (HD > 64) tc_tma_load_3d(sQ + i * Q_BYTES + AT_BM * 128, &map_q, &bars[B_QFULL + i], 64, head, q0 + i * AT_BM);
                 }
                 for (int l = 0; l < 2 * nmax && ok; ++l, ++t) {
                     const int slot = t % AT_STAGES;
                     const int j = l >> 1;
-                    long long page = a.bt_dtype == KTB_I64 ? bt64[j] : (long long)bt32[j];
-                    if (page < 0) {
+                    long long page = DENSE ? j : a.bt_dtype == KTB_I64 ? bt64[j] : (long long)bt32[j];
+                    if (!DENSE && page < 0) {
                         if (atomicExch(&st->negative_index, 1) == 0) st->bad_index_value = (int32_t)page;
                         page = 0;
                     }
@@ -280,6 +244,11 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                     tc_mbar_expect_tx(&bars[B_KVFULL + slot], KV_BYTES);
                     const CUtensorMap* map = (l & 1) ? &map_v : &map_k;
+                    if (DENSE) {
+                        tc_tma_load_3d(sKV + slot * KV_BYTES, map, &bars[B_KVFULL + slot], 0, kv_head, j * BN);
+                        if (HD > 64) tc_tma_load_3d(sKV + slot * KV_BYTES + KV_BLK, map, &bars[B_KVFULL + slot], 64, kv_head, j * BN);
+                        continue;
+                    }
                     at_tma_load_4d(sKV + slot * KV_BYTES, map, &bars[B_KVFULL + slot], 0, kv_head, 0, (int)page);
                     at_tma_load_4d(sKV + slot * KV_BYTES + KV_BLK, map, &bars[B_KVFULL + slot], 64, kv_head, 0, (int)page);
                 }
@@ -299,9 +268,9 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const uint32_t lead = tc_elect_one();
             const int i = warp - 1;
             const uint32_t idesc_s = tc_idesc_f16(AT_BM, SB, 0, 0);
-            const uint32_t idesc_pv = tc_idesc_f16(AT_BM, AT_D, 0, 1);
+            const uint32_t idesc_pv = tc_idesc_f16(AT_BM, HD, 0, 1);
             const uint32_t ts = tmem_s + i * 128, to = tmem_o + i * 128;
-            const uint64_t qd0 = tc_smem_desc(tc_smem_u32(sQ + i * AT_Q_BYTES), 16, 1024);
+            const uint64_t qd0 = tc_smem_desc(tc_smem_u32(sQ + i * Q_BYTES), 16, 1024);
             const uint32_t kv_addr0 = tc_smem_u32(sKV);
             int t0 = 0;                 // ring loads before this sub-item (load t0 + 2 m is K of page m, t0 + 2 m + 1 its V)
             int g0 = 0;                 // steps of this tile before this sub-item
@@ -328,7 +297,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const int g = g0 + u;
                 const uint32_t d = ts + (g & 1) * 64;
 #pragma unroll
-                for (int kk = 0; kk < AT_D / 16; ++kk) {
+                for (int kk = 0; kk < HD / 16; ++kk) {
                     const uint32_t ao = ((kk >> 2) * (AT_BM * 128) + (kk & 3) * 32) >> 4;
                     const uint32_t bo = ((kk >> 2) * KV_BLK + (kk & 3) * 32) >> 4;
                     tc_mma_f16_p(d, qd0 + ao, bd0 + bo, idesc_s, kk != 0, lead);
@@ -351,7 +320,8 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             bool ok = true;
             for (int s = 0; ok; ++s) {
                 int head, q0, n_of[2], nmax;
-                if (!sub_item(s, head, q0, n_of, nmax)) break;
+            bool again;
+                if (!sub_item(s, head, q0, n_of, nmax, again)) break;
                 n = n_of[i];
                 if (n > 0) {
                     ok = __all_sync(0xffffffffu, tc_mbar_wait(&bars[B_QFULL + i], q_uses & 1, abort_flag, st, 21)) != 0;
@@ -404,7 +374,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         constexpr int HB = SB / TPR;                 // score columns per thread
         constexpr int CW = HB < 32 ? HB : 32;        // columns per TMEM load
         constexpr int NCH = HB / CW;
-        constexpr int OH = AT_D / TPR;               // output columns per thread
+        constexpr int OH = HD / TPR;               // output columns per thread
         const int tile = (warp - 4) / (4 * TPR);     // which query tile this warpgroup (pair) owns
         const int half = TPR == 2 ? ((warp - 4) >> 2) & 1 : 0;
         const int q = warp & 3;                      // TMEM lane quadrant this warp may access
@@ -437,14 +407,23 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 
         for (int s = 0; ok; ++s) {
         int head, q0, n_of[2], nmax;
-        if (!sub_item(s, head, q0, n_of, nmax)) break;
+            bool again;
+        if (!sub_item(s, head, q0, n_of, nmax, again)) break;
         const int n = n_of[tile];
-        if (n == 0) continue;
         const int R = q0 + tile * AT_BM + r;
+        if (n == 0) {
+            if (DENSE && !again && R < a.seq_q) {               // a tile whose rows see nothing
+                __half* dst = reinterpret_cast<__half*>(a.arena) + a.o_off + (int64_t)R * a.o_row_stride + (int64_t)head * a.o_head_stride + half * OH;
+                for (int c = 0; c < OH; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
+                if (half == 0 && d.lse) d.lse[(int64_t)R * d.row + (int64_t)head * d.head] = -INFINITY;
+            }
+            continue;
+        }
         float m_ref = a.m_init * 1.4426950408889634f;           // exponent reference, log2 domain
         float m_run = m_ref;                                    // true running maximum
         float l_run = half == 0 ? a.l_init : 0.f;               // this thread's share of the running sum
-        const long long limit = (long long)R + a.causal_delta;  // last visible kv position
+        long long limit = (long long)R + a.causal_delta;        // last visible kv position
+        if (DENSE && (!a.causal || limit >= d.kv_len)) limit = d.kv_len - 1;
         const long long tile_limit = (long long)q0 + tile * AT_BM + a.causal_delta;
         // first step with a hidden column for some row of the tile: (j + 1) * SB - 1 > tile_limit
         // (kept as one int so that the common, unmasked step pays one compare for the mask)
@@ -453,6 +432,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const long long jm = tile_limit + 1 >= 0 ? (tile_limit + 1) / SB : 0;
             j_mask = jm > 0x7fffffff ? 0x7fffffff : (int)jm;
         }
+        if (DENSE && d.kv_len / SB < j_mask) j_mask = d.kv_len / SB;      // the last keys do not fill a step
         for (int j = 0; j < n && ok; ++j) {            // j counts steps of SB kv rows
             const int g = g0 + j;                      // step number of the tile across sub-items
             const uint32_t slot_off = (g & 1) * 64;
@@ -525,7 +505,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
                 uint32_t packed[CW / 2];
-                at_chunk_prob<CW, POLY>(v[c], sl, m_exp, acc2, packed);
+                at_chunk_prob<CW, POLY, DENSE>(v[c], sl, m_exp, acc2, packed);
                 tc_tmem_st<CW / 2>(p_addr + slot_off + c * (CW / 2), packed);
             }
             float s0, s1;
@@ -544,8 +524,13 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             // total row sum = the two partial sums (same rescaling history on both threads)
             float l_other = 0.f;
             if (TPR == 1 || swap_with_partner(l_run, l_other)) {
-                const float inv = 1.0f / (l_run + l_other);
+                // (the polynomial leaves 2^-125 of a hidden key: a row that sees none is known by its limit)
+                const float sum = DENSE && limit < 0 ? 0.f : l_run + l_other;
+                const float inv = DENSE && limit < 0 ? 0.f : 1.0f / sum;
                 const bool store = *abort_flag == 0 && R < a.seq_q;
+                // (m_ref in units of log 2; the logarithm of an empty sum is -inf)
+                if (DENSE && store && half == 0 && d.lse)
+                    d.lse[(int64_t)R * d.row + (int64_t)head * d.head] = (m_ref + log2f(sum)) * 0.6931471805599453f;
                 __half* dst = reinterpret_cast<__half*>(a.arena) + a.o_off + (int64_t)R * a.o_row_stride +
                               (int64_t)head * a.o_head_stride + half * OH;
 #pragma unroll
@@ -575,14 +560,14 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (warp == 1) tc_tmem_dealloc(tmem_base, 512);
 }
 
-template <int BN, int TPR, int POLY = 0>
+template <int BN, int TPR, int POLY = 0, int HD = AT_D, bool DENSE = false>
 static int launch_attn(ktb_ctx* ctx, const ktb_attn_args& a, const CUtensorMap& mq, const CUtensorMap& mk,
-                       const CUtensorMap& mv) {
+                       const CUtensorMap& mv, const at_dense& d = at_dense()) {
     constexpr int AT_STAGES = BN == 128 ? 4 : 8;
-    constexpr size_t SMEM = 2 * AT_Q_BYTES + AT_STAGES * (size_t)(BN * AT_D * 2) + 2 * 2 * 2 * AT_BM * 4 + 1024 + 512;
+    constexpr size_t SMEM = 2 * AT_BM * HD * 2 + AT_STAGES * (size_t)(BN * HD * 2) + 2 * 2 * 2 * AT_BM * 4 + 1024 + 512;
     static bool attr_set[KTB_MAX_DEVICES] = {};     // the attribute is per device
     if (!attr_set[ctx->device & (KTB_MAX_DEVICES - 1)]) {
-        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_fwd_kernel<BN, TPR, POLY>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_fwd_kernel<BN, TPR, POLY, HD, DENSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
         attr_set[ctx->device & (KTB_MAX_DEVICES - 1)] = true;
     }
     const int q_pairs = (a.seq_q + 2 * AT_BM - 1) / (2 * AT_BM);
@@ -590,7 +575,7 @@ static int launch_attn(ktb_ctx* ctx, const ktb_attn_args& a, const CUtensorMap& 
     const long long items = (long long)((q_pairs + 1) / 2) * a.heads;
     if (items > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_fwd", "too many query tiles");
     const int grid = items < ctx->sm_count ? (int)items : ctx->sm_count;
-    ktb_attention_fwd_kernel<BN, TPR, POLY><<<grid, 128 + 256 * TPR, SMEM, ctx->stream>>>(mq, mk, mv, a, q_pairs, (int)items, ctx->dev_status);
+    ktb_attention_fwd_kernel<BN, TPR, POLY, HD, DENSE><<<grid, 128 + 256 * TPR, SMEM, ctx->stream>>>(mq, mk, mv, a, d, q_pairs, (int)items, ctx->dev_status);
     KTB_CHECK_LAUNCH(ctx, "ktb_attention_fwd_kernel");
     return KTB_OK;
 }
@@ -641,4 +626,53 @@ extern "C" int ktb_launch_attention_fwd(ktb_ctx* ctx, const ktb_attn_args* args)
         case 64: return launch_attn<64, 1, 1>(ctx, a, mq, mk, mv);
         default: return launch_attn<128, 1, 1>(ctx, a, mq, mk, mv);
     }
+}
+
+extern "C" int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_args* args) {
+    if (!ctx || !args) return KTB_E_ARG;
+    const ktb_attn_dense_args& b = *args;
+    const char* me = "attention_dense";
+    if (b.head_dim != 64 && b.head_dim != 128) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "head_dim must be 64 or 128");
+    if (b.q_len < 0 || b.kv_len < 0 || b.heads < 0 || b.kv_group < 1 || b.heads % b.kv_group)
+        return ktb_fail(ctx, KTB_E_ARG, me, "lengths, heads or kv_group");
+    if (b.q_len == 0 || b.heads == 0) return KTB_OK;
+    if (b.kv_len == 0 || b.q_len > (1 << 30) || b.kv_len > (1 << 30)) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "lengths");
+    if (!(b.scale > 0.f && b.scale <= 3.0e38f)) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "score scale must be positive");
+    const int64_t all = b.q_off | b.k_off | b.v_off | b.o_off | b.q_row | b.q_head | b.k_row | b.k_head | b.v_row | b.v_head | b.o_row | b.o_head;
+    if ((all & 7) || (reinterpret_cast<uintptr_t>(b.arena) & 15))
+        return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "strides and offsets must be multiples of 8 elements");
+    __half* base = reinterpret_cast<__half*>(b.arena);
+    CUtensorMap mq, mk, mv;
+    const uint32_t box[3] = {64, 1, 128};
+    const struct { CUtensorMap* map; int64_t off, rows, heads, row, head; } t[3] = {
+        {&mq, b.q_off, b.q_len, b.heads, b.q_row, b.q_head},
+        {&mk, b.k_off, b.kv_len, b.heads / b.kv_group, b.k_row, b.k_head},
+        {&mv, b.v_off, b.kv_len, b.heads / b.kv_group, b.v_row, b.v_head}};
+    for (int i = 0; i < 3; ++i) {
+        const uint64_t dims[3] = {(uint64_t)b.head_dim, (uint64_t)t[i].heads, (uint64_t)t[i].rows};
+        const uint64_t str[2] = {(uint64_t)t[i].head * 2, (uint64_t)t[i].row * 2};
+        if (!tc_make_map_f16(t[i].map, base + t[i].off, 3, dims, str, box))
+            return ktb_fail(ctx, KTB_E_CUDA, me, "cuTensorMapEncodeTiled failed");
+    }
+    ktb_attn_args a;
+    memset(&a, 0, sizeof(a));
+    a.arena = b.arena;
+    a.o_off = b.o_off;
+    a.o_row_stride = b.o_row;
+    a.o_head_stride = b.o_head;
+    a.seq_q = b.q_len;
+    a.heads = b.heads;
+    a.head_dim = b.head_dim;
+    a.kv_group = b.kv_group;
+    a.causal = b.causal != 0;
+    a.causal_delta = b.causal_delta;
+    a.scale = b.scale;
+    a.m_init = -1e30f;
+    a.l_init = 0.f;
+    at_dense d;
+    d.lse = b.lse_off < 0 ? nullptr : reinterpret_cast<float*>(b.arena) + b.lse_off;
+    d.row = b.lse_row;
+    d.head = b.lse_head;
+    d.kv_len = b.kv_len;
+    return b.head_dim == 64 ? launch_attn<128, 1, 1, 64, true>(ctx, a, mq, mk, mv, d) : launch_attn<128, 1, 1, 128, true>(ctx, a, mq, mk, mv, d);
 }

@@ -91,6 +91,13 @@ static __device__ __forceinline__ void tc_tma_load_3d(void* smem_dst, const CUte
         : "memory");
 }
 
+// Untiled copy: both addresses and `bytes` multiples of 16.
+static __device__ __forceinline__ void tc_bulk_load(void* smem_dst, const void* src, uint64_t* bar, uint32_t bytes) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(tc_smem_u32(smem_dst)), "l"(src), "r"(bytes), "r"(tc_smem_u32(bar))
+                 : "memory");
+}
+
 // Tile store shared -> global (clipped at the tensor's edges), tracked by the issuing thread's bulk groups.
 static __device__ __forceinline__ void tc_tma_store_2d(const CUtensorMap* map, const void* smem_src, int x, int y) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
@@ -346,6 +353,68 @@ __device__ __forceinline__ void tc_tmem_st<8>(uint32_t taddr, const uint32_t (&r
 
 static __device__ __forceinline__ void tc_tmem_st_wait() {
     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// ---- arithmetic of the attention kernels ------------------------------------------------------
+static __device__ __forceinline__ float at_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// two f32 lanes in one 64-bit register: Blackwell issues fma / add on such pairs as one instruction
+static __device__ __forceinline__ uint64_t at_pack2(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+static __device__ __forceinline__ void at_unpack2(uint64_t v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+static __device__ __forceinline__ uint64_t at_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+static __device__ __forceinline__ uint64_t at_add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+static __device__ __forceinline__ uint64_t at_mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+
+// 2^x for two values at once on the FMA pipe (the exp unit is the busiest unit of the softmax):
+// x = r + f with r = round(x), 2^f by a cubic on [-0.5, 0.5] (relative error 7.5e-5, a sixth of
+// an f16 ulp) or, where the sum of the values is a result of its own, by a quartic (2.7e-6), 2^r by an
+// add into the exponent field.  x is clamped to >= -125 so that the exponent stays positive (such a term is
+// zero in f16 either way).
+template <bool FINE>
+static __device__ __forceinline__ void at_ex2_poly2(float x0, float x1, float& p0, float& p1) {
+    const float magic = 12582912.f;                     // 1.5 * 2^23: the sum keeps round(x) in the low mantissa bits
+    const uint64_t x2 = at_pack2(fmaxf(x0, -125.f), fmaxf(x1, -125.f));
+    const uint64_t t2 = at_add2(x2, at_pack2(magic, magic));
+    const uint64_t r2 = at_add2(t2, at_pack2(-magic, -magic));
+    const uint64_t f2 = at_fma2(r2, at_pack2(-1.f, -1.f), x2);
+    uint64_t q2;
+    if (FINE) {
+        q2 = at_fma2(at_pack2(0.009570101276040077f, 0.009570101276040077f), f2, at_pack2(0.05591785907745361f, 0.05591785907745361f));
+        q2 = at_fma2(q2, f2, at_pack2(0.240247443318367f, 0.240247443318367f));
+        q2 = at_fma2(q2, f2, at_pack2(0.6931217908859253f, 0.6931217908859253f));
+        q2 = at_fma2(q2, f2, at_pack2(0.9999992847442627f, 0.9999992847442627f));
+    } else {
+        q2 = at_fma2(at_pack2(0.05517164617776871f, 0.05517164617776871f), f2, at_pack2(0.2426111251115799f, 0.2426111251115799f));
+        q2 = at_fma2(q2, f2, at_pack2(0.6932609677314758f, 0.6932609677314758f));
+        q2 = at_fma2(q2, f2, at_pack2(0.9999280571937561f, 0.9999280571937561f));
+    }
+    float q0, q1, t0, t1;
+    at_unpack2(q2, q0, q1);
+    at_unpack2(t2, t0, t1);
+    p0 = __int_as_float(__float_as_int(q0) + (__float_as_int(t0) << 23));
+    p1 = __int_as_float(__float_as_int(q1) + (__float_as_int(t1) << 23));
 }
 
 // ---- descriptors ----------------------------------------------------------------------------

@@ -936,8 +936,9 @@ def _fused_statement(dev, st: Store, arena: ArenaMap, sid: int, row_shard):
 
 def _fused_stores(dev, stores: List[Store], arena: ArenaMap, sid: int):
     """A fused kernel that runs several of the next stores: (statement, how many), or None."""
+    from .lower_attn_train import try_lower_attention_train
     from .lower_rotary import try_lower_rotary
-    return try_lower_rotary(dev, stores, arena, sid)
+    return try_lower_rotary(dev, stores, arena, sid) or try_lower_attention_train(dev, stores, arena, sid)
 
 
 # A statement that stores one value per row made of its neighbour's row reductions joins that neighbour's launch.

@@ -134,6 +134,24 @@ class AttnArgs(C.Structure):
                 ("steps", C.c_int32), ("reserved", C.c_int32), ("scratch_bytes", C.c_int64)]
 
 
+class AttnDenseArgs(C.Structure):
+    _fields_ = [("arena", C.c_void_p)] + \
+        [(n, C.c_int64) for n in "q_off k_off v_off o_off lse_off q_row q_head k_row k_head v_row v_head o_row o_head lse_row lse_head".split()] + \
+        [(n, C.c_int32) for n in "q_len kv_len heads kv_group head_dim causal causal_delta".split()] + [("scale", C.c_float)]
+
+
+ATTN_DQ, ATTN_DK, ATTN_DV = 1, 2, 4
+
+
+class AttnBwdArgs(C.Structure):
+    _fields_ = [("arena", C.c_void_p)] + \
+        [(n, C.c_int64) for n in ("q_off k_off v_off o_off do_off lse_off dq_off dk_off dv_off q_row q_head k_row k_head v_row v_head "
+                                  "o_row o_head do_row do_head lse_row lse_head dq_row dq_head dk_row dk_head dv_row dv_head").split()] + \
+        [(n, C.c_int32) for n in "q_len kv_len heads kv_group head_dim causal causal_delta".split()] + [("scale", C.c_float)] + \
+        [(n, C.c_int32) for n in "want dq_row0 dq_rows dq_head0 dq_heads dk_row0 dk_rows dk_head0 dk_heads reserved".split()] + \
+        [("dev_scratch", C.c_void_p), ("scratch_bytes", C.c_int64)]
+
+
 ROTARY_TENSORS = 4
 
 
@@ -230,6 +248,9 @@ SYMBOLS = {
     "ktb_launch_generic": (C.c_int, [C.c_void_p, C.POINTER(GenOpArgs)]),
     "ktb_launch_gemm_f16": (C.c_int, [C.c_void_p, C.POINTER(GemmArgs)]),
     "ktb_launch_attention_fwd": (C.c_int, [C.c_void_p, C.POINTER(AttnArgs)]),
+    "ktb_launch_attention_dense": (C.c_int, [C.c_void_p, C.POINTER(AttnDenseArgs)]),
+    "ktb_attention_bwd_scratch_bytes": (C.c_int64, [C.POINTER(AttnBwdArgs)]),
+    "ktb_launch_attention_bwd": (C.c_int, [C.c_void_p, C.POINTER(AttnBwdArgs)]),
     "ktb_launch_rotary": (C.c_int, [C.c_void_p, C.POINTER(RotaryArgs)]),
 }
 
