@@ -19,16 +19,19 @@
 // value on average, the only roundings before the results') after a shift by powers of two that keeps them in range:
 // P by 2^14, dS by 2^14 / B with B >= |dO V^T - D| a power of two from the norms of dO and V (per row for dQ, per key head
 // for dK, whose sums run over rows).  Sums, D and the statistics are f32.
+#include <type_traits>
+
 #include "tc_common.cuh"
 
 #define AB_M 128                   // rows that a CTA owns
-#define AB_N 64                    // rows of a step
+#define AB_N 64                    // streamed rows of a step
 #define AB_SHIFT 14.f
 #define AB_LOG2E 1.4426950408889634f
 
 // ---- what the rows bring: 14 - lse / ln 2, D, |dO| per row, and the largest norms --------------------------------
 // One block takes 64 rows of one head, LANES = head_dim / 8 threads a row.  blockIdx.y counts blocks of queries, then of keys.
 struct ab_scratch {
+    unsigned* taken;               // items handed out beyond the first of every CTA
     float* neg_lse;                // [heads][padded queries]
     float* d;
     float* norm;
@@ -128,7 +131,7 @@ static __device__ __forceinline__ float ab_shrink(float bound) {
     return __uint_as_float((unsigned)(127 - (e + 1)) << 23);
 }
 
-// ---- the two kernels -----------------------------------------------------------------------------------------------
+// ---- the kernel ----------------------------------------------------------------------------------------------------
 template <int HD>
 struct ab_shape {
     static constexpr int BLOCKS = HD / 64;                  // 64-column blocks of a tile (a 128-byte swizzled row each)
@@ -136,6 +139,9 @@ struct ab_shape {
     static constexpr int STEP = AB_N * HD * 2;              // bytes of X', of Y'
     static constexpr int STAGES = 4;
     static constexpr size_t SMEM = 2 * OWN + STAGES * (2 * STEP + 2 * AB_N * 4) + 1024 + 256;
+    // columns of TMEM: two accumulators (for queries X and Y as f16 pairs in place of the second), then the slots: S and T
+    static constexpr int ACC1 = HD, X = HD, Y = HD + HD / 2, SLOT = 2 * HD;
+    static constexpr int SLOTS = (512 - SLOT) / (2 * AB_N);
 };
 
 // Waits for a phase no matter what else has failed, so that no copy is under way into memory that the CTA gives up.
@@ -145,65 +151,90 @@ static __device__ void ab_drain(uint64_t* bar, uint32_t parity) {
         if (clock64() - start > 1000000000ll) return;
 }
 
-template <int HD, bool KEYS>
+// What there is to do: the tiles of keys, then those of queries; among each, longest walks first, either head by head (so that
+// the CTAs at work share their streams in L2) or over all heads (where there are few tiles and a long one must not come last).
+struct ab_work {
+    int key_tiles, key_heads, query_tiles, query_heads;
+    int by_head;
+};
+
+struct ab_item {
+    bool keys;
+    int row0, head, first, per_head, n;                     // n steps: per_head streamed tiles from `first` on, for every streamed head
+};
+
+static __device__ __forceinline__ ab_item ab_decode(const ktb_attn_bwd_args& a, const ab_work& j, int index) {
+    ab_item t;
+    const int of_keys = j.key_tiles * j.key_heads;
+    t.keys = index < of_keys;
+    const int at = t.keys ? index : index - of_keys, tiles = t.keys ? j.key_tiles : j.query_tiles, heads = t.keys ? j.key_heads : j.query_heads;
+    const int rank = j.by_head ? at % tiles : at / heads, head_here = j.by_head ? at / tiles : at % heads;
+    t.first = 0;
+    if (t.keys) {
+        t.row0 = a.dk_row0 + rank * AB_M;
+        t.head = a.dk_head0 + head_here;
+        t.per_head = (a.q_len + AB_N - 1) / AB_N;
+        if (a.causal) {
+            const long long q = (long long)t.row0 - a.causal_delta;             // the first query that sees key row0
+            t.first = q <= 0 ? 0 : q >= a.q_len ? t.per_head : (int)(q / AB_N);
+        }
+        t.per_head -= t.first;
+        t.n = t.per_head * a.kv_group;
+    } else {
+        t.row0 = a.dq_row0 + (tiles - 1 - rank) * AB_M;
+        t.head = a.dq_head0 + head_here;
+        t.per_head = (a.kv_len + AB_N - 1) / AB_N;
+        if (a.causal) {
+            const int last_row = t.row0 + AB_M - 1 < a.q_len - 1 ? t.row0 + AB_M - 1 : a.q_len - 1;
+            const long long key = (long long)last_row + a.causal_delta;         // the last key that the tile sees
+            const long long n = key < 0 ? 0 : key / AB_N + 1;
+            if (n < t.per_head) t.per_head = (int)n;
+        }
+        t.n = t.per_head;
+    }
+    return t;
+}
+
+template <int HD>
 __global__ void __launch_bounds__(384, 1)
-ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_y,
-                         const __grid_constant__ CUtensorMap map_xs, const __grid_constant__ CUtensorMap map_ys,
-                         const ktb_attn_bwd_args a, const ab_scratch w, int row_tiles, int heads_here, int by_head, ktb_status* st) {
+ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                         const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
+                         const ktb_attn_bwd_args a, const ab_scratch w, const ab_work work, ktb_status* st) {
     typedef ab_shape<HD> Z;
-    constexpr int SLOTS = KEYS ? 2 : 3;                     // S and T, 64 columns of TMEM each
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sX = smem;
     uint8_t* sY = sX + Z::OWN;
     uint8_t* ring = sY + Z::OWN;                            // per stage X', then Y'
-    float* sRow = reinterpret_cast<float*>(ring + Z::STAGES * 2 * Z::STEP);     // KEYS: per stage 64 x (14 - lse / ln 2), 64 x D
-    uint64_t* bars = reinterpret_cast<uint64_t*>(sRow + Z::STAGES * 2 * AB_N);
-    uint64_t *full = bars, *empty = bars + Z::STAGES, *own = bars + 2 * Z::STAGES, *s_full = own + 1, *p_full = s_full + SLOTS, *done = p_full + SLOTS;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(done + 1);
+    float* sRow = reinterpret_cast<float*>(ring + Z::STAGES * 2 * Z::STEP);     // keys: per stage 64 x (14 - lse / ln 2), 64 x D
+    uint64_t* full = reinterpret_cast<uint64_t*>(sRow + Z::STAGES * 2 * AB_N);
+    uint64_t *empty = full + Z::STAGES, *own_full = empty + Z::STAGES, *own_free = own_full + 1, *a_ready = own_free + 1;
+    uint64_t *acc_free = a_ready + 1, *done = acc_free + 1, *next_full = done + 1, *next_free = next_full + 2;
+    uint64_t *s_full = next_free + 2, *p_full = s_full + Z::SLOTS;
+    volatile int* next = reinterpret_cast<volatile int*>(p_full + Z::SLOTS);    // items handed out, two at a time
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(next) + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int grp = a.kv_group;
-
-    // The CTA's tile, longest walks first: of all heads (few tiles, so that the long ones do not come last), or head by head
-    // (so that the CTAs at work share their stream in L2).
-    const int tile_order = by_head ? blockIdx.x % row_tiles : blockIdx.x / heads_here;
-    const int head_here = by_head ? blockIdx.x / row_tiles : blockIdx.x % heads_here;
-    const int tile = KEYS ? tile_order : row_tiles - 1 - tile_order;            // causal: early keys, late queries
-    const int row0 = (KEYS ? a.dk_row0 : a.dq_row0) + tile * AB_M;
-    const int row_end = KEYS ? a.dk_row0 + a.dk_rows : a.dq_row0 + a.dq_rows;
-    const int head = (KEYS ? a.dk_head0 : a.dq_head0) + head_here;              // KEYS: key head; else query head
-    // steps: `per_head` tiles of 64 streamed rows from first * 64 on; for keys once for every query head of the group
-    int first = 0, per_head;
-    if (KEYS) {
-        per_head = (a.q_len + AB_N - 1) / AB_N;
-        if (a.causal) {
-            const long long q = (long long)row0 - a.causal_delta;               // the first query that sees key row0
-            first = q <= 0 ? 0 : q >= a.q_len ? per_head : (int)(q / AB_N);
-        }
-        per_head -= first;
-    } else {
-        per_head = (a.kv_len + AB_N - 1) / AB_N;
-        if (a.causal) {
-            const int last_row = row0 + AB_M - 1 < a.q_len - 1 ? row0 + AB_M - 1 : a.q_len - 1;
-            const long long k = (long long)last_row + a.causal_delta;           // the last key that the tile sees
-            const long long n = k < 0 ? 0 : k / AB_N + 1;
-            if (n < per_head) per_head = (int)n;
-        }
-    }
-    const int n = KEYS ? per_head * grp : per_head;
+    const int grp = a.kv_group, total = work.key_tiles * work.key_heads + work.query_tiles * work.query_heads;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < Z::STAGES; ++i) {
             tc_mbar_init(&full[i], 1);
             tc_mbar_init(&empty[i], 1);
         }
-        tc_mbar_init(own, 1);
-        for (int i = 0; i < SLOTS; ++i) {
-            tc_mbar_init(&s_full[i], 1);
-            tc_mbar_init(&p_full[i], 8);
-        }
+        tc_mbar_init(own_full, 1);
+        tc_mbar_init(own_free, 1);
+        tc_mbar_init(a_ready, 8);
+        tc_mbar_init(acc_free, 8);
         tc_mbar_init(done, 1);
+        for (int i = 0; i < 2; ++i) {
+            tc_mbar_init(&next_full[i], 1);
+            tc_mbar_init(&next_free[i], 10);                // warps 1 and 2, eight warps of the softmax
+        }
+        for (int i = 0; i < Z::SLOTS; ++i) {
+            tc_mbar_init(&s_full[i], 1);
+            tc_mbar_init(&p_full[i], 4);
+        }
         *abort_flag = 0;
         tc_fence_barrier_init();
     }
@@ -213,47 +244,82 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
     __syncthreads();
     tc_fence_after_sync();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-    const uint32_t t_acc0 = tmem, t_acc1 = tmem + 128, t_slot = tmem + (KEYS ? 256 : 128);      // slot i: S at 128 i, T at 128 i + 64
 
-    if (warp == 0) {
-        if (lane == 0 && n > 0) {
-            tc_prefetch_tmap(&map_x);
-            tc_prefetch_tmap(&map_xs);
-            tc_prefetch_tmap(&map_y);
-            tc_prefetch_tmap(&map_ys);
-            tc_mbar_expect_tx(own, 2 * Z::OWN);
+    // The k-th item of this CTA (whichever CTA is free takes the next one; what is computed does not depend on which that is), for
+    // all lanes of a warp.  -1: no more, or a wait ran out.
+    auto take = [&](int k) -> int {
+        const int q = k & 1;
+        if (!__all_sync(0xffffffffu, tc_mbar_wait(&next_full[q], (k >> 1) & 1, abort_flag, st, 72))) return -1;
+        const int index = __shfl_sync(0xffffffffu, next[q], 0);
+        if (lane == 0) tc_mbar_arrive(&next_free[q]);
+        return index < total ? index : -1;
+    };
+
+    if (warp == 0) {                                        // hands the items out and streams X' and Y'
+        if (lane == 0) {
+            tc_prefetch_tmap(&map_q);
+            tc_prefetch_tmap(&map_g);
+            int t = 0;                                      // stages filled
+            bool ok = true;
+            for (int k = 0; ok; ++k) {
+                const int q = k & 1;
+                const int index = k == 0 ? (int)blockIdx.x : (int)(gridDim.x + atomicAdd(w.taken, 1u));
+                if (k >= 2 && !tc_mbar_wait(&next_free[q], ((k >> 1) - 1) & 1, abort_flag, st, 73)) break;
+                next[q] = index;
+                tc_mbar_arrive(&next_full[q]);
+                if (index >= total) break;
+                const ab_item it = ab_decode(a, work, index);
+                const CUtensorMap *mx = it.keys ? &map_q : &map_k, *my = it.keys ? &map_g : &map_v;
+                int sh = it.keys ? it.head * grp : it.head / grp, s = 0;                             // streamed head and step of it
+                for (int i = 0; i < it.n; ++i, ++t) {
+                    const int stage = t % Z::STAGES;
+                    if (!tc_mbar_wait(&empty[stage], ((t / Z::STAGES) & 1) ^ 1, abort_flag, st, 61)) {
+                        ok = false;
+                        break;
+                    }
+                    const int r = (it.first + s) * AB_N;
+                    uint8_t* to = ring + stage * 2 * Z::STEP;
+                    tc_mbar_expect_tx(&full[stage], 2 * Z::STEP + (it.keys ? 2 * AB_N * 4 : 0));
 #pragma unroll
-            for (int b = 0; b < Z::BLOCKS; ++b)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    tc_tma_load_3d(sX + b * (AB_M * 128) + h * (AB_N * 128), &map_x, own, b * 64, head, row0 + h * AB_N);
-                    tc_tma_load_3d(sY + b * (AB_M * 128) + h * (AB_N * 128), &map_y, own, b * 64, head, row0 + h * AB_N);
+                    for (int b = 0; b < Z::BLOCKS; ++b) {
+                        tc_tma_load_3d(to + b * (AB_N * 128), mx, &full[stage], b * 64, sh, r);
+                        tc_tma_load_3d(to + Z::STEP + b * (AB_N * 128), my, &full[stage], b * 64, sh, r);
+                    }
+                    if (it.keys) {
+                        float* rows = sRow + stage * 2 * AB_N;
+                        tc_bulk_load(rows, w.neg_lse + (int64_t)sh * w.padded + r, &full[stage], AB_N * 4);
+                        tc_bulk_load(rows + AB_N, w.d + (int64_t)sh * w.padded + r, &full[stage], AB_N * 4);
+                    }
+                    if (++s == it.per_head) s = 0, ++sh;
                 }
-            int loaded = 0;
-            for (int i = 0; i < n; ++i) {
-                const int stage = i % Z::STAGES;
-                if (!tc_mbar_wait(&empty[stage], ((i / Z::STAGES) & 1) ^ 1, abort_flag, st, 61)) break;
-                const int sh = KEYS ? head * grp + i / per_head : head / grp;   // streamed head
-                const int r = (first + (KEYS ? i % per_head : i)) * AB_N;
-                uint8_t* to = ring + stage * 2 * Z::STEP;
-                tc_mbar_expect_tx(&full[stage], 2 * Z::STEP + (KEYS ? 2 * AB_N * 4 : 0));
-#pragma unroll
-                for (int b = 0; b < Z::BLOCKS; ++b) {
-                    tc_tma_load_3d(to + b * (AB_N * 128), &map_xs, &full[stage], b * 64, sh, r);
-                    tc_tma_load_3d(to + Z::STEP + b * (AB_N * 128), &map_ys, &full[stage], b * 64, sh, r);
-                }
-                if (KEYS) {
-                    float* rows = sRow + stage * 2 * AB_N;
-                    tc_bulk_load(rows, w.neg_lse + (int64_t)sh * w.padded + r, &full[stage], AB_N * 4);
-                    tc_bulk_load(rows + AB_N, w.d + (int64_t)sh * w.padded + r, &full[stage], AB_N * 4);
-                }
-                loaded = i + 1;
             }
-            if (*abort_flag) {
-                ab_drain(own, 0);
-                for (int i = loaded > Z::STAGES ? loaded - Z::STAGES : 0; i < loaded; ++i) ab_drain(&full[i % Z::STAGES], (i / Z::STAGES) & 1);
-            }
+            if (*abort_flag)
+                for (int i = t > Z::STAGES ? t - Z::STAGES : 0; i < t; ++i) ab_drain(&full[i % Z::STAGES], (i / Z::STAGES) & 1);
         }
+    } else if (warp == 2) {                                 // X and Y of the next item, as soon as these are not read any more
+        int c = 0;                                          // walks so far
+        for (int k = 0;; ++k) {
+            const int index = take(k);
+            if (index < 0) break;
+            const ab_item it = ab_decode(a, work, index);
+            if (it.n <= 0) continue;
+            if (c > 0 && !__all_sync(0xffffffffu, tc_mbar_wait(own_free, (c - 1) & 1, abort_flag, st, 69))) break;
+            if (lane == 0) {
+                const CUtensorMap *mx = it.keys ? &map_k : &map_q, *my = it.keys ? &map_v : &map_g;
+                tc_mbar_expect_tx(own_full, 2 * Z::OWN);
+#pragma unroll
+                for (int b = 0; b < Z::BLOCKS; ++b)
+#pragma unroll
+                    for (int h = 0; h < AB_M / AB_N; ++h) {
+                        const int at = b * (AB_M * 128) + h * (AB_N * 128);
+                        tc_tma_load_3d(sX + at, mx, own_full, b * 64, it.head, it.row0 + h * AB_N);
+                        tc_tma_load_3d(sY + at, my, own_full, b * 64, it.head, it.row0 + h * AB_N);
+                    }
+            }
+            __syncwarp();
+            ++c;
+        }
+        if (lane == 0 && *abort_flag && c > 0) ab_drain(own_full, (c - 1) & 1);
     } else if (warp == 1) {
         // the warp runs this converged; one elected lane issues the tcgen05 instructions
         const uint32_t lead = tc_elect_one();
@@ -265,178 +331,260 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_x, const __grid
             tc_fence_after_sync();
             return ok;
         };
-        auto scores = [&](int i) {                              // S and T of step i
-            const uint32_t at = ring_at + (i % Z::STAGES) * 2 * Z::STEP, d = t_slot + (i % SLOTS) * 128;
-            const uint64_t xs = tc_smem_desc(at, 16, 1024), ys = tc_smem_desc(at + Z::STEP, 16, 1024);
+        int g0 = 0, c = 0, cq = 0;                              // steps (= stages), walks, walks of queries before this item
+        // A walk.  Keys: X and Y from shared memory.  Queries: from TMEM, where they have room; that halves the operand bytes of S
+        // and T, which shared memory's bandwidth bounds (48 cycles a product with both operands there, 32 with one).
+        auto walk = [&](auto of_keys, const int n) -> bool {
+            constexpr bool KEYS = decltype(of_keys)::value;
+            auto scores = [&](int g) {                          // S = X X'^T and T = Y Y'^T of one step
+                const uint32_t at = ring_at + (g % Z::STAGES) * 2 * Z::STEP, d = tmem + Z::SLOT + (g % Z::SLOTS) * (2 * AB_N);
+                const uint64_t xs = tc_smem_desc(at, 16, 1024), ys = tc_smem_desc(at + Z::STEP, 16, 1024);
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-                const uint32_t ao = ((kk >> 2) * (AB_M * 128) + (kk & 3) * 32) >> 4, bo = ((kk >> 2) * (AB_N * 128) + (kk & 3) * 32) >> 4;
-                tc_mma_f16_p(d, xd + ao, xs + bo, idesc_s, kk != 0, lead);
-            }
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    const uint32_t ao = ((kk >> 2) * (AB_M * 128) + (kk & 3) * 32) >> 4, bo = ((kk >> 2) * (AB_N * 128) + (kk & 3) * 32) >> 4;
+                    if (KEYS) tc_mma_f16_p(d, xd + ao, xs + bo, idesc_s, kk != 0, lead);
+                    else tc_mma_f16_ts_p(d, tmem + Z::X + kk * 8, xs + bo, idesc_s, kk != 0, lead);
+                }
 #pragma unroll
-            for (int kk = 0; kk < HD / 16; ++kk) {
-                const uint32_t ao = ((kk >> 2) * (AB_M * 128) + (kk & 3) * 32) >> 4, bo = ((kk >> 2) * (AB_N * 128) + (kk & 3) * 32) >> 4;
-                tc_mma_f16_p(d + 64, yd + ao, ys + bo, idesc_s, kk != 0, lead);
+                for (int kk = 0; kk < HD / 16; ++kk) {
+                    const uint32_t ao = ((kk >> 2) * (AB_M * 128) + (kk & 3) * 32) >> 4, bo = ((kk >> 2) * (AB_N * 128) + (kk & 3) * 32) >> 4;
+                    if (KEYS) tc_mma_f16_p(d + AB_N, yd + ao, ys + bo, idesc_s, kk != 0, lead);
+                    else tc_mma_f16_ts_p(d + AB_N, tmem + Z::Y + kk * 8, ys + bo, idesc_s, kk != 0, lead);
+                }
+                tc_mma_commit_p(&s_full[g % Z::SLOTS], lead);
+            };
+            bool ok = wait(KEYS ? own_full : a_ready, (KEYS ? c : cq) & 1, 62);
+            if (!KEYS && ok && lane == 0) tc_mbar_arrive(own_free);             // the softmax has moved them to TMEM
+            for (int i = 0; i < Z::SLOTS && i < n && ok; ++i) {
+                ok = wait(&full[(g0 + i) % Z::STAGES], ((g0 + i) / Z::STAGES) & 1, 63);
+                if (ok) scores(g0 + i);
             }
-            tc_mma_commit_p(&s_full[i % SLOTS], lead);
-        };
-        auto sums = [&](int i) {                                // the accumulators take step i; its stage is free then
-            const uint32_t at = ring_at + (i % Z::STAGES) * 2 * Z::STEP, p = t_slot + (i % SLOTS) * 128;
-            const uint64_t xs = tc_smem_desc(at, AB_N * 128, 1024), ys = tc_smem_desc(at + Z::STEP, AB_N * 128, 1024);
-            if (KEYS) {
+            if (KEYS && ok && n <= Z::SLOTS) tc_mma_commit_p(own_free, lead);   // (X and Y have been read when these products are done)
+            for (int i = 0; i < n && ok; ++i) {
+                const int g = g0 + i;
+                ok = wait(&p_full[g % Z::SLOTS], (g / Z::SLOTS) & 1, 64);
+                if (ok && i == 0 && c > 0) ok = wait(acc_free, (c - 1) & 1, 70);
+                if (!ok) break;
+                // the accumulators take the step; its stage is free then
+                const uint32_t at = ring_at + (g % Z::STAGES) * 2 * Z::STEP, p = tmem + Z::SLOT + (g % Z::SLOTS) * (2 * AB_N);
+                const uint64_t xs = tc_smem_desc(at, AB_N * 128, 1024), ys = tc_smem_desc(at + Z::STEP, AB_N * 128, 1024);
+                if (KEYS) {
+#pragma unroll
+                    for (int kk = 0; kk < AB_N / 16; ++kk)
+                        tc_mma_f16_ts_p(tmem + Z::ACC1, p + kk * 8, ys + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u, lead);
+                }
 #pragma unroll
                 for (int kk = 0; kk < AB_N / 16; ++kk)
-                    tc_mma_f16_ts_p(t_acc1, p + (kk >> 1) * 32 + (kk & 1) * 8, ys + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u, lead);
+                    tc_mma_f16_ts_p(tmem, p + AB_N + kk * 8, xs + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u, lead);
+                tc_mma_commit_p(&empty[g % Z::STAGES], lead);
+                if (i + Z::SLOTS < n) {
+                    // (the tensor core runs one thread's products in their order: the slot has been read by then)
+                    const int h = g + Z::SLOTS;
+                    ok = wait(&full[h % Z::STAGES], (h / Z::STAGES) & 1, 65);
+                    if (ok) scores(h);
+                    if (KEYS && ok && i + Z::SLOTS == n - 1) tc_mma_commit_p(own_free, lead);
+                }
             }
-#pragma unroll
-            for (int kk = 0; kk < AB_N / 16; ++kk)
-                tc_mma_f16_ts_p(t_acc0, p + 64 + (kk >> 1) * 32 + (kk & 1) * 8, xs + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u, lead);
-            tc_mma_commit_p(&empty[i % Z::STAGES], lead);
+            if (ok) tc_mma_commit_p(done, lead);
+            return ok;
         };
-        bool ok = n > 0 && wait(own, 0, 62);
-        for (int i = 0; i < SLOTS && i < n && ok; ++i) {
-            ok = wait(&full[i % Z::STAGES], (i / Z::STAGES) & 1, 63);
-            if (ok) scores(i);
+        for (int k = 0;; ++k) {
+            const int index = take(k);
+            if (index < 0) break;
+            const ab_item it = ab_decode(a, work, index);
+            if (it.n <= 0) continue;
+            if (!(it.keys ? walk(std::true_type(), it.n) : walk(std::false_type(), it.n))) break;
+            g0 += it.n;
+            ++c;
+            cq += !it.keys;
         }
-        for (int i = 0; i < n && ok; ++i) {
-            ok = wait(&p_full[i % SLOTS], (i / SLOTS) & 1, 64);
-            if (!ok) break;
-            sums(i);
-            if (const int k = i + SLOTS; k < n) {
-                // (the tensor core runs one thread's products in their order: the slot has been read by then)
-                ok = wait(&full[k % Z::STAGES], (k / Z::STAGES) & 1, 65);
-                if (ok) scores(k);
-            }
-        }
-        if (ok) tc_mma_commit_p(done, lead);
     } else if (warp >= 4) {
-        const int half = (warp - 4) >> 2;                       // which 32 columns of a step are this warpgroup's
+        const int group = (warp - 4) >> 2;                      // two warpgroups take the steps in turn
         const int r = (warp & 3) * 32 + lane;                   // row of the tile == TMEM lane
-        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-        const uint32_t at0 = t_slot + lane_off + half * 32;
-        const int row = row0 + r;
+        const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float sl = a.scale * AB_LOG2E;
-        const int kvh = KEYS ? head : head / grp;
-        const float most_v = __uint_as_float(w.most[kvh * 4 + 2]);
-        float shrink, row_nl = 0.f, row_d = 0.f;
-        if (KEYS) {
-            shrink = ab_shrink(__uint_as_float(w.most[kvh * 4]) * most_v + __uint_as_float(w.most[kvh * 4 + 1]));
-        } else {
-            const bool live = row < a.q_len;
-            const int64_t at_row = (int64_t)head * w.padded + row;
-            row_nl = live ? w.neg_lse[at_row] : -INFINITY;
-            row_d = live ? w.d[at_row] : 0.f;
-            shrink = ab_shrink((live ? w.norm[at_row] : 0.f) * most_v + fabsf(row_d));
-        }
-        const uint64_t sl2 = at_pack2(sl, sl), shrink2 = at_pack2(shrink, shrink);
-        const uint64_t row_nl2 = at_pack2(row_nl, row_nl), row_d2 = at_pack2(-row_d, -row_d);
-        bool ok = true;
-        for (int i = 0; i < n; ++i) {
-            const int slot = i % SLOTS;
-            const uint32_t at = at0 + slot * 128;
-            const int s0 = (first + (KEYS ? i % per_head : i)) * AB_N;          // first streamed row of the step
-            // columns [lo, hi) of this thread's are visible
-            int lo = 0, hi = 32;
-            bool masked = false;
-            if (KEYS) {
-                if (a.causal && (long long)row0 + AB_M - 1 > (long long)s0 + a.causal_delta) {
-                    const long long l = (long long)row - a.causal_delta - s0 - half * 32;
-                    lo = l < 0 ? 0 : l > 32 ? 32 : (int)l;
-                    masked = true;
-                }
-            } else {
-                if (s0 + AB_N > a.kv_len || (a.causal && (long long)s0 + AB_N - 1 > (long long)row0 + a.causal_delta)) {
-                    long long h = (long long)a.kv_len - s0;
-                    if (a.causal && (long long)row + a.causal_delta + 1 - s0 < h) h = (long long)row + a.causal_delta + 1 - s0;
-                    h -= half * 32;
-                    hi = h < 0 ? 0 : h > 32 ? 32 : (int)h;
-                    masked = true;
-                }
-            }
-            const float4* nl4 = reinterpret_cast<const float4*>(sRow + (i % Z::STAGES) * 2 * AB_N + half * 32);
-            const float4* d4 = nl4 + AB_N / 4;
-            bool there = tc_mbar_wait(&s_full[slot], (i / SLOTS) & 1, abort_flag, st, 66);
-            if (KEYS) there = there && tc_mbar_wait(&full[i % Z::STAGES], (i / Z::STAGES) & 1, abort_flag, st, 68);   // (the copies into sRow)
-            if (!__all_sync(0xffffffffu, there)) {
-                ok = false;
-                break;
-            }
+        const uint64_t sl2 = at_pack2(sl, sl);
+        int g0 = 0, c = 0;
+        bool of_keys_before = false;                            // the last walk was one of keys
+        // Queries: the first warpgroup moves X, the second Y, from shared memory (a row is 16-byte pieces, swizzled by its number) to
+        // TMEM.  `count`: the walk that they belong to.
+        auto own = [&](int count) {
+            // their place was the second accumulator of a walk of keys: both warpgroups have to have read it
+            if (of_keys_before && !__all_sync(0xffffffffu, tc_mbar_wait(acc_free, (count - 1) & 1, abort_flag, st, 74))) return false;
+            of_keys_before = false;
             tc_fence_after_sync();
-            uint32_t s[32], t[32];
-            tc_tmem_ld32(at, s);
-            tc_tmem_ld32(at + 64, t);
-            tc_tmem_ld_wait();
-            if (masked) {
+            if (!__all_sync(0xffffffffu, tc_mbar_wait(own_full, count & 1, abort_flag, st, 71))) return false;
+            const uint8_t* from = group ? sY : sX;
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                    if (j < lo || j >= hi) s[j] = 0xff800000u;                  // exp2 makes it a zero
-            }
-            uint32_t p16[16], s16[16];
+            for (int h = 0; h < HD / 64; ++h) {
+                uint32_t v[32];
 #pragma unroll
-            for (int j = 0; j < 32; j += 4) {
-                uint64_t nl2[2] = {row_nl2, row_nl2}, d2[2] = {row_d2, row_d2};
-                if (KEYS) {
-                    const float4 f = nl4[j >> 2], g = d4[j >> 2];
-                    nl2[0] = at_pack2(f.x, f.y), nl2[1] = at_pack2(f.z, f.w);
-                    d2[0] = at_pack2(-g.x, -g.y), d2[1] = at_pack2(-g.z, -g.w);
+                for (int q = 0; q < 8; ++q) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(from + h * (AB_M * 128) + r * 128 + ((q ^ (r & 7)) * 16));
+                    v[4 * q] = x.x, v[4 * q + 1] = x.y, v[4 * q + 2] = x.z, v[4 * q + 3] = x.w;
                 }
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int k = j + 2 * e;
-                    float x0, x1, y0, y1;
-                    at_unpack2(at_fma2(at_pack2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), sl2, nl2[e]), x0, x1);
-                    const float p0 = at_ex2(x0), p1 = at_ex2(x1);
-                    const uint64_t diff = at_add2(at_pack2(__uint_as_float(t[k]), __uint_as_float(t[k + 1])), d2[e]);
-                    at_unpack2(at_mul2(at_mul2(diff, shrink2), at_pack2(p0, p1)), y0, y1);
-                    const __half2 hp = __floats2half2_rn(p0, p1), hs = __floats2half2_rn(y0, y1);
-                    p16[k >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
-                    s16[k >> 1] = *reinterpret_cast<const uint32_t*>(&hs);
-                }
+                tc_tmem_st32(lanes + (group ? Z::Y : Z::X) + h * 32, v);
             }
-            // over the columns that this warpgroup has read: those of the other one may still be waited for
-            if (KEYS) tc_tmem_st16(at, p16);
-            tc_tmem_st16(at + 64, s16);
             tc_tmem_st_wait();
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) tc_mbar_arrive(&p_full[slot]);
-        }
-        if (ok && n > 0) ok = __all_sync(0xffffffffu, tc_mbar_wait(done, 0, abort_flag, st, 67)) != 0;
-        tc_fence_after_sync();
-        // results: keys: the first warpgroup dK, the second dV; queries: half of the columns of dQ each
-        const bool store = ok && row < row_end && *abort_flag == 0;
-        const float back = 0x1p-14f;
-        const bool of_v = KEYS && half == 1;
-        const int want = KEYS ? (of_v ? a.want & KTB_ATTN_DV : a.want & KTB_ATTN_DK) : a.want & KTB_ATTN_DQ;
-        const int64_t off = !KEYS ? a.dq_off + (int64_t)row * a.dq_row + (int64_t)head * a.dq_head
-                          : of_v  ? a.dv_off + (int64_t)row * a.dv_row + (int64_t)head * a.dv_head
-                                  : a.dk_off + (int64_t)row * a.dk_row + (int64_t)head * a.dk_head;
-        const float factor = of_v ? back : a.scale * (back / shrink);
-        constexpr int COLS = KEYS ? HD : HD / 2;
-        const int col0 = KEYS ? 0 : half * (HD / 2);
-        __half* dst = reinterpret_cast<__half*>(a.arena) + off + col0;
-        const uint32_t from = (of_v ? t_acc1 : t_acc0) + lane_off + col0;
-#pragma unroll
-        for (int c = 0; c < COLS; c += 32) {
-            uint32_t v[32];
-            if (n > 0 && ok) {                              // (the same for the whole warp)
-                tc_tmem_ld32(from + c, v);
-                tc_tmem_ld_wait();
+            if (lane == 0) tc_mbar_arrive(a_ready);
+            return true;
+        };
+        // One item: its steps, then its results.  `index` becomes the next item's.
+        auto walk = [&](auto of_keys, const ab_item& it, int k, int& index) -> bool {
+            constexpr bool KEYS = decltype(of_keys)::value;
+            const int row = it.row0 + r, kvh = KEYS ? it.head : it.head / grp;
+            float shrink = 1.f, row_nl = 0.f, row_d = 0.f;
+            if (KEYS) {
+                shrink = ab_shrink(__uint_as_float(w.most[kvh * 4]) * __uint_as_float(w.most[kvh * 4 + 2]) + __uint_as_float(w.most[kvh * 4 + 1]));
             } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = 0;
+                const bool live = row < a.q_len;
+                const int64_t at_row = (int64_t)it.head * w.padded + row;
+                row_nl = live ? w.neg_lse[at_row] : -INFINITY;
+                row_d = live ? w.d[at_row] : 0.f;
+                shrink = ab_shrink((live ? w.norm[at_row] : 0.f) * __uint_as_float(w.most[kvh * 4 + 2]) + fabsf(row_d));
             }
-            if (store && want) {
+            const uint64_t shrink2 = at_pack2(shrink, shrink);
+            const uint64_t row_nl2 = at_pack2(row_nl, row_nl), row_d2 = at_pack2(-row_d, -row_d);
+            int s = it.first + (((g0 & 1) != group) ? 1 : 0);   // streamed tile of the step
+            const int last = it.first + it.per_head;
+            if (KEYS && s >= last) s -= it.per_head;
+            for (int i = (g0 & 1) != group ? 1 : 0; i < it.n; i += 2) {
+                const int g = g0 + i;
+                const uint32_t slot = lanes + Z::SLOT + (g % Z::SLOTS) * (2 * AB_N);
+                const int s0 = s * AB_N;                        // first streamed row of the step
+                s += 2;
+                if (KEYS)
+                    while (s >= last) s -= it.per_head;
+                // columns [lo, hi) of this row are visible
+                int lo = 0, hi = AB_N;
+                bool masked = false;
+                if (KEYS) {
+                    if (a.causal && (long long)it.row0 + AB_M - 1 > (long long)s0 + a.causal_delta) {
+                        const long long l = (long long)row - a.causal_delta - s0;
+                        lo = l < 0 ? 0 : l > AB_N ? AB_N : (int)l;
+                        masked = true;
+                    }
+                } else {
+                    if (s0 + AB_N > a.kv_len || (a.causal && (long long)s0 + AB_N - 1 > (long long)it.row0 + a.causal_delta)) {
+                        long long h = (long long)a.kv_len - s0;
+                        if (a.causal && (long long)row + a.causal_delta + 1 - s0 < h) h = (long long)row + a.causal_delta + 1 - s0;
+                        hi = h < 0 ? 0 : h > AB_N ? AB_N : (int)h;
+                        masked = true;
+                    }
+                }
+                const float4* nl4 = reinterpret_cast<const float4*>(sRow + (g % Z::STAGES) * 2 * AB_N);
+                const float4* d4 = nl4 + AB_N / 4;
+                bool there = tc_mbar_wait(&s_full[g % Z::SLOTS], (g / Z::SLOTS) & 1, abort_flag, st, 66);
+                if (KEYS) there = there && tc_mbar_wait(&full[g % Z::STAGES], (g / Z::STAGES) & 1, abort_flag, st, 68);   // (the copies into sRow)
+                if (!__all_sync(0xffffffffu, there)) return false;
+                tc_fence_after_sync();
 #pragma unroll
-                for (int j = 0; j < 32; j += 8) {
-                    uint4 o;
-                    __half2* h = reinterpret_cast<__half2*>(&o);
+                for (int col = 0; col < AB_N; col += 32) {
+                    uint32_t s[32], t[32];
+                    tc_tmem_ld32(slot + col, s);
+                    tc_tmem_ld32(slot + AB_N + col, t);
+                    tc_tmem_ld_wait();
+                    if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        h[e] = __floats2half2_rn(__uint_as_float(v[j + 2 * e]) * factor, __uint_as_float(v[j + 2 * e + 1]) * factor);
-                    *reinterpret_cast<uint4*>(dst + c + j) = o;
+                        for (int j = 0; j < 32; ++j)
+                            if (col + j < lo || col + j >= hi) s[j] = 0xff800000u;      // exp2 makes it a zero
+                    }
+                    uint32_t p16[16], s16[16];
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4) {
+                        uint64_t nl2[2] = {row_nl2, row_nl2}, d2[2] = {row_d2, row_d2};
+                        if (KEYS) {
+                            const float4 f = nl4[(col + j) >> 2], e = d4[(col + j) >> 2];
+                            nl2[0] = at_pack2(f.x, f.y), nl2[1] = at_pack2(f.z, f.w);
+                            d2[0] = at_pack2(-e.x, -e.y), d2[1] = at_pack2(-e.z, -e.w);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const int q = j + 2 * e;
+                            float x0, x1, y0, y1;
+                            at_unpack2(at_fma2(at_pack2(__uint_as_float(s[q]), __uint_as_float(s[q + 1])), sl2, nl2[e]), x0, x1);
+                            const float p0 = at_ex2(x0), p1 = at_ex2(x1);
+                            const uint64_t diff = at_add2(at_pack2(__uint_as_float(t[q]), __uint_as_float(t[q + 1])), d2[e]);
+                            at_unpack2(at_mul2(at_mul2(diff, shrink2), at_pack2(p0, p1)), y0, y1);
+                            const __half2 hp = __floats2half2_rn(p0, p1), hs = __floats2half2_rn(y0, y1);
+                            p16[q >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
+                            s16[q >> 1] = *reinterpret_cast<const uint32_t*>(&hs);
+                        }
+                    }
+                    // (over columns that this thread has read)
+                    if (KEYS) tc_tmem_st16(slot + (col >> 1), p16);
+                    tc_tmem_st16(slot + AB_N + (col >> 1), s16);
+                }
+                tc_tmem_st_wait();
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc_mbar_arrive(&p_full[g % Z::SLOTS]);
+            }
+            if (it.n > 0) {
+                if (!__all_sync(0xffffffffu, tc_mbar_wait(done, c & 1, abort_flag, st, 67))) return false;
+                tc_fence_after_sync();
+            }
+            // Every product of this item has been made.  If the next one is of queries too, its X and Y go to TMEM before the results
+            // are read, so that its first scores are made meanwhile.
+            index = take(k + 1);
+            if (!KEYS && index >= 0) {
+                const ab_item then = ab_decode(a, work, index);
+                if (then.n > 0 && !own(c + (it.n > 0))) return false;
+            }
+            // results: keys: the first warpgroup dK, the second dV; queries: half of the columns of dQ each
+            const bool store = row < (KEYS ? a.dk_row0 + a.dk_rows : a.dq_row0 + a.dq_rows) && *abort_flag == 0;
+            const float back = 0x1p-14f;
+            const bool of_v = KEYS && group == 1;
+            const int want = KEYS ? (of_v ? a.want & KTB_ATTN_DV : a.want & KTB_ATTN_DK) : a.want & KTB_ATTN_DQ;
+            const int64_t off = !KEYS ? a.dq_off + (int64_t)row * a.dq_row + (int64_t)it.head * a.dq_head
+                              : of_v  ? a.dv_off + (int64_t)row * a.dv_row + (int64_t)it.head * a.dv_head
+                                      : a.dk_off + (int64_t)row * a.dk_row + (int64_t)it.head * a.dk_head;
+            const float factor = of_v ? back : a.scale * (back / shrink);
+            constexpr int COLS = KEYS ? HD : HD / 2;
+            const int col0 = KEYS ? 0 : group * (HD / 2);
+            __half* dst = reinterpret_cast<__half*>(a.arena) + off + col0;
+            const uint32_t from = lanes + (of_v ? Z::ACC1 : 0) + col0;
+#pragma unroll
+            for (int x = 0; x < COLS; x += 32) {
+                uint32_t v[32];
+                if (it.n > 0) {                                 // (the same for the whole warp)
+                    tc_tmem_ld32(from + x, v);
+                    tc_tmem_ld_wait();
+                    if (x + 32 == COLS) {                       // all read: the next item may sum
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) tc_mbar_arrive(acc_free);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0;
+                }
+                if (store && want) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8) {
+                        uint4 o;
+                        __half2* h = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            h[e] = __floats2half2_rn(__uint_as_float(v[j + 2 * e]) * factor, __uint_as_float(v[j + 2 * e + 1]) * factor);
+                        *reinterpret_cast<uint4*>(dst + x + j) = o;
+                    }
                 }
             }
+            return true;
+        };
+        int index = take(0);
+        bool keys_before = true;                                // the item before has not moved this one's X and Y
+        for (int k = 0; index >= 0; ++k) {
+            const ab_item it = ab_decode(a, work, index);
+            if (!it.keys && keys_before && it.n > 0 && !own(c)) break;
+            keys_before = it.keys;
+            if (it.n > 0) of_keys_before = it.keys;
+            if (!(it.keys ? walk(std::true_type(), it, k, index) : walk(std::false_type(), it, k, index))) break;
+            g0 += it.n;
+            c += it.n > 0;
         }
         tc_fence_before_sync();
     }
@@ -456,29 +604,7 @@ static int64_t ab_padded(const ktb_attn_bwd_args& a) { return ((int64_t)a.q_len 
 
 extern "C" int64_t ktb_attention_bwd_scratch_bytes(const ktb_attn_bwd_args* args) {
     if (!args || args->kv_group < 1 || args->heads < 1 || args->q_len < 1) return 0;
-    return (int64_t)(args->heads / args->kv_group) * 16 + 256 + 3 * 4 * (int64_t)args->heads * ab_padded(*args);
-}
-
-template <int HD, bool KEYS>
-static int ab_launch(ktb_ctx* ctx, const ktb_attn_bwd_args& a, const ab_scratch& w, const CUtensorMap& mq, const CUtensorMap& mk,
-                     const CUtensorMap& mv, const CUtensorMap& mg) {
-    const int rows = KEYS ? a.dk_rows : a.dq_rows, heads = KEYS ? a.dk_heads : a.dq_heads;
-    if (rows <= 0 || heads <= 0) return KTB_OK;
-    static bool attr_set[KTB_MAX_DEVICES] = {};     // the attribute is per device
-    if (!attr_set[ctx->device & (KTB_MAX_DEVICES - 1)]) {
-        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
-        attr_set[ctx->device & (KTB_MAX_DEVICES - 1)] = true;
-    }
-    const int tiles = (rows + AB_M - 1) / AB_M;
-    const long long items = (long long)tiles * heads;
-    if (items > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many tiles");
-    const int by_head = items >= 8ll * ctx->sm_count;
-    if (KEYS)
-        ktb_attention_bwd_kernel<HD, true><<<(int)items, 384, ab_shape<HD>::SMEM, ctx->stream>>>(mk, mv, mq, mg, a, w, tiles, heads, by_head, ctx->dev_status);
-    else
-        ktb_attention_bwd_kernel<HD, false><<<(int)items, 384, ab_shape<HD>::SMEM, ctx->stream>>>(mq, mg, mk, mv, a, w, tiles, heads, by_head, ctx->dev_status);
-    KTB_CHECK_LAUNCH(ctx, "ktb_attention_bwd_kernel");
-    return KTB_OK;
+    return (int64_t)(args->heads / args->kv_group) * 16 + 512 + 3 * 4 * (int64_t)args->heads * ab_padded(*args);
 }
 
 template <int HD>
@@ -486,23 +612,39 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     const int kv_heads = a.heads / a.kv_group;
     ab_scratch w;
     w.padded = ab_padded(a);
-    w.most = reinterpret_cast<unsigned*>(a.dev_scratch);
-    w.neg_lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.dev_scratch) + ((int64_t)kv_heads * 16 + 255) / 256 * 256);
+    w.taken = reinterpret_cast<unsigned*>(a.dev_scratch);
+    w.most = w.taken + 4;
+    w.neg_lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.dev_scratch) + ((int64_t)kv_heads * 16 + 16 + 255) / 256 * 256);
     w.d = w.neg_lse + (int64_t)a.heads * w.padded;
     w.norm = w.d + (int64_t)a.heads * w.padded;
     CUtensorMap mq, mk, mv, mg;
     if (!ab_map(&mq, a, a.q_off, a.q_len, a.heads, a.q_row, a.q_head) || !ab_map(&mg, a, a.do_off, a.q_len, a.heads, a.do_row, a.do_head) ||
         !ab_map(&mk, a, a.k_off, a.kv_len, kv_heads, a.k_row, a.k_head) || !ab_map(&mv, a, a.v_off, a.kv_len, kv_heads, a.v_row, a.v_head))
         return ktb_fail(ctx, KTB_E_CUDA, "attention_bwd", "cuTensorMapEncodeTiled failed");
-    KTB_CUDA(ctx, cudaMemsetAsync(w.most, 0, (size_t)kv_heads * 16, ctx->stream));
+    KTB_CUDA(ctx, cudaMemsetAsync(w.taken, 0, (size_t)kv_heads * 16 + 16, ctx->stream));
     const int q_blocks = (a.q_len + 63) / 64, k_blocks = (a.kv_len + 63) / 64;
     if (q_blocks + k_blocks > 65535) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "more than 2^21 positions");
     ktb_attention_rows_kernel<HD><<<dim3(a.heads, q_blocks + k_blocks), 256, 0, ctx->stream>>>(a, w, q_blocks);
     KTB_CHECK_LAUNCH(ctx, "ktb_attention_rows_kernel");
-    if (a.want & (KTB_ATTN_DK | KTB_ATTN_DV))
-        if (int rc = ab_launch<HD, true>(ctx, a, w, mq, mk, mv, mg)) return rc;
-    if (a.want & KTB_ATTN_DQ)
-        if (int rc = ab_launch<HD, false>(ctx, a, w, mq, mk, mv, mg)) return rc;
+    static bool attr_set[KTB_MAX_DEVICES] = {};     // the attribute is per device
+    if (!attr_set[ctx->device & (KTB_MAX_DEVICES - 1)]) {
+        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
+        attr_set[ctx->device & (KTB_MAX_DEVICES - 1)] = true;
+    }
+    ab_work work;
+    const bool keys = (a.want & (KTB_ATTN_DK | KTB_ATTN_DV)) && a.dk_rows > 0 && a.dk_heads > 0;
+    const bool queries = (a.want & KTB_ATTN_DQ) && a.dq_rows > 0 && a.dq_heads > 0;
+    work.key_tiles = keys ? (a.dk_rows + AB_M - 1) / AB_M : 0;
+    work.key_heads = keys ? a.dk_heads : 0;
+    work.query_tiles = queries ? (a.dq_rows + AB_M - 1) / AB_M : 0;
+    work.query_heads = queries ? a.dq_heads : 0;
+    const long long items = (long long)work.key_tiles * work.key_heads + (long long)work.query_tiles * work.query_heads;
+    if (items == 0) return KTB_OK;
+    if (items > 0x3fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many tiles");
+    work.by_head = items >= 16ll * ctx->sm_count;
+    const int grid = items < ctx->sm_count ? (int)items : ctx->sm_count;
+    ktb_attention_bwd_kernel<HD><<<grid, 384, ab_shape<HD>::SMEM, ctx->stream>>>(mq, mk, mv, mg, a, w, work, ctx->dev_status);
+    KTB_CHECK_LAUNCH(ctx, "ktb_attention_bwd_kernel");
     return KTB_OK;
 }
 

@@ -477,7 +477,7 @@ class AttentionDenseStatement(Statement):
 class AttentionGradStatement(Statement):
     """dQ, dK and dV, or some of them, of one attention: stores join as long as they are of the same tensors and mask."""
     kind = "attention_bwd"
-    launches = 4                                  # the statistics cleared, the rows' statistics, dK and dV, dQ
+    launches = 3                                  # maxima cleared, what the rows bring, the gradients
 
     def __init__(self, dev: R.Device, store: Store, arena: ArenaMap, stmt_id: int):
         self.dev, self.arena, self.id = dev, arena, stmt_id
@@ -599,7 +599,7 @@ class AttentionGradStatement(Statement):
         for ptr in self.device_arrays:
             self.dev.free(ptr)
         # per key head three maxima, per query head and query (in tiles of 64) three floats
-        a.scratch_bytes = k.heads * 16 + 256 + 12 * q.heads * (-(-q.rows // 64) * 64)
+        a.scratch_bytes = k.heads * 16 + 512 + 12 * q.heads * (-(-q.rows // 64) * 64)
         a.dev_scratch = self.dev.alloc(a.scratch_bytes)
         self.device_arrays = [a.dev_scratch]
         self.fps = _footprints(self.arena, walks.values(), writes, self.id)
