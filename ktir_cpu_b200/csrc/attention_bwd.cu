@@ -28,15 +28,23 @@
 #define AB_SHIFT 14.f
 #define AB_LOG2E 1.4426950408889634f
 
-// ---- what the rows bring: 14 - lse / ln 2, D, |dO| per row, and the largest norms --------------------------------
-// One block takes 64 rows of one head, LANES = head_dim / 8 threads a row.  blockIdx.y counts blocks of queries, then of keys.
+// A kernel that follows another on its stream may start while that one ends, up to where it waits; `ab_follow` allows it.
+static __device__ __forceinline__ void ab_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+static __device__ __forceinline__ void ab_wait_for_rows() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// ---- what the rows bring: 14 - lse / ln 2, D, |dO| per row, and the largest norms of a block of rows ---------------
+// HBM bounds it (O, dO and V once).  A block takes 256 heads of rows, 2^heads_log neighbouring heads of 256 >> heads_log rows (so
+// that what it reads lies together), head_dim / 8 threads each, four of their loads ahead of the arithmetic.
 struct ab_scratch {
     unsigned* taken;               // items handed out beyond the first of every CTA
     float* neg_lse;                // [heads][padded queries]
     float* d;
     float* norm;
-    unsigned* most;                // [key heads][4]: bits of max |dO|, max |D|, max |V|
+    float2* most_q;                // [heads][q_blocks]: largest |dO| and |D| of a block of queries
+    float* most_v;                 // [key heads][k_blocks]: largest |V| of a block of keys
     int64_t padded;
+    int q_log, k_log;              // heads_log for queries, for keys
+    int q_blocks, k_blocks;
 };
 
 static __device__ __forceinline__ float ab_dot8(uint4 a, uint4 b) {
@@ -53,74 +61,77 @@ static __device__ __forceinline__ float ab_dot8(uint4 a, uint4 b) {
 }
 
 template <int HD>
-__global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_bwd_args a, const ab_scratch w, int q_blocks) {
-    constexpr int LANES = HD / 8, ROWS = 256 / LANES;
-    const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
-    const int grp = a.kv_group;
+__global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_bwd_args a, const ab_scratch w) {
+    constexpr int LANES = HD / 8, GROUPS = 256 / LANES, BATCH = 4;
+    ab_follow();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *w.taken = 0;
+    const int lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
     const __half* base = reinterpret_cast<const __half*>(a.arena);
-    float most_a = 0.f, most_d = 0.f;
-    const bool keys = (int)blockIdx.y >= q_blocks;
-    const int64_t row0 = (int64_t)(keys ? blockIdx.y - q_blocks : blockIdx.y) * 64;
-    const int head = blockIdx.x;
-    if (keys && head >= a.heads / grp) return;
+    const int kv_heads = a.heads / a.kv_group;
+    const int q_wide = (a.heads + (1 << w.q_log) - 1) >> w.q_log, k_wide = (kv_heads + (1 << w.k_log) - 1) >> w.k_log;
+    const bool keys = blockIdx.x >= (unsigned)q_wide * w.q_blocks;
+    const int at = keys ? blockIdx.x - q_wide * w.q_blocks : blockIdx.x, wide = keys ? k_wide : q_wide, log = keys ? w.k_log : w.q_log;
+    const int block = at / wide, head0 = (at % wide) << log, heads = keys ? kv_heads : a.heads;
+    const int64_t row0 = (int64_t)block * (256 >> log), rows = keys ? a.kv_len : a.q_len;
+    const __half* from = base + (keys ? a.v_off : a.do_off) + lane * 8;
+    const __half* from_o = base + a.o_off + lane * 8;
+    const int64_t stride = keys ? a.v_row : a.do_row, head_stride = keys ? a.v_head : a.do_head;
+    // (a group's heads are all the same one when there are no more heads side by side than groups)
+    const int head = head0 + (group & ((1 << log) - 1));
+    float most = 0.f, most_d = 0.f;
+#pragma unroll 1
+    for (int i0 = 0; i0 < 256; i0 += BATCH * GROUPS) {
+        uint4 g[BATCH], o[BATCH];
+        float lse[BATCH];
 #pragma unroll
-    for (int i = 0; i < 64; i += ROWS) {
-        const int64_t row = row0 + i + r0;
-        if (keys) {
-            float v2 = 0.f;
-            if (row < a.kv_len) {
-                const uint4 v = *reinterpret_cast<const uint4*>(base + a.v_off + row * a.v_row + (int64_t)head * a.v_head + lane * 8);
-                v2 = ab_dot8(v, v);
+        for (int i = 0; i < BATCH; ++i) {
+            const int64_t row = row0 + ((i0 + i * GROUPS + group) >> log);
+            g[i] = o[i] = make_uint4(0, 0, 0, 0);
+            lse[i] = -INFINITY;
+            if (row < rows && head < heads) {
+                g[i] = *reinterpret_cast<const uint4*>(from + row * stride + head * head_stride);
+                if (!keys) {
+                    o[i] = *reinterpret_cast<const uint4*>(from_o + row * a.o_row + head * a.o_head);
+                    lse[i] = (reinterpret_cast<const float*>(a.arena) + a.lse_off)[row * a.lse_row + (int64_t)head * a.lse_head];
+                }
             }
-#pragma unroll
-            for (int o = LANES / 2; o; o >>= 1) v2 += __shfl_xor_sync(0xffffffffu, v2, o);
-            if (v2 <= 3.0e38f) most_a = fmaxf(most_a, v2);              // (a row with an infinity has no say)
-            continue;
-        }
-        float d = 0.f, g2 = 0.f;
-        if (row < a.q_len) {
-            const uint4 g = *reinterpret_cast<const uint4*>(base + a.do_off + row * a.do_row + (int64_t)head * a.do_head + lane * 8);
-            const uint4 o = *reinterpret_cast<const uint4*>(base + a.o_off + row * a.o_row + (int64_t)head * a.o_head + lane * 8);
-            d = ab_dot8(g, o);
-            g2 = ab_dot8(g, g);
         }
 #pragma unroll
-        for (int o = LANES / 2; o; o >>= 1) {
-            d += __shfl_xor_sync(0xffffffffu, d, o);
-            g2 += __shfl_xor_sync(0xffffffffu, g2, o);
-        }
-        if (lane == 0) {
-            float nl = -INFINITY;                                       // no probability: rows past the end, rows that see nothing
-            if (row < a.q_len) {
-                const float lse = (reinterpret_cast<const float*>(a.arena) + a.lse_off)[row * a.lse_row + (int64_t)head * a.lse_head];
-                if (lse != -INFINITY) nl = fmaf(-lse, AB_LOG2E, AB_SHIFT);
+        for (int i = 0; i < BATCH; ++i) {
+            const int64_t row = row0 + ((i0 + i * GROUPS + group) >> log);
+            float g2 = ab_dot8(g[i], g[i]), d = ab_dot8(g[i], o[i]);
+#pragma unroll
+            for (int x = LANES / 2; x; x >>= 1) {
+                g2 += __shfl_xor_sync(0xffffffffu, g2, x);
+                d += __shfl_xor_sync(0xffffffffu, d, x);
             }
-            const int64_t at = (int64_t)head * w.padded + row;
-            w.neg_lse[at] = nl;
-            w.d[at] = d;
-            w.norm[at] = g2 <= 3.0e38f ? sqrtf(g2) : 0.f;
+            g2 = g2 <= 3.0e38f ? g2 : 0.f;                              // (a row with an infinity has no say in the shift)
+            most = fmaxf(most, g2);
+            if (fabsf(d) <= 3.0e38f) most_d = fmaxf(most_d, fabsf(d));
+            if (!keys && lane == 0 && row < w.padded && head < heads) {
+                const int64_t to = (int64_t)head * w.padded + row;
+                // (no probability: rows past the end, rows that see nothing)
+                w.neg_lse[to] = lse[i] == -INFINITY ? -INFINITY : fmaf(-lse[i], AB_LOG2E, AB_SHIFT);
+                w.d[to] = d;
+                w.norm[to] = sqrtf(g2);
+            }
         }
-        if (g2 <= 3.0e38f) most_a = fmaxf(most_a, g2);
-        if (fabsf(d) <= 3.0e38f) most_d = fmaxf(most_d, fabsf(d));
     }
-    // largest of the block, one atomic each: a maximum does not depend on the order
-    __shared__ float sa[8], sd[8];
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        most_a = fmaxf(most_a, __shfl_xor_sync(0xffffffffu, most_a, o));
-        most_d = fmaxf(most_d, __shfl_xor_sync(0xffffffffu, most_d, o));
-    }
-    if ((threadIdx.x & 31) == 0) {
-        sa[threadIdx.x >> 5] = most_a;
-        sd[threadIdx.x >> 5] = most_d;
+    __shared__ float sa[GROUPS], sd[GROUPS];
+    if (lane == 0) {
+        sa[group] = most;
+        sd[group] = most_d;
     }
     __syncthreads();
-    if (threadIdx.x < 2) {
-        float m = 0.f;
-        for (int i = 0; i < 8; ++i) m = fmaxf(m, threadIdx.x ? sd[i] : sa[i]);
-        unsigned* to = w.most + (keys ? head : head / grp) * 4;
-        if (threadIdx.x == 0) atomicMax(to + (keys ? 2 : 0), __float_as_uint(sqrtf(m)));
-        else if (!keys) atomicMax(to + 1, __float_as_uint(m));
+    const int mine = threadIdx.x;
+    if (mine < (1 << log) && head0 + mine < heads) {
+        most = most_d = 0.f;
+        for (int i = mine; i < GROUPS; i += 1 << log) {
+            most = fmaxf(most, sa[i]);
+            most_d = fmaxf(most_d, sd[i]);
+        }
+        if (keys) w.most_v[(int64_t)(head0 + mine) * w.k_blocks + block] = sqrtf(most);
+        else w.most_q[(int64_t)(head0 + mine) * w.q_blocks + block] = make_float2(sqrtf(most), most_d);
     }
 }
 
@@ -137,11 +148,14 @@ struct ab_shape {
     static constexpr int BLOCKS = HD / 64;                  // 64-column blocks of a tile (a 128-byte swizzled row each)
     static constexpr int OWN = AB_M * HD * 2;               // bytes of X, of Y
     static constexpr int STEP = AB_N * HD * 2;              // bytes of X', of Y'
-    static constexpr int STAGES = 4;
-    static constexpr size_t SMEM = 2 * OWN + STAGES * (2 * STEP + 2 * AB_N * 4) + 1024 + 256;
+    static constexpr int STAGES = HD == 64 ? 8 : 4;         // 128 KB of the stream on its way
+    static constexpr size_t SMEM = 2 * OWN + STAGES * (2 * STEP + 2 * AB_N * 4) + 1024 + 512;
     // columns of TMEM: two accumulators (for queries X and Y as f16 pairs in place of the second), then the slots: S and T
     static constexpr int ACC1 = HD, X = HD, Y = HD + HD / 2, SLOT = 2 * HD;
     static constexpr int SLOTS = (512 - SLOT) / (2 * AB_N);
+    // With two slots a step's way from its scores to its sums and back is what a step takes: it is cut in two (see the softmax).
+    // Where three slots hide it the cut only costs barriers (64 wide, a step of keys 0.60 us, cut 0.62; 128 wide 0.88, cut 0.79).
+    static constexpr bool CUT = SLOTS < 3;
 };
 
 // Waits for a phase no matter what else has failed, so that no copy is under way into memory that the CTA gives up.
@@ -210,8 +224,8 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     uint64_t* full = reinterpret_cast<uint64_t*>(sRow + Z::STAGES * 2 * AB_N);
     uint64_t *empty = full + Z::STAGES, *own_full = empty + Z::STAGES, *own_free = own_full + 1, *a_ready = own_free + 1;
     uint64_t *acc_free = a_ready + 1, *done = acc_free + 1, *next_full = done + 1, *next_free = next_full + 2;
-    uint64_t *s_full = next_free + 2, *p_full = s_full + Z::SLOTS;
-    volatile int* next = reinterpret_cast<volatile int*>(p_full + Z::SLOTS);    // items handed out, two at a time
+    uint64_t *s_full = next_free + 2, *t_full = s_full + Z::SLOTS, *p_full = t_full + Z::SLOTS;     // p_full: per slot and half of its columns
+    volatile int* next = reinterpret_cast<volatile int*>(p_full + 2 * Z::SLOTS);        // items handed out, two at a time
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(next) + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
@@ -233,7 +247,9 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         for (int i = 0; i < Z::SLOTS; ++i) {
             tc_mbar_init(&s_full[i], 1);
-            tc_mbar_init(&p_full[i], 4);
+            tc_mbar_init(&t_full[i], 1);
+            tc_mbar_init(&p_full[2 * i], 4);
+            tc_mbar_init(&p_full[2 * i + 1], 4);
         }
         *abort_flag = 0;
         tc_fence_barrier_init();
@@ -263,12 +279,14 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             bool ok = true;
             for (int k = 0; ok; ++k) {
                 const int q = k & 1;
+                if (k == 1) ab_wait_for_rows();
                 const int index = k == 0 ? (int)blockIdx.x : (int)(gridDim.x + atomicAdd(w.taken, 1u));
                 if (k >= 2 && !tc_mbar_wait(&next_free[q], ((k >> 1) - 1) & 1, abort_flag, st, 73)) break;
                 next[q] = index;
                 tc_mbar_arrive(&next_full[q]);
                 if (index >= total) break;
                 const ab_item it = ab_decode(a, work, index);
+                if (k == 0 && it.keys) ab_wait_for_rows();
                 const CUtensorMap *mx = it.keys ? &map_q : &map_k, *my = it.keys ? &map_g : &map_v;
                 int sh = it.keys ? it.head * grp : it.head / grp, s = 0;                             // streamed head and step of it
                 for (int i = 0; i < it.n; ++i, ++t) {
@@ -321,13 +339,13 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         }
         if (lane == 0 && *abort_flag && c > 0) ab_drain(own_full, (c - 1) & 1);
     } else if (warp == 1) {
+        if (tc_elect_one()) {
         // the warp runs this converged; one elected lane issues the tcgen05 instructions
-        const uint32_t lead = tc_elect_one();
         const uint32_t idesc_s = tc_idesc_f16(AB_M, AB_N, 0, 0), idesc_a = tc_idesc_f16(AB_M, HD, 0, 1);
         const uint64_t xd = tc_smem_desc(tc_smem_u32(sX), 16, 1024), yd = tc_smem_desc(tc_smem_u32(sY), 16, 1024);
         const uint32_t ring_at = tc_smem_u32(ring);
         auto wait = [&](uint64_t* bar, uint32_t parity, int site) {
-            const bool ok = __all_sync(0xffffffffu, tc_mbar_wait(bar, parity, abort_flag, st, site)) != 0;
+            const bool ok = tc_mbar_wait(bar, parity, abort_flag, st, site);
             tc_fence_after_sync();
             return ok;
         };
@@ -342,55 +360,62 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk) {
                     const uint32_t ao = ((kk >> 2) * (AB_M * 128) + (kk & 3) * 32) >> 4, bo = ((kk >> 2) * (AB_N * 128) + (kk & 3) * 32) >> 4;
-                    if (KEYS) tc_mma_f16_p(d, xd + ao, xs + bo, idesc_s, kk != 0, lead);
-                    else tc_mma_f16_ts_p(d, tmem + Z::X + kk * 8, xs + bo, idesc_s, kk != 0, lead);
+                    if (KEYS) tc_mma_f16(d, xd + ao, xs + bo, idesc_s, kk != 0);
+                    else tc_mma_f16_ts(d, tmem + Z::X + kk * 8, xs + bo, idesc_s, kk != 0);
                 }
+                if (Z::CUT) tc_mma_commit(&s_full[g % Z::SLOTS]);
 #pragma unroll
                 for (int kk = 0; kk < HD / 16; ++kk) {
                     const uint32_t ao = ((kk >> 2) * (AB_M * 128) + (kk & 3) * 32) >> 4, bo = ((kk >> 2) * (AB_N * 128) + (kk & 3) * 32) >> 4;
-                    if (KEYS) tc_mma_f16_p(d + AB_N, yd + ao, ys + bo, idesc_s, kk != 0, lead);
-                    else tc_mma_f16_ts_p(d + AB_N, tmem + Z::Y + kk * 8, ys + bo, idesc_s, kk != 0, lead);
+                    if (KEYS) tc_mma_f16(d + AB_N, yd + ao, ys + bo, idesc_s, kk != 0);
+                    else tc_mma_f16_ts(d + AB_N, tmem + Z::Y + kk * 8, ys + bo, idesc_s, kk != 0);
                 }
-                tc_mma_commit_p(&s_full[g % Z::SLOTS], lead);
+                tc_mma_commit(&(Z::CUT ? t_full : s_full)[g % Z::SLOTS]);
             };
             bool ok = wait(KEYS ? own_full : a_ready, (KEYS ? c : cq) & 1, 62);
-            if (!KEYS && ok && lane == 0) tc_mbar_arrive(own_free);             // the softmax has moved them to TMEM
+            if (!KEYS && ok) tc_mbar_arrive(own_free);             // the softmax has moved them to TMEM
             for (int i = 0; i < Z::SLOTS && i < n && ok; ++i) {
                 ok = wait(&full[(g0 + i) % Z::STAGES], ((g0 + i) / Z::STAGES) & 1, 63);
                 if (ok) scores(g0 + i);
             }
-            if (KEYS && ok && n <= Z::SLOTS) tc_mma_commit_p(own_free, lead);   // (X and Y have been read when these products are done)
+            if (KEYS && ok && n <= Z::SLOTS) tc_mma_commit(own_free);   // (X and Y have been read when these products are done)
             for (int i = 0; i < n && ok; ++i) {
                 const int g = g0 + i;
-                ok = wait(&p_full[g % Z::SLOTS], (g / Z::SLOTS) & 1, 64);
-                if (ok && i == 0 && c > 0) ok = wait(acc_free, (c - 1) & 1, 70);
-                if (!ok) break;
-                // the accumulators take the step; its stage is free then
                 const uint32_t at = ring_at + (g % Z::STAGES) * 2 * Z::STEP, p = tmem + Z::SLOT + (g % Z::SLOTS) * (2 * AB_N);
                 const uint64_t xs = tc_smem_desc(at, AB_N * 128, 1024), ys = tc_smem_desc(at + Z::STEP, AB_N * 128, 1024);
-                if (KEYS) {
+                // the accumulators take the step, half by half where it is cut; its stage is free then
 #pragma unroll
-                    for (int kk = 0; kk < AB_N / 16; ++kk)
-                        tc_mma_f16_ts_p(tmem + Z::ACC1, p + kk * 8, ys + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u, lead);
+                for (int h = 0; h < 2; ++h) {
+                    if (Z::CUT || h == 0) ok = ok && wait(&p_full[(g % Z::SLOTS) * 2 + h], (g / Z::SLOTS) & 1, 64);
+                    if (ok && h == 0 && i == 0 && c > 0) ok = wait(acc_free, (c - 1) & 1, 70);
+                    if (!ok) break;
+                    if (KEYS) {
+#pragma unroll
+                        for (int kk = 2 * h; kk < 2 * h + 2; ++kk)
+                            tc_mma_f16_ts(tmem + Z::ACC1, p + kk * 8, ys + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u);
+                    }
+#pragma unroll
+                    for (int kk = 2 * h; kk < 2 * h + 2; ++kk)
+                        tc_mma_f16_ts(tmem, p + AB_N + kk * 8, xs + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u);
                 }
-#pragma unroll
-                for (int kk = 0; kk < AB_N / 16; ++kk)
-                    tc_mma_f16_ts_p(tmem, p + AB_N + kk * 8, xs + (uint32_t)(kk * 2048 >> 4), idesc_a, (i > 0 || kk > 0) ? 1u : 0u, lead);
-                tc_mma_commit_p(&empty[g % Z::STAGES], lead);
+                if (!ok) break;
+                tc_mma_commit(&empty[g % Z::STAGES]);
                 if (i + Z::SLOTS < n) {
                     // (the tensor core runs one thread's products in their order: the slot has been read by then)
                     const int h = g + Z::SLOTS;
                     ok = wait(&full[h % Z::STAGES], (h / Z::STAGES) & 1, 65);
                     if (ok) scores(h);
-                    if (KEYS && ok && i + Z::SLOTS == n - 1) tc_mma_commit_p(own_free, lead);
+                    if (KEYS && ok && i + Z::SLOTS == n - 1) tc_mma_commit(own_free);
                 }
             }
-            if (ok) tc_mma_commit_p(done, lead);
+            if (ok) tc_mma_commit(done);
             return ok;
         };
         for (int k = 0;; ++k) {
-            const int index = take(k);
-            if (index < 0) break;
+            if (!tc_mbar_wait(&next_full[k & 1], (k >> 1) & 1, abort_flag, st, 72)) break;
+            const int index = next[k & 1];
+            tc_mbar_arrive(&next_free[k & 1]);
+            if (index >= total) break;
             const ab_item it = ab_decode(a, work, index);
             if (it.n <= 0) continue;
             if (!(it.keys ? walk(std::true_type(), it.n) : walk(std::false_type(), it.n))) break;
@@ -398,12 +423,14 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             ++c;
             cq += !it.keys;
         }
+        }
     } else if (warp >= 4) {
         const int group = (warp - 4) >> 2;                      // two warpgroups take the steps in turn
         const int r = (warp & 3) * 32 + lane;                   // row of the tile == TMEM lane
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         const float sl = a.scale * AB_LOG2E;
         const uint64_t sl2 = at_pack2(sl, sl);
+        ab_wait_for_rows();
         int g0 = 0, c = 0;
         bool of_keys_before = false;                            // the last walk was one of keys
         // Queries: the first warpgroup moves X, the second Y, from shared memory (a row is 16-byte pieces, swizzled by its number) to
@@ -431,20 +458,40 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (lane == 0) tc_mbar_arrive(a_ready);
             return true;
         };
+        // What an item needs of its rows, asked for while the item before it ends: the largest |dO|, |D| and |V| of its key head
+        // (this lane's share of them), and of a query row 14 - lse / ln 2, D and |dO|.
+        struct ab_known { float most_g, most_d, most_v, nl, d, norm; };
+        auto ask = [&](const ab_item& it) {
+            ab_known v = {0.f, 0.f, 0.f, -INFINITY, 0.f, 0.f};
+            const int kvh = it.keys ? it.head : it.head / grp;
+            if (it.keys) {
+                for (int i = lane; i < w.q_blocks * grp; i += 32) {
+                    const float2 m = w.most_q[(int64_t)kvh * grp * w.q_blocks + i];
+                    v.most_g = fmaxf(v.most_g, m.x);
+                    v.most_d = fmaxf(v.most_d, m.y);
+                }
+            } else if (it.row0 + r < a.q_len) {
+                const int64_t at = (int64_t)it.head * w.padded + it.row0 + r;
+                v.nl = w.neg_lse[at];
+                v.d = w.d[at];
+                v.norm = w.norm[at];
+            }
+            for (int i = lane; i < w.k_blocks; i += 32) v.most_v = fmaxf(v.most_v, w.most_v[(int64_t)kvh * w.k_blocks + i]);
+            return v;
+        };
+        auto of_warp = [&](float x) {
+#pragma unroll
+            for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            return x;
+        };
+        ab_known known = {};
         // One item: its steps, then its results.  `index` becomes the next item's.
         auto walk = [&](auto of_keys, const ab_item& it, int k, int& index) -> bool {
             constexpr bool KEYS = decltype(of_keys)::value;
-            const int row = it.row0 + r, kvh = KEYS ? it.head : it.head / grp;
-            float shrink = 1.f, row_nl = 0.f, row_d = 0.f;
-            if (KEYS) {
-                shrink = ab_shrink(__uint_as_float(w.most[kvh * 4]) * __uint_as_float(w.most[kvh * 4 + 2]) + __uint_as_float(w.most[kvh * 4 + 1]));
-            } else {
-                const bool live = row < a.q_len;
-                const int64_t at_row = (int64_t)it.head * w.padded + row;
-                row_nl = live ? w.neg_lse[at_row] : -INFINITY;
-                row_d = live ? w.d[at_row] : 0.f;
-                shrink = ab_shrink((live ? w.norm[at_row] : 0.f) * __uint_as_float(w.most[kvh * 4 + 2]) + fabsf(row_d));
-            }
+            const int row = it.row0 + r;
+            const float most_v = of_warp(known.most_v);
+            const float row_nl = known.nl, row_d = known.d;
+            const float shrink = KEYS ? ab_shrink(of_warp(known.most_g) * most_v + of_warp(known.most_d)) : ab_shrink(known.norm * most_v + fabsf(row_d));
             const uint64_t shrink2 = at_pack2(shrink, shrink);
             const uint64_t row_nl2 = at_pack2(row_nl, row_nl), row_d2 = at_pack2(-row_d, -row_d);
             int s = it.first + (((g0 & 1) != group) ? 1 : 0);   // streamed tile of the step
@@ -474,53 +521,119 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         masked = true;
                     }
                 }
-                const float4* nl4 = reinterpret_cast<const float4*>(sRow + (g % Z::STAGES) * 2 * AB_N);
-                const float4* d4 = nl4 + AB_N / 4;
-                bool there = tc_mbar_wait(&s_full[g % Z::SLOTS], (g / Z::SLOTS) & 1, abort_flag, st, 66);
-                if (KEYS) there = there && tc_mbar_wait(&full[g % Z::STAGES], (g / Z::STAGES) & 1, abort_flag, st, 68);   // (the copies into sRow)
+                // Half of the columns at a time.  Cut: P needs S alone, so that T may still be in the making; the sums over the first half
+                // are made while the second one is worked on.  (Row values are asked for early: shared memory is busy with operands.)
+                const float4* rows = reinterpret_cast<const float4*>(sRow + (g % Z::STAGES) * 2 * AB_N);
+                float4 nl[8], dd[8];
+                bool there = true;
+                if (KEYS) {
+                    there = tc_mbar_wait(&full[g % Z::STAGES], (g / Z::STAGES) & 1, abort_flag, st, 68);        // (the copies into sRow)
+                    if (Z::CUT) {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) nl[j] = rows[j];
+                    }
+                }
+                there = there && tc_mbar_wait(&s_full[g % Z::SLOTS], (g / Z::SLOTS) & 1, abort_flag, st, 66);
                 if (!__all_sync(0xffffffffu, there)) return false;
                 tc_fence_after_sync();
+                if constexpr (Z::CUT) {
 #pragma unroll
-                for (int col = 0; col < AB_N; col += 32) {
-                    uint32_t s[32], t[32];
-                    tc_tmem_ld32(slot + col, s);
-                    tc_tmem_ld32(slot + AB_N + col, t);
-                    tc_tmem_ld_wait();
-                    if (masked) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (col + j < lo || col + j >= hi) s[j] = 0xff800000u;      // exp2 makes it a zero
-                    }
-                    uint32_t p16[16], s16[16];
-#pragma unroll
-                    for (int j = 0; j < 32; j += 4) {
-                        uint64_t nl2[2] = {row_nl2, row_nl2}, d2[2] = {row_d2, row_d2};
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t s[32], t[32], half16[16];
+                        tc_tmem_ld32(slot + 32 * h, s);
                         if (KEYS) {
-                            const float4 f = nl4[(col + j) >> 2], e = d4[(col + j) >> 2];
-                            nl2[0] = at_pack2(f.x, f.y), nl2[1] = at_pack2(f.z, f.w);
-                            d2[0] = at_pack2(-e.x, -e.y), d2[1] = at_pack2(-e.z, -e.w);
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) dd[j] = rows[AB_N / 4 + 8 * h + j];
+                        }
+                        tc_tmem_ld_wait();
+                        if (masked) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (32 * h + j < lo || 32 * h + j >= hi) s[j] = 0xff800000u;        // exp2 makes it a zero
+                        }
+                        float p[32];
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            uint64_t nl2 = row_nl2;
+                            if (KEYS) nl2 = (j & 2) ? at_pack2(nl[j >> 2].z, nl[j >> 2].w) : at_pack2(nl[j >> 2].x, nl[j >> 2].y);
+                            float x0, x1;
+                            at_unpack2(at_fma2(at_pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), sl2, nl2), x0, x1);
+                            p[j] = at_ex2(x0);
+                            p[j + 1] = at_ex2(x1);
+                            const __half2 hp = __floats2half2_rn(p[j], p[j + 1]);
+                            half16[j >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
+                        }
+                        // (over columns that this thread has read)
+                        if (KEYS) tc_tmem_st16(slot + 16 * h, half16);
+                        if (h == 0) {
+                            if (!__all_sync(0xffffffffu, tc_mbar_wait(&t_full[g % Z::SLOTS], (g / Z::SLOTS) & 1, abort_flag, st, 75))) return false;
+                            tc_fence_after_sync();
+                        }
+                        tc_tmem_ld32(slot + AB_N + 32 * h, t);
+                        if (KEYS && h == 0) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) nl[j] = rows[8 + j];
+                        }
+                        tc_tmem_ld_wait();
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            uint64_t d2 = row_d2;
+                            if (KEYS) d2 = (j & 2) ? at_pack2(-dd[j >> 2].z, -dd[j >> 2].w) : at_pack2(-dd[j >> 2].x, -dd[j >> 2].y);
+                            float y0, y1;
+                            const uint64_t diff = at_add2(at_pack2(__uint_as_float(t[j]), __uint_as_float(t[j + 1])), d2);
+                            at_unpack2(at_mul2(at_mul2(diff, shrink2), at_pack2(p[j], p[j + 1])), y0, y1);
+                            const __half2 hs = __floats2half2_rn(y0, y1);
+                            half16[j >> 1] = *reinterpret_cast<const uint32_t*>(&hs);
+                        }
+                        tc_tmem_st16(slot + AB_N + 16 * h, half16);
+                        tc_tmem_st_wait();
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) tc_mbar_arrive(&p_full[(g % Z::SLOTS) * 2 + h]);
+                    }
+                } else {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        uint32_t s[32], t[32], p16[16], s16[16];
+                        tc_tmem_ld32(slot + 32 * h, s);
+                        tc_tmem_ld32(slot + AB_N + 32 * h, t);
+                        tc_tmem_ld_wait();
+                        if (masked) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j)
+                                if (32 * h + j < lo || 32 * h + j >= hi) s[j] = 0xff800000u;
                         }
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int q = j + 2 * e;
+                        for (int j = 0; j < 32; j += 2) {
+                            uint64_t nl2 = row_nl2, d2 = row_d2;
+                            if (KEYS) {
+                                if (j % 4 == 0) nl[0] = rows[8 * h + j / 4], dd[0] = rows[AB_N / 4 + 8 * h + j / 4];
+                                nl2 = (j & 2) ? at_pack2(nl[0].z, nl[0].w) : at_pack2(nl[0].x, nl[0].y);
+                                d2 = (j & 2) ? at_pack2(-dd[0].z, -dd[0].w) : at_pack2(-dd[0].x, -dd[0].y);
+                            }
                             float x0, x1, y0, y1;
-                            at_unpack2(at_fma2(at_pack2(__uint_as_float(s[q]), __uint_as_float(s[q + 1])), sl2, nl2[e]), x0, x1);
+                            at_unpack2(at_fma2(at_pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), sl2, nl2), x0, x1);
                             const float p0 = at_ex2(x0), p1 = at_ex2(x1);
-                            const uint64_t diff = at_add2(at_pack2(__uint_as_float(t[q]), __uint_as_float(t[q + 1])), d2[e]);
+                            const uint64_t diff = at_add2(at_pack2(__uint_as_float(t[j]), __uint_as_float(t[j + 1])), d2);
                             at_unpack2(at_mul2(at_mul2(diff, shrink2), at_pack2(p0, p1)), y0, y1);
                             const __half2 hp = __floats2half2_rn(p0, p1), hs = __floats2half2_rn(y0, y1);
-                            p16[q >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
-                            s16[q >> 1] = *reinterpret_cast<const uint32_t*>(&hs);
+                            p16[j >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
+                            s16[j >> 1] = *reinterpret_cast<const uint32_t*>(&hs);
                         }
+                        if (KEYS) tc_tmem_st16(slot + 16 * h, p16);
+                        tc_tmem_st16(slot + AB_N + 16 * h, s16);
                     }
-                    // (over columns that this thread has read)
-                    if (KEYS) tc_tmem_st16(slot + (col >> 1), p16);
-                    tc_tmem_st16(slot + AB_N + (col >> 1), s16);
+                    tc_tmem_st_wait();
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) tc_mbar_arrive(&p_full[(g % Z::SLOTS) * 2]);
                 }
-                tc_tmem_st_wait();
-                tc_fence_before_sync();
-                __syncwarp();
-                if (lane == 0) tc_mbar_arrive(&p_full[g % Z::SLOTS]);
+            }
+            index = take(k + 1);
+            ab_item then = it;
+            if (index >= 0) {
+                then = ab_decode(a, work, index);
+                known = ask(then);
             }
             if (it.n > 0) {
                 if (!__all_sync(0xffffffffu, tc_mbar_wait(done, c & 1, abort_flag, st, 67))) return false;
@@ -528,11 +641,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             }
             // Every product of this item has been made.  If the next one is of queries too, its X and Y go to TMEM before the results
             // are read, so that its first scores are made meanwhile.
-            index = take(k + 1);
-            if (!KEYS && index >= 0) {
-                const ab_item then = ab_decode(a, work, index);
-                if (then.n > 0 && !own(c + (it.n > 0))) return false;
-            }
+            if (!KEYS && index >= 0 && then.n > 0 && !own(c + (it.n > 0))) return false;
             // results: keys: the first warpgroup dK, the second dV; queries: half of the columns of dQ each
             const bool store = row < (KEYS ? a.dk_row0 + a.dk_rows : a.dq_row0 + a.dq_rows) && *abort_flag == 0;
             const float back = 0x1p-14f;
@@ -576,6 +685,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             return true;
         };
         int index = take(0);
+        if (index >= 0) known = ask(ab_decode(a, work, index));
         bool keys_before = true;                                // the item before has not moved this one's X and Y
         for (int k = 0; index >= 0; ++k) {
             const ab_item it = ab_decode(a, work, index);
@@ -602,9 +712,16 @@ static bool ab_map(CUtensorMap* m, const ktb_attn_bwd_args& a, int64_t off, int6
 
 static int64_t ab_padded(const ktb_attn_bwd_args& a) { return ((int64_t)a.q_len + AB_N - 1) / AB_N * AB_N; }
 
+// Neighbouring heads that a block of the rows kernel takes (a power of two, eight at most), and the rows of it.
+static int ab_heads_log(int heads) { return heads >= 8 ? 3 : heads >= 4 ? 2 : heads >= 2 ? 1 : 0; }
+static int64_t ab_row_blocks(int64_t rows, int heads) { return (rows + (256 >> ab_heads_log(heads)) - 1) / (256 >> ab_heads_log(heads)); }
+
+// Counter; per query and head three floats; per block of queries and head two, per block of keys and key head one.
 extern "C" int64_t ktb_attention_bwd_scratch_bytes(const ktb_attn_bwd_args* args) {
-    if (!args || args->kv_group < 1 || args->heads < 1 || args->q_len < 1) return 0;
-    return (int64_t)(args->heads / args->kv_group) * 16 + 512 + 3 * 4 * (int64_t)args->heads * ab_padded(*args);
+    if (!args || args->kv_group < 1 || args->heads < args->kv_group || args->q_len < 1 || args->kv_len < 1) return 0;
+    const int kv_heads = args->heads / args->kv_group;
+    return 256 + 4 * (int64_t)args->heads * (3 * ab_padded(*args) + 2 * ab_row_blocks(ab_padded(*args), args->heads)) +
+           4 * kv_heads * ab_row_blocks(args->kv_len, kv_heads);
 }
 
 template <int HD>
@@ -612,19 +729,23 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     const int kv_heads = a.heads / a.kv_group;
     ab_scratch w;
     w.padded = ab_padded(a);
+    w.q_log = ab_heads_log(a.heads);
+    w.k_log = ab_heads_log(kv_heads);
+    w.q_blocks = (int)ab_row_blocks(w.padded, a.heads);
+    w.k_blocks = (int)ab_row_blocks(a.kv_len, kv_heads);
+    const int64_t row_blocks = (int64_t)w.q_blocks * ((a.heads + (1 << w.q_log) - 1) >> w.q_log) + (int64_t)w.k_blocks * ((kv_heads + (1 << w.k_log) - 1) >> w.k_log);
+    if (row_blocks > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many rows");
     w.taken = reinterpret_cast<unsigned*>(a.dev_scratch);
-    w.most = w.taken + 4;
-    w.neg_lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.dev_scratch) + ((int64_t)kv_heads * 16 + 16 + 255) / 256 * 256);
+    w.neg_lse = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(a.dev_scratch) + 256);
     w.d = w.neg_lse + (int64_t)a.heads * w.padded;
     w.norm = w.d + (int64_t)a.heads * w.padded;
+    w.most_q = reinterpret_cast<float2*>(w.norm + (int64_t)a.heads * w.padded);
+    w.most_v = reinterpret_cast<float*>(w.most_q + (int64_t)a.heads * w.q_blocks);
     CUtensorMap mq, mk, mv, mg;
     if (!ab_map(&mq, a, a.q_off, a.q_len, a.heads, a.q_row, a.q_head) || !ab_map(&mg, a, a.do_off, a.q_len, a.heads, a.do_row, a.do_head) ||
         !ab_map(&mk, a, a.k_off, a.kv_len, kv_heads, a.k_row, a.k_head) || !ab_map(&mv, a, a.v_off, a.kv_len, kv_heads, a.v_row, a.v_head))
         return ktb_fail(ctx, KTB_E_CUDA, "attention_bwd", "cuTensorMapEncodeTiled failed");
-    KTB_CUDA(ctx, cudaMemsetAsync(w.taken, 0, (size_t)kv_heads * 16 + 16, ctx->stream));
-    const int q_blocks = (a.q_len + 63) / 64, k_blocks = (a.kv_len + 63) / 64;
-    if (q_blocks + k_blocks > 65535) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "more than 2^21 positions");
-    ktb_attention_rows_kernel<HD><<<dim3(a.heads, q_blocks + k_blocks), 256, 0, ctx->stream>>>(a, w, q_blocks);
+    ktb_attention_rows_kernel<HD><<<(unsigned)row_blocks, 256, 0, ctx->stream>>>(a, w);
     KTB_CHECK_LAUNCH(ctx, "ktb_attention_rows_kernel");
     static bool attr_set[KTB_MAX_DEVICES] = {};     // the attribute is per device
     if (!attr_set[ctx->device & (KTB_MAX_DEVICES - 1)]) {
@@ -643,7 +764,18 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     if (items > 0x3fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many tiles");
     work.by_head = items >= 16ll * ctx->sm_count;
     const int grid = items < ctx->sm_count ? (int)items : ctx->sm_count;
-    ktb_attention_bwd_kernel<HD><<<grid, 384, ab_shape<HD>::SMEM, ctx->stream>>>(mq, mk, mv, mg, a, w, work, ctx->dev_status);
+    // It sets up, and fetches what does not come from the kernel before it, while that one ends.
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(384);
+    config.dynamicSmemBytes = ab_shape<HD>::SMEM;
+    config.stream = ctx->stream;
+    config.attrs = &early;
+    config.numAttrs = 1;
+    KTB_CUDA(ctx, cudaLaunchKernelEx(&config, ktb_attention_bwd_kernel<HD>, mq, mk, mv, mg, a, w, work, ctx->dev_status));
     KTB_CHECK_LAUNCH(ctx, "ktb_attention_bwd_kernel");
     return KTB_OK;
 }

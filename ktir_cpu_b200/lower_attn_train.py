@@ -474,10 +474,19 @@ class AttentionDenseStatement(Statement):
         return self._bytes
 
 
+def grad_scratch_bytes(q_len: int, heads: int, kv_len: int, kv_heads: int) -> int:
+    """``ktb_attention_bwd_scratch_bytes``: a counter, three floats per query (in tiles of 64) and head, two per block of queries
+    and head and one per block of keys and key head, where a block is 256 rows of a head or as many of up to eight heads."""
+    def blocks(rows, n):
+        return -(-rows // (256 >> min(3, n.bit_length() - 1)))
+    padded = -(-q_len // 64) * 64
+    return 256 + 4 * heads * (3 * padded + 2 * blocks(padded, heads)) + 4 * kv_heads * blocks(kv_len, kv_heads)
+
+
 class AttentionGradStatement(Statement):
     """dQ, dK and dV, or some of them, of one attention: stores join as long as they are of the same tensors and mask."""
     kind = "attention_bwd"
-    launches = 3                                  # maxima cleared, what the rows bring, the gradients
+    launches = 2                                  # what the rows bring, the gradients
 
     def __init__(self, dev: R.Device, store: Store, arena: ArenaMap, stmt_id: int):
         self.dev, self.arena, self.id = dev, arena, stmt_id
@@ -598,8 +607,7 @@ class AttentionGradStatement(Statement):
         self.flops = int(10 * q.heads * hd * seen.sum())
         for ptr in self.device_arrays:
             self.dev.free(ptr)
-        # per key head three maxima, per query head and query (in tiles of 64) three floats
-        a.scratch_bytes = k.heads * 16 + 512 + 12 * q.heads * (-(-q.rows // 64) * 64)
+        a.scratch_bytes = grad_scratch_bytes(q.rows, q.heads, k.rows, k.heads)
         a.dev_scratch = self.dev.alloc(a.scratch_bytes)
         self.device_arrays = [a.dev_scratch]
         self.fps = _footprints(self.arena, walks.values(), writes, self.id)
