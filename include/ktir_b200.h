@@ -521,6 +521,9 @@ typedef struct {
     int32_t want;
     int32_t dq_row0, dq_rows, dq_head0, dq_heads;
     int32_t dk_row0, dk_rows, dk_head0, dk_heads;
+    /* parts that the walk of a tile of keys over the queries, of queries over the keys, is cut into (0, 1: none; 64 at most): for few
+       tiles with long walks.  The order of a sum depends on them. */
+    int32_t key_parts, query_parts;
     int32_t reserved;
     void* dev_scratch;
     int64_t scratch_bytes;

@@ -167,21 +167,35 @@ static __device__ void ab_drain(uint64_t* bar, uint32_t parity) {
 
 // What there is to do: the tiles of keys, then those of queries; among each, longest walks first, either head by head (so that
 // the CTAs at work share their streams in L2) or over all heads (where there are few tiles and a long one must not come last).
+// A walk may be cut into parts, where a few long ones would leave most SMs idle; the parts' sums are joined afterwards.
 struct ab_work {
-    int key_tiles, key_heads, query_tiles, query_heads;
+    int key_tiles, key_heads, key_parts, query_tiles, query_heads, query_parts;
     int by_head;
+    float *part_k, *part_v, *part_q;                        // [part][row][head][head_dim] of the rows and heads that are wanted
+    template <bool PARTS> __device__ __forceinline__ int of_keys() const { return key_tiles * key_heads * (PARTS ? key_parts : 1); }
+    template <bool PARTS> __device__ __forceinline__ int total() const { return of_keys<PARTS>() + query_tiles * query_heads * (PARTS ? query_parts : 1); }
 };
 
 struct ab_item {
     bool keys;
-    int row0, head, first, per_head, n;                     // n steps: per_head streamed tiles from `first` on, for every streamed head
+    int row0, head, part;
+    int first, per_head;                                    // a whole walk: per_head streamed tiles from `first` on, for every streamed head
+    int skip, n;                                            // this part of it: n steps after `skip`
 };
 
+template <bool PARTS>
 static __device__ __forceinline__ ab_item ab_decode(const ktb_attn_bwd_args& a, const ab_work& j, int index) {
     ab_item t;
-    const int of_keys = j.key_tiles * j.key_heads;
+    const int of_keys = j.of_keys<PARTS>();
     t.keys = index < of_keys;
-    const int at = t.keys ? index : index - of_keys, tiles = t.keys ? j.key_tiles : j.query_tiles, heads = t.keys ? j.key_heads : j.query_heads;
+    const int parts = t.keys ? j.key_parts : j.query_parts, tiles = t.keys ? j.key_tiles : j.query_tiles, heads = t.keys ? j.key_heads : j.query_heads;
+    int at = t.keys ? index : index - of_keys;
+    t.part = 0;
+    if (PARTS) {
+        const int whole = at / parts;
+        t.part = at - whole * parts;
+        at = whole;
+    }
     const int rank = j.by_head ? at % tiles : at / heads, head_here = j.by_head ? at / tiles : at % heads;
     t.first = 0;
     if (t.keys) {
@@ -193,7 +207,6 @@ static __device__ __forceinline__ ab_item ab_decode(const ktb_attn_bwd_args& a, 
             t.first = q <= 0 ? 0 : q >= a.q_len ? t.per_head : (int)(q / AB_N);
         }
         t.per_head -= t.first;
-        t.n = t.per_head * a.kv_group;
     } else {
         t.row0 = a.dq_row0 + (tiles - 1 - rank) * AB_M;
         t.head = a.dq_head0 + head_here;
@@ -204,12 +217,18 @@ static __device__ __forceinline__ ab_item ab_decode(const ktb_attn_bwd_args& a, 
             const long long n = key < 0 ? 0 : key / AB_N + 1;
             if (n < t.per_head) t.per_head = (int)n;
         }
-        t.n = t.per_head;
+    }
+    t.skip = 0;
+    t.n = t.per_head * (t.keys ? a.kv_group : 1);
+    if (PARTS) {
+        const long long steps = t.n;
+        t.skip = (int)(steps * t.part / parts);
+        t.n = (int)(steps * (t.part + 1) / parts) - t.skip;
     }
     return t;
 }
 
-template <int HD>
+template <int HD, bool PARTS>
 __global__ void __launch_bounds__(384, 1)
 ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
@@ -229,7 +248,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(const_cast<int*>(next) + 2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
-    const int grp = a.kv_group, total = work.key_tiles * work.key_heads + work.query_tiles * work.query_heads;
+    const int grp = a.kv_group, total = work.total<PARTS>();
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < Z::STAGES; ++i) {
@@ -285,10 +304,11 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 next[q] = index;
                 tc_mbar_arrive(&next_full[q]);
                 if (index >= total) break;
-                const ab_item it = ab_decode(a, work, index);
+                const ab_item it = ab_decode<PARTS>(a, work, index);
                 if (k == 0 && it.keys) ab_wait_for_rows();
                 const CUtensorMap *mx = it.keys ? &map_q : &map_k, *my = it.keys ? &map_g : &map_v;
-                int sh = it.keys ? it.head * grp : it.head / grp, s = 0;                             // streamed head and step of it
+                int sh = it.keys ? it.head * grp : it.head / grp, s = PARTS ? it.skip : 0;          // streamed head and tile of it
+                if (PARTS && it.keys && it.n > 0) sh += s / it.per_head, s %= it.per_head;
                 for (int i = 0; i < it.n; ++i, ++t) {
                     const int stage = t % Z::STAGES;
                     if (!tc_mbar_wait(&empty[stage], ((t / Z::STAGES) & 1) ^ 1, abort_flag, st, 61)) {
@@ -319,7 +339,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (int k = 0;; ++k) {
             const int index = take(k);
             if (index < 0) break;
-            const ab_item it = ab_decode(a, work, index);
+            const ab_item it = ab_decode<PARTS>(a, work, index);
             if (it.n <= 0) continue;
             if (c > 0 && !__all_sync(0xffffffffu, tc_mbar_wait(own_free, (c - 1) & 1, abort_flag, st, 69))) break;
             if (lane == 0) {
@@ -416,7 +436,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int index = next[k & 1];
             tc_mbar_arrive(&next_free[k & 1]);
             if (index >= total) break;
-            const ab_item it = ab_decode(a, work, index);
+            const ab_item it = ab_decode<PARTS>(a, work, index);
             if (it.n <= 0) continue;
             if (!(it.keys ? walk(std::true_type(), it.n) : walk(std::false_type(), it.n))) break;
             g0 += it.n;
@@ -494,9 +514,10 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const float shrink = KEYS ? ab_shrink(of_warp(known.most_g) * most_v + of_warp(known.most_d)) : ab_shrink(known.norm * most_v + fabsf(row_d));
             const uint64_t shrink2 = at_pack2(shrink, shrink);
             const uint64_t row_nl2 = at_pack2(row_nl, row_nl), row_d2 = at_pack2(-row_d, -row_d);
-            int s = it.first + (((g0 & 1) != group) ? 1 : 0);   // streamed tile of the step
             const int last = it.first + it.per_head;
-            if (KEYS && s >= last) s -= it.per_head;
+            int s = (PARTS ? it.skip : 0) + ((g0 & 1) != group ? 1 : 0);            // streamed tile of the step
+            if (KEYS && it.n > 0 && s >= it.per_head) s = PARTS ? s % it.per_head : 0;
+            s += it.first;
             for (int i = (g0 & 1) != group ? 1 : 0; i < it.n; i += 2) {
                 const int g = g0 + i;
                 const uint32_t slot = lanes + Z::SLOT + (g % Z::SLOTS) * (2 * AB_N);
@@ -632,7 +653,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             index = take(k + 1);
             ab_item then = it;
             if (index >= 0) {
-                then = ab_decode(a, work, index);
+                then = ab_decode<PARTS>(a, work, index);
                 known = ask(then);
             }
             if (it.n > 0) {
@@ -650,6 +671,12 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int64_t off = !KEYS ? a.dq_off + (int64_t)row * a.dq_row + (int64_t)it.head * a.dq_head
                               : of_v  ? a.dv_off + (int64_t)row * a.dv_row + (int64_t)it.head * a.dv_head
                                       : a.dk_off + (int64_t)row * a.dk_row + (int64_t)it.head * a.dk_head;
+            float* sum = nullptr;                               // a part's sums stay f32
+            if (PARTS && (KEYS ? work.key_parts : work.query_parts) > 1) {
+                const int row_here = row - (KEYS ? a.dk_row0 : a.dq_row0), head_here = it.head - (KEYS ? a.dk_head0 : a.dq_head0);
+                sum = (!KEYS ? work.part_q : of_v ? work.part_v : work.part_k) +
+                      (((int64_t)it.part * (KEYS ? a.dk_rows : a.dq_rows) + row_here) * (KEYS ? a.dk_heads : a.dq_heads) + head_here) * HD + (KEYS ? 0 : group * (HD / 2));
+            }
             const float factor = of_v ? back : a.scale * (back / shrink);
             constexpr int COLS = KEYS ? HD : HD / 2;
             const int col0 = KEYS ? 0 : group * (HD / 2);
@@ -670,7 +697,12 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = 0;
                 }
-                if (store && want) {
+                if (PARTS && store && want && sum) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 4)
+                        *reinterpret_cast<float4*>(sum + x + j) = make_float4(__uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor,
+                                                                             __uint_as_float(v[j + 2]) * factor, __uint_as_float(v[j + 3]) * factor);
+                } else if (store && want) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 8) {
                         uint4 o;
@@ -685,10 +717,10 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             return true;
         };
         int index = take(0);
-        if (index >= 0) known = ask(ab_decode(a, work, index));
+        if (index >= 0) known = ask(ab_decode<PARTS>(a, work, index));
         bool keys_before = true;                                // the item before has not moved this one's X and Y
         for (int k = 0; index >= 0; ++k) {
-            const ab_item it = ab_decode(a, work, index);
+            const ab_item it = ab_decode<PARTS>(a, work, index);
             if (!it.keys && keys_before && it.n > 0 && !own(c)) break;
             keys_before = it.keys;
             if (it.n > 0) of_keys_before = it.keys;
@@ -700,6 +732,32 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     }
     __syncthreads();
     if (warp == 1) tc_tmem_dealloc(tmem, 512);
+}
+
+// Joins the parts of cut walks: sums in the order of the parts, rounded once.  Eight columns of a row to a thread.
+struct ab_joined {
+    const float* part;
+    int64_t off, row, head;        // where the result goes
+    int rows, heads, row0, head0, parts;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(256) ktb_attention_join_kernel(__half* arena, const ab_joined q, const ab_joined k, const ab_joined v) {
+    const ab_joined t = blockIdx.y == 0 ? q : blockIdx.y == 1 ? k : v;
+    const int64_t all = (int64_t)t.rows * t.heads * (HD / 8), at = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (t.parts < 2 || at >= all) return;
+    float s[8] = {};
+    for (int p = 0; p < t.parts; ++p) {
+        const float4* from = reinterpret_cast<const float4*>(t.part + (p * all + at) * 8);
+        const float4 x = from[0], y = from[1];
+        s[0] += x.x, s[1] += x.y, s[2] += x.z, s[3] += x.w, s[4] += y.x, s[5] += y.y, s[6] += y.z, s[7] += y.w;
+    }
+    uint4 o;
+    __half2* h = reinterpret_cast<__half2*>(&o);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(s[2 * i], s[2 * i + 1]);
+    const int64_t r = at / (HD / 8);
+    *reinterpret_cast<uint4*>(arena + t.off + (t.row0 + r / t.heads) * t.row + (t.head0 + r % t.heads) * t.head + (at % (HD / 8)) * 8) = o;
 }
 
 // Tensor [rows][heads][HD] in boxes of 64 rows x 64 columns of one head.
@@ -716,12 +774,24 @@ static int64_t ab_padded(const ktb_attn_bwd_args& a) { return ((int64_t)a.q_len 
 static int ab_heads_log(int heads) { return heads >= 8 ? 3 : heads >= 4 ? 2 : heads >= 2 ? 1 : 0; }
 static int64_t ab_row_blocks(int64_t rows, int heads) { return (rows + (256 >> ab_heads_log(heads)) - 1) / (256 >> ab_heads_log(heads)); }
 
-// Counter; per query and head three floats; per block of queries and head two, per block of keys and key head one.
+static int64_t ab_up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+// A counter; per query and head three floats; per block of queries and head two, per block of keys and key head one ...
+static int64_t ab_rows_bytes(const ktb_attn_bwd_args& a) {
+    const int kv_heads = a.heads / a.kv_group;
+    return ab_up(256 + 4 * (int64_t)a.heads * (3 * ab_padded(a) + 2 * ab_row_blocks(ab_padded(a), a.heads)) + 4 * kv_heads * ab_row_blocks(a.kv_len, kv_heads));
+}
+// ... and, of walks that are cut, the parts' sums.
+static int64_t ab_part_bytes(const ktb_attn_bwd_args& a, bool keys) {
+    const int parts = keys ? a.key_parts : a.query_parts;
+    return parts < 2 ? 0 : ab_up(4 * (int64_t)parts * a.head_dim * (keys ? (int64_t)a.dk_rows * a.dk_heads : (int64_t)a.dq_rows * a.dq_heads));
+}
+
 extern "C" int64_t ktb_attention_bwd_scratch_bytes(const ktb_attn_bwd_args* args) {
     if (!args || args->kv_group < 1 || args->heads < args->kv_group || args->q_len < 1 || args->kv_len < 1) return 0;
-    const int kv_heads = args->heads / args->kv_group;
-    return 256 + 4 * (int64_t)args->heads * (3 * ab_padded(*args) + 2 * ab_row_blocks(ab_padded(*args), args->heads)) +
-           4 * kv_heads * ab_row_blocks(args->kv_len, kv_heads);
+    int64_t n = ab_rows_bytes(*args);
+    if (args->want & KTB_ATTN_DQ) n += ab_part_bytes(*args, false);
+    if (args->want & (KTB_ATTN_DK | KTB_ATTN_DV)) n += 2 * ab_part_bytes(*args, true);
+    return n;
 }
 
 template <int HD>
@@ -749,7 +819,8 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     KTB_CHECK_LAUNCH(ctx, "ktb_attention_rows_kernel");
     static bool attr_set[KTB_MAX_DEVICES] = {};     // the attribute is per device
     if (!attr_set[ctx->device & (KTB_MAX_DEVICES - 1)]) {
-        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
+        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
+        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
         attr_set[ctx->device & (KTB_MAX_DEVICES - 1)] = true;
     }
     ab_work work;
@@ -759,7 +830,14 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     work.key_heads = keys ? a.dk_heads : 0;
     work.query_tiles = queries ? (a.dq_rows + AB_M - 1) / AB_M : 0;
     work.query_heads = queries ? a.dq_heads : 0;
-    const long long items = (long long)work.key_tiles * work.key_heads + (long long)work.query_tiles * work.query_heads;
+    work.key_parts = a.key_parts > 1 ? a.key_parts : 1;
+    work.query_parts = a.query_parts > 1 ? a.query_parts : 1;
+    const long long items = (long long)work.key_tiles * work.key_heads * work.key_parts + (long long)work.query_tiles * work.query_heads * work.query_parts;
+    uint8_t* parts = reinterpret_cast<uint8_t*>(a.dev_scratch) + ab_rows_bytes(a);
+    work.part_q = reinterpret_cast<float*>(parts);
+    parts += (a.want & KTB_ATTN_DQ) ? ab_part_bytes(a, false) : 0;
+    work.part_k = reinterpret_cast<float*>(parts);
+    work.part_v = reinterpret_cast<float*>(parts + ab_part_bytes(a, true));
     if (items == 0) return KTB_OK;
     if (items > 0x3fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many tiles");
     work.by_head = items >= 16ll * ctx->sm_count;
@@ -775,7 +853,22 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     config.stream = ctx->stream;
     config.attrs = &early;
     config.numAttrs = 1;
-    KTB_CUDA(ctx, cudaLaunchKernelEx(&config, ktb_attention_bwd_kernel<HD>, mq, mk, mv, mg, a, w, work, ctx->dev_status));
+    // (not cutting is a kernel of its own: finding a part cost the others up to 9 %)
+    auto kernel = work.key_parts > 1 || work.query_parts > 1 ? ktb_attention_bwd_kernel<HD, true> : ktb_attention_bwd_kernel<HD, false>;
+    KTB_CUDA(ctx, cudaLaunchKernelEx(&config, kernel, mq, mk, mv, mg, a, w, work, ctx->dev_status));
+    const bool join_q = queries && work.query_parts > 1, join_k = keys && work.key_parts > 1;
+    if (join_q || join_k) {
+        KTB_CHECK_LAUNCH(ctx, "ktb_attention_bwd_kernel");
+        ab_joined q = {work.part_q, a.dq_off, a.dq_row, a.dq_head, a.dq_rows, a.dq_heads, a.dq_row0, a.dq_head0, join_q ? work.query_parts : 0};
+        ab_joined k = {work.part_k, a.dk_off, a.dk_row, a.dk_head, a.dk_rows, a.dk_heads, a.dk_row0, a.dk_head0, join_k && (a.want & KTB_ATTN_DK) ? work.key_parts : 0};
+        ab_joined v = {work.part_v, a.dv_off, a.dv_row, a.dv_head, a.dk_rows, a.dk_heads, a.dk_row0, a.dk_head0, join_k && (a.want & KTB_ATTN_DV) ? work.key_parts : 0};
+        const int64_t nq = join_q ? (int64_t)a.dq_rows * a.dq_heads : 0, nk = join_k ? (int64_t)a.dk_rows * a.dk_heads : 0;
+        const int64_t blocks = ((nq > nk ? nq : nk) * (HD / 8) + 255) / 256;
+        if (blocks > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many rows in parts");
+        ktb_attention_join_kernel<HD><<<dim3((unsigned)blocks, 3), 256, 0, ctx->stream>>>(reinterpret_cast<__half*>(a.arena), q, k, v);
+        KTB_CHECK_LAUNCH(ctx, "ktb_attention_join_kernel");
+        return KTB_OK;
+    }
     KTB_CHECK_LAUNCH(ctx, "ktb_attention_bwd_kernel");
     return KTB_OK;
 }
@@ -787,6 +880,7 @@ extern "C" int ktb_launch_attention_bwd(ktb_ctx* ctx, const ktb_attn_bwd_args* a
     if (a.head_dim != 64 && a.head_dim != 128) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "head_dim must be 64 or 128");
     if (a.q_len < 0 || a.kv_len < 0 || a.heads < 0 || a.kv_group < 1 || a.heads % a.kv_group)
         return ktb_fail(ctx, KTB_E_ARG, me, "lengths, heads or kv_group");
+    if (a.key_parts < 0 || a.key_parts > 64 || a.query_parts < 0 || a.query_parts > 64) return ktb_fail(ctx, KTB_E_ARG, me, "parts of a walk");
     if ((a.want & ~7) || a.want == 0) return ktb_fail(ctx, KTB_E_ARG, me, "which gradients are wanted");
     if (a.q_len == 0 || a.kv_len == 0 || a.heads == 0) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "no queries, keys or heads");
     if (a.q_len > (1 << 30) || a.kv_len > (1 << 30) || a.heads > 65535 * 32) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "lengths or heads");

@@ -474,13 +474,44 @@ class AttentionDenseStatement(Statement):
         return self._bytes
 
 
-def grad_scratch_bytes(q_len: int, heads: int, kv_len: int, kv_heads: int) -> int:
+SMS, TILE, STEP = 148, 128, 64           # rows that a CTA owns, rows that it streams at a time
+
+
+def grad_parts(q_len: int, kv_len: int, heads: int, kv_heads: int, causal: int, delta: int) -> Tuple[int, int]:
+    """Parts that the walks of the key tiles and of the query tiles are cut into.
+
+    CTAs take tiles as they come free, longest first, so that a walk matters only where it is not well below an SM's share of
+    all steps: one key head of eight over 1000 positions is 8 walks of 128 steps of 0.8 us, and 64 of 16 for the queries (64
+    wide 92 us whole, 31 in eight parts; over 8192 positions, 128 wide 846 whole, 459 in two, 395 in four).  Such walks are cut to
+    three quarters of the share, or to nine steps where that is more (a part costs two microseconds to start and end, joining three)."""
+    def steps(rows, first, last, copies):
+        """Of every tile: streamed tiles from that of position ``first`` to that of ``last`` (arrays over the tiles)."""
+        return np.maximum(last // STEP + 1 - first // STEP, 0) * copies
+    k0, q0 = np.arange(0, kv_len, TILE, dtype=np.int64), np.arange(0, q_len, TILE, dtype=np.int64)
+    k_first = np.clip(k0 - delta, 0, None) if causal else np.zeros_like(k0)
+    of_keys = np.where(k_first < q_len, steps(kv_len, k_first, q_len - 1, heads // kv_heads), 0)
+    q_last = np.minimum(np.minimum(q0 + TILE, q_len) - 1 + delta, kv_len - 1) if causal else np.full_like(q0, kv_len - 1)
+    of_queries = np.where(q_last >= 0, steps(q_len, 0, np.maximum(q_last, 0), 1), 0)
+    most = max(0.75 * (int(of_keys.sum()) * kv_heads * 1.3 + int(of_queries.sum()) * heads) / SMS, 9)
+    return tuple(min(16, max(1, round(int(n.max()) / most))) for n in (of_keys, of_queries))
+
+
+def grad_scratch_bytes(a: "R.AttnBwdArgs") -> int:
     """``ktb_attention_bwd_scratch_bytes``: a counter, three floats per query (in tiles of 64) and head, two per block of queries
-    and head and one per block of keys and key head, where a block is 256 rows of a head or as many of up to eight heads."""
+    and head and one per block of keys and key head, where a block is 256 rows of a head or as many of up to eight heads; and the
+    f32 sums of the parts of cut walks."""
+    def up(n):
+        return -(-n // 256) * 256
+
     def blocks(rows, n):
         return -(-rows // (256 >> min(3, n.bit_length() - 1)))
-    padded = -(-q_len // 64) * 64
-    return 256 + 4 * heads * (3 * padded + 2 * blocks(padded, heads)) + 4 * kv_heads * blocks(kv_len, kv_heads)
+    padded, kv_heads = -(-a.q_len // 64) * 64, a.heads // a.kv_group
+    total = up(256 + 4 * a.heads * (3 * padded + 2 * blocks(padded, a.heads)) + 4 * kv_heads * blocks(a.kv_len, kv_heads))
+    if a.want & R.ATTN_DQ and a.query_parts > 1:
+        total += up(4 * a.query_parts * a.head_dim * a.dq_rows * a.dq_heads)
+    if a.want & (R.ATTN_DK | R.ATTN_DV) and a.key_parts > 1:
+        total += 2 * up(4 * a.key_parts * a.head_dim * a.dk_rows * a.dk_heads)
+    return total
 
 
 class AttentionGradStatement(Statement):
@@ -607,10 +638,21 @@ class AttentionGradStatement(Statement):
         self.flops = int(10 * q.heads * hd * seen.sum())
         for ptr in self.device_arrays:
             self.dev.free(ptr)
-        a.scratch_bytes = grad_scratch_bytes(q.rows, q.heads, k.rows, k.heads)
-        a.dev_scratch = self.dev.alloc(a.scratch_bytes)
-        self.device_arrays = [a.dev_scratch]
+        self.device_arrays = []
+        self._cut(self.dev, *grad_parts(a.q_len, a.kv_len, a.heads, k.heads, a.causal, a.causal_delta))
         self.fps = _footprints(self.arena, walks.values(), writes, self.id)
+
+    def _cut(self, dev, key_parts: int, query_parts: int):
+        """The parts of the walks, and scratch for them.  (They follow from the whole tensors: a rank that has some of the cores
+        sums in the same parts.)"""
+        a = self.args
+        for ptr in self.device_arrays:
+            dev.free(ptr)
+        a.key_parts, a.query_parts = key_parts, query_parts
+        a.scratch_bytes = grad_scratch_bytes(a)
+        a.dev_scratch = dev.alloc(a.scratch_bytes)
+        self.device_arrays = [a.dev_scratch]
+        self.launches = 3 if max(key_parts, query_parts) > 1 else 2
 
     def launch(self, dev, arena_ptr):
         self.args.arena = arena_ptr

@@ -148,7 +148,7 @@ class AttnBwdArgs(C.Structure):
         [(n, C.c_int64) for n in ("q_off k_off v_off o_off do_off lse_off dq_off dk_off dv_off q_row q_head k_row k_head v_row v_head "
                                   "o_row o_head do_row do_head lse_row lse_head dq_row dq_head dk_row dk_head dv_row dv_head").split()] + \
         [(n, C.c_int32) for n in "q_len kv_len heads kv_group head_dim causal causal_delta".split()] + [("scale", C.c_float)] + \
-        [(n, C.c_int32) for n in "want dq_row0 dq_rows dq_head0 dq_heads dk_row0 dk_rows dk_head0 dk_heads reserved".split()] + \
+        [(n, C.c_int32) for n in "want dq_row0 dq_rows dq_head0 dq_heads dk_row0 dk_rows dk_head0 dk_heads key_parts query_parts reserved".split()] + \
         [("dev_scratch", C.c_void_p), ("scratch_bytes", C.c_int64)]
 
 

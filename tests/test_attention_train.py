@@ -14,6 +14,7 @@ import pytest
 
 from ktir_cpu_b200 import HardwareConfig, KTIRInterpreter, kernels as K, runtime as R
 from ktir_cpu_b200.interpreter import Session
+from ktir_cpu_b200.lower_attn_train import grad_parts, grad_scratch_bytes
 from ktir_cpu_b200.parser import KTIRParser
 from oracle.numpy_interp import OracleInterpreter
 
@@ -253,13 +254,34 @@ def test_ranks_take_their_heads(world):
     assert covered == [(r * per * 2, per * 2, r * per, per, 7) for r in range(world)]
 
 
+@pytest.mark.parametrize("q_len,kv_len,heads,kv_heads,causal,parts", [
+    (2048, 2048, 256, 256, True, (1, 1)), (197, 197, 12, 12, False, (1, 1)), (8192, 8192, 16, 4, True, (1, 1)),   # enough tiles
+    (1000, 1000, 8, 1, False, (13, 2)), (1, 8192, 32, 8, True, (1, 5)), (4096, 4096, 1, 1, False, (3, 3)), (1, 1, 1, 1, True, (1, 1)),
+    (100, 20, 2, 2, True, (1, 1)), (4096, 64, 8, 1, False, (16, 1))])
+def test_long_walks_are_cut_where_there_are_few(q_len, kv_len, heads, kv_heads, causal, parts):
+    assert grad_parts(q_len, kv_len, heads, kv_heads, int(causal), kv_len - q_len if causal else 0) == parts
+
+
+@pytest.mark.parametrize("parts", [(1, 1), (3, 1), (1, 5), (8, 8), (0, 0)])
+@pytest.mark.parametrize("want", [7, 1, 2, 6])
+def test_scratch_is_what_the_library_asks_for(parts, want, build_lib):
+    a = R.AttnBwdArgs()
+    for heads, group, q_len, kv_len, hd in ((1, 1, 1, 1, 64), (14, 2, 333, 1, 128), (256, 1, 2048, 2048, 128), (40, 8, 65, 8191, 64)):
+        a.q_len, a.kv_len, a.heads, a.kv_group, a.head_dim, a.want = q_len, kv_len, heads, group, hd, want
+        a.dq_rows, a.dq_heads, a.dk_rows, a.dk_heads = q_len, heads, kv_len, heads // group
+        a.key_parts, a.query_parts = parts
+        assert grad_scratch_bytes(a) == R.lib().ktb_attention_bwd_scratch_bytes(C.byref(a))
+
+
 # ---- kernels -------------------------------------------------------------------------------------------------------
 # (queries, keys, heads, key heads, head size, causal): one token; keys and queries around tiles of 64 and 128; odd lengths;
 # groups; more queries than keys by more and by less than a tile; a context before a few queries; no mask
 CASES = [(1, 1, 1, 1, 128, True), (1, 1, 2, 1, 64, False), (1, 300, 6, 2, 128, True), (64, 64, 2, 2, 64, True), (65, 65, 2, 2, 128, True),
          (127, 129, 3, 3, 64, True), (128, 128, 4, 1, 128, True), (129, 127, 4, 2, 128, True), (197, 197, 5, 5, 64, False), (300, 111, 3, 1, 64, True),
          (513, 100, 2, 2, 128, True), (70, 500, 14, 2, 128, False), (257, 771, 3, 3, 128, True), (640, 640, 2, 1, 64, True), (191, 64, 2, 2, 64, False),
-         (1000, 3, 2, 2, 128, False), (3, 1000, 10, 2, 64, True), (385, 449, 7, 1, 128, True)]
+         (1000, 3, 2, 2, 128, False), (3, 1000, 10, 2, 64, True), (385, 449, 7, 1, 128, True),
+         # few tiles with long walks: in parts
+         (1000, 1000, 8, 1, 64, True), (1, 3000, 4, 2, 128, True), (130, 4000, 2, 2, 64, False), (2000, 70, 5, 1, 128, False)]
 
 
 def _run(src, fn, full, kind, times=1):
@@ -419,12 +441,12 @@ def test_a_training_step_of_an_attention_layer(build_lib):
 
 
 @pytest.mark.gpu
-def test_shards_add_up_to_the_whole(build_lib):
-    c = (100, 200, 8, 4, 64, True)
+@pytest.mark.parametrize("c", [(100, 200, 8, 4, 64, True), (400, 300, 8, 2, 128, False)])         # (the second one in parts)
+def test_shards_add_up_to_the_whole(c, build_lib):
     kw, do = _inputs(*c[:5])
-    o, lse = _forward_results(kw, True)
-    for fn, make, full, kind in ((FWD, K.attention_forward, _kwargs(FWD, kw, 100, 8, 64), "attention_dense"),
-                                 (BWD, K.attention_backward, _kwargs(BWD, kw, 100, 8, 64, do, o, lse), "attention_bwd")):
+    o, lse = _forward_results(kw, c[5])
+    for fn, make, full, kind in ((FWD, K.attention_forward, _kwargs(FWD, kw, c[0], 8, c[4]), "attention_dense"),
+                                 (BWD, K.attention_backward, _kwargs(BWD, kw, c[0], 8, c[4], do, o, lse), "attention_bwd")):
         src = make(*c, 16, 64)
         whole = _run(src, fn, full, kind)
         gpu = KTIRInterpreter()
@@ -535,9 +557,10 @@ def test_launchers_refuse(build_lib):
                                ("q_len", 0, -3), ("kv_len", 0, -3), ("want", 0, -2), ("want", 8, -2), ("scale", float("nan"), -2), ("scale", float("inf"), -2),
                                ("dq_row0", -1, -2), ("dq_rows", 65, -2), ("dq_heads", 5, -2), ("dq_head0", 1, -2), ("dk_rows", 65, -2), ("dk_head0", 1, -2),
                                ("dk_row0", 64, -2), ("k_row", 12, -3), ("q_off", st.args.q_off + 4, -3), ("dv_head", 2, -3), ("dev_scratch", None, -2),
-                               ("dev_scratch", st.args.dev_scratch + 16, -2), ("scratch_bytes", st.args.scratch_bytes - 1, -2)):
+                               ("dev_scratch", st.args.dev_scratch + 16, -2), ("scratch_bytes", st.args.scratch_bytes - 1, -2),
+                               ("key_parts", -1, -2), ("query_parts", 65, -2), ("key_parts", 2, -2), ("query_parts", 2, -2)):
         refused("ktb_launch_attention_bwd", st.args, field, value, code, "attention_bwd")
-    assert dev.lib.ktb_attention_bwd_scratch_bytes(C.byref(st.args)) <= st.args.scratch_bytes
+    assert dev.lib.ktb_attention_bwd_scratch_bytes(C.byref(st.args)) == st.args.scratch_bytes
     fwd = KTIRInterpreter()
     fwd.load(K.attention_forward(64, 64, 4, 2, 64, True))
     fs, _ = fwd.session(FWD, **_kwargs(FWD, kw, 64, 4, 64))
