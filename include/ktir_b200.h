@@ -558,6 +558,7 @@ typedef struct {
     int64_t table_stride, cos_off, sin_off;   /* f32 elements: from row to row, first rows */
     int64_t cos_end, sin_end;
     int32_t align, reserved;                  /* a power of two that divides the tensors' offsets in the item table */
+    int64_t first[1 + 2 * KTB_ROTARY_TENSORS];/* a single item's entries; the table is not read then */
     ktb_rotary_tensor t[KTB_ROTARY_TENSORS];
 } ktb_rotary_args;
 int ktb_launch_rotary(ktb_ctx* ctx, const ktb_rotary_args* args);

@@ -248,6 +248,8 @@ class RotaryStatement(Statement):
                 if f is not w and _runs_overlap(w.starts, w.ends, f.starts, f.ends):
                     raise Unsupported("a rotary launch that reads what it writes")
         self.table = table
+        for n, v in enumerate(table[0]):
+            a.first[n] = int(v)
         a.dev_item_offsets = self.dev_table = dev.upload(table)
         self.device_arrays = [self.dev_table]
 

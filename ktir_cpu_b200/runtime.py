@@ -166,7 +166,8 @@ class RotaryArgs(C.Structure):
                 ("tokens", C.c_int32), ("pairs", C.c_int32), ("dtype", C.c_int32), ("idx_dtype", C.c_int32),
                 ("n_tensors", C.c_int32), ("inverse", C.c_int32), ("pos_stride", C.c_int64), ("pair_stride", C.c_int64),
                 ("table_stride", C.c_int64), ("cos_off", C.c_int64), ("sin_off", C.c_int64), ("cos_end", C.c_int64),
-                ("sin_end", C.c_int64), ("align", C.c_int32), ("reserved", C.c_int32), ("t", RotaryTensor * ROTARY_TENSORS)]
+                ("sin_end", C.c_int64), ("align", C.c_int32), ("reserved", C.c_int32),
+                ("first", C.c_int64 * (1 + 2 * ROTARY_TENSORS)), ("t", RotaryTensor * ROTARY_TENSORS)]
 
 
 G_MAXDIM = 6

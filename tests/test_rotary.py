@@ -143,8 +143,8 @@ def test_every_vector_length(build_lib):
     """Lengths whose halves start at 2, 4, 8 and 16 bytes, rests likewise."""
     for dtype in ("f16", "f32"):
         for layout in ("half", "interleaved"):
-            for dim, part in ((64, 32), (64, 24), (64, 20), (62, 22), (61, 18)):
-                case = (9, 3, 2, dim, part, layout, False, dtype, 3)
+            for dim, part in ((64, 32), (64, 24), (64, 20), (62, 22), (61, 18), (64, 62), (72, 50), (16, 14), (16, 6), (8, 6)):
+                case = (9, 13, 2, dim, part, layout, False, dtype, 3)
                 src, kw = _case(*case)
                 gpu = KTIRInterpreter()
                 gpu.load(src)
