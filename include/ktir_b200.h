@@ -495,6 +495,13 @@ typedef struct {
     int32_t q_len, kv_len, heads, kv_group, head_dim;
     int32_t causal, causal_delta;
     float scale;
+    /* few queries and heads: parts that the keys are cut into (0, 1: none; 64 at most), with dev_scratch (16-byte boundary) of
+       4 * parts * q_len * heads * (head_dim + 1) bytes to join them in.  The order of a sum depends on them; launches that share
+       scratch must be ordered. */
+    int32_t parts;
+    int32_t twice;              /* 1: P is multiplied as f16 and once more as what that left out (half the rate; for few rows) */
+    void* dev_scratch;
+    int64_t scratch_bytes;
 } ktb_attn_dense_args;
 int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_args* args);
 
@@ -524,7 +531,9 @@ typedef struct {
     /* parts that the walk of a tile of keys over the queries, of queries over the keys, is cut into (0, 1: none; 64 at most): for few
        tiles with long walks.  The order of a sum depends on them. */
     int32_t key_parts, query_parts;
-    int32_t reserved;
+    /* 1: P and dS are multiplied as f16 and once more as what that left out (half the rate; for few rows, where roundings do not
+       average out). */
+    int32_t twice;
     void* dev_scratch;
     int64_t scratch_bytes;
 } ktb_attn_bwd_args;

@@ -149,7 +149,7 @@ struct ab_shape {
     static constexpr int OWN = AB_M * HD * 2;               // bytes of X, of Y
     static constexpr int STEP = AB_N * HD * 2;              // bytes of X', of Y'
     static constexpr int STAGES = HD == 64 ? 8 : 4;         // 128 KB of the stream on its way
-    static constexpr size_t SMEM = 2 * OWN + STAGES * (2 * STEP + 2 * AB_N * 4) + 1024 + 512;
+    static constexpr size_t SMEM = 2 * OWN + STAGES * (2 * STEP + 3 * AB_N * 4) + 1024 + 512;
     // columns of TMEM: two accumulators (for queries X and Y as f16 pairs in place of the second), then the slots: S and T
     static constexpr int ACC1 = HD, X = HD, Y = HD + HD / 2, SLOT = 2 * HD;
     static constexpr int SLOTS = (512 - SLOT) / (2 * AB_N);
@@ -171,6 +171,7 @@ static __device__ void ab_drain(uint64_t* bar, uint32_t parity) {
 struct ab_work {
     int key_tiles, key_heads, key_parts, query_tiles, query_heads, query_parts;
     int by_head;
+    int twice;                                              // every step comes twice (only where PARTS)
     float *part_k, *part_v, *part_q;                        // [part][row][head][head_dim] of the rows and heads that are wanted
     template <bool PARTS> __device__ __forceinline__ int of_keys() const { return key_tiles * key_heads * (PARTS ? key_parts : 1); }
     template <bool PARTS> __device__ __forceinline__ int total() const { return of_keys<PARTS>() + query_tiles * query_heads * (PARTS ? query_parts : 1); }
@@ -223,24 +224,37 @@ static __device__ __forceinline__ ab_item ab_decode(const ktb_attn_bwd_args& a, 
     if (PARTS) {
         const long long steps = t.n;
         t.skip = (int)(steps * t.part / parts);
-        t.n = (int)(steps * (t.part + 1) / parts) - t.skip;
+        t.n = ((int)(steps * (t.part + 1) / parts) - t.skip) << j.twice;
     }
     return t;
 }
 
-template <int HD, bool PARTS>
+// Two values as f16, or what that rounding leaves out of them (nothing of an infinity).
+template <bool RESTS>
+static __device__ __forceinline__ __half2 ab_pack(float x, float y, bool rest) {
+    __half2 h = __floats2half2_rn(x, y);
+    if (RESTS && rest) {
+        const float u = __low2float(h), v = __high2float(h);
+        h = __floats2half2_rn(fabsf(u) <= 65504.f ? x - u : 0.f, fabsf(v) <= 65504.f ? y - v : 0.f);
+    }
+    return h;
+}
+
+// MODE: 0 whole walks, 1 parts of walks, 2 parts of walks whose steps come twice: P and dS as f16, then what that left out of them.
+template <int HD, int MODE>
 __global__ void __launch_bounds__(384, 1)
 ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_g,
                          const ktb_attn_bwd_args a, const ab_scratch w, const ab_work work, ktb_status* st) {
     typedef ab_shape<HD> Z;
+    constexpr bool PARTS = MODE > 0, TWICE = MODE == 2;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sX = smem;
     uint8_t* sY = sX + Z::OWN;
     uint8_t* ring = sY + Z::OWN;                            // per stage X', then Y'
-    float* sRow = reinterpret_cast<float*>(ring + Z::STAGES * 2 * Z::STEP);     // keys: per stage 64 x (14 - lse / ln 2), 64 x D
-    uint64_t* full = reinterpret_cast<uint64_t*>(sRow + Z::STAGES * 2 * AB_N);
+    float* sRow = reinterpret_cast<float*>(ring + Z::STAGES * 2 * Z::STEP);     // keys: per stage 64 x (14 - lse / ln 2), 64 x D, 64 x |dO| where steps come twice
+    uint64_t* full = reinterpret_cast<uint64_t*>(sRow + Z::STAGES * 3 * AB_N);
     uint64_t *empty = full + Z::STAGES, *own_full = empty + Z::STAGES, *own_free = own_full + 1, *a_ready = own_free + 1;
     uint64_t *acc_free = a_ready + 1, *done = acc_free + 1, *next_full = done + 1, *next_free = next_full + 2;
     uint64_t *s_full = next_free + 2, *t_full = s_full + Z::SLOTS, *p_full = t_full + Z::SLOTS;     // p_full: per slot and half of its columns
@@ -317,17 +331,19 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     }
                     const int r = (it.first + s) * AB_N;
                     uint8_t* to = ring + stage * 2 * Z::STEP;
-                    tc_mbar_expect_tx(&full[stage], 2 * Z::STEP + (it.keys ? 2 * AB_N * 4 : 0));
+                    tc_mbar_expect_tx(&full[stage], 2 * Z::STEP + (it.keys ? (TWICE ? 3 : 2) * AB_N * 4 : 0));
 #pragma unroll
                     for (int b = 0; b < Z::BLOCKS; ++b) {
                         tc_tma_load_3d(to + b * (AB_N * 128), mx, &full[stage], b * 64, sh, r);
                         tc_tma_load_3d(to + Z::STEP + b * (AB_N * 128), my, &full[stage], b * 64, sh, r);
                     }
                     if (it.keys) {
-                        float* rows = sRow + stage * 2 * AB_N;
+                        float* rows = sRow + stage * 3 * AB_N;
                         tc_bulk_load(rows, w.neg_lse + (int64_t)sh * w.padded + r, &full[stage], AB_N * 4);
                         tc_bulk_load(rows + AB_N, w.d + (int64_t)sh * w.padded + r, &full[stage], AB_N * 4);
+                        if (TWICE) tc_bulk_load(rows + 2 * AB_N, w.norm + (int64_t)sh * w.padded + r, &full[stage], AB_N * 4);
                     }
+                    if (TWICE && !(i & 1)) continue;
                     if (++s == it.per_head) s = 0, ++sh;
                 }
             }
@@ -504,6 +520,21 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
             return x;
         };
+        // Columns [32 h, 32 h + 32) of T: a difference of T and D within the rounding of their sums, 2^-22 of |dO| |V|, is none: a
+        // query that sees one key has no gradient.  (Where there are more keys than a step's, others' gradients are far above that.)
+        auto settle = [&](auto of_keys, uint32_t (&t)[32], const float4* rows, int h, float d, float near) {
+            constexpr bool KEYS = decltype(of_keys)::value;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+                float dj = d, most = near;
+                if (KEYS) {
+                    const float* of_row = reinterpret_cast<const float*>(rows) + 32 * h + j;
+                    dj = of_row[AB_N];
+                    most = near * of_row[2 * AB_N];
+                }
+                if (fabsf(__uint_as_float(t[j]) - dj) <= most) t[j] = __float_as_uint(dj);
+            }
+        };
         ab_known known = {};
         // One item: its steps, then its results.  `index` becomes the next item's.
         auto walk = [&](auto of_keys, const ab_item& it, int k, int& index) -> bool {
@@ -512,17 +543,20 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const float most_v = of_warp(known.most_v);
             const float row_nl = known.nl, row_d = known.d;
             const float shrink = KEYS ? ab_shrink(of_warp(known.most_g) * most_v + of_warp(known.most_d)) : ab_shrink(known.norm * most_v + fabsf(row_d));
+            const float near = (KEYS ? most_v : known.norm * most_v) * 0x1p-22f;
             const uint64_t shrink2 = at_pack2(shrink, shrink);
             const uint64_t row_nl2 = at_pack2(row_nl, row_nl), row_d2 = at_pack2(-row_d, -row_d);
             const int last = it.first + it.per_head;
-            int s = (PARTS ? it.skip : 0) + ((g0 & 1) != group ? 1 : 0);            // streamed tile of the step
+            const int pace = TWICE ? 1 : 2;                           // streamed tiles from one of my steps to the next
+            int s = (PARTS ? it.skip : 0) + ((g0 & 1) != group && pace == 2 ? 1 : 0);        // streamed tile of the step
             if (KEYS && it.n > 0 && s >= it.per_head) s = PARTS ? s % it.per_head : 0;
             s += it.first;
             for (int i = (g0 & 1) != group ? 1 : 0; i < it.n; i += 2) {
                 const int g = g0 + i;
                 const uint32_t slot = lanes + Z::SLOT + (g % Z::SLOTS) * (2 * AB_N);
                 const int s0 = s * AB_N;                        // first streamed row of the step
-                s += 2;
+                s += pace;
+                const bool rest = TWICE && (i & 1);
                 if (KEYS)
                     while (s >= last) s -= it.per_head;
                 // columns [lo, hi) of this row are visible
@@ -544,7 +578,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 }
                 // Half of the columns at a time.  Cut: P needs S alone, so that T may still be in the making; the sums over the first half
                 // are made while the second one is worked on.  (Row values are asked for early: shared memory is busy with operands.)
-                const float4* rows = reinterpret_cast<const float4*>(sRow + (g % Z::STAGES) * 2 * AB_N);
+                const float4* rows = reinterpret_cast<const float4*>(sRow + (g % Z::STAGES) * 3 * AB_N);
                 float4 nl[8], dd[8];
                 bool there = true;
                 if (KEYS) {
@@ -581,7 +615,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             at_unpack2(at_fma2(at_pack2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])), sl2, nl2), x0, x1);
                             p[j] = at_ex2(x0);
                             p[j + 1] = at_ex2(x1);
-                            const __half2 hp = __floats2half2_rn(p[j], p[j + 1]);
+                            const __half2 hp = ab_pack<TWICE>(p[j], p[j + 1], rest);
                             half16[j >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
                         }
                         // (over columns that this thread has read)
@@ -596,6 +630,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             for (int j = 0; j < 8; ++j) nl[j] = rows[8 + j];
                         }
                         tc_tmem_ld_wait();
+                        if (TWICE && a.kv_len <= AB_N) settle(of_keys, t, rows, h, row_d, near);
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
                             uint64_t d2 = row_d2;
@@ -603,7 +638,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             float y0, y1;
                             const uint64_t diff = at_add2(at_pack2(__uint_as_float(t[j]), __uint_as_float(t[j + 1])), d2);
                             at_unpack2(at_mul2(at_mul2(diff, shrink2), at_pack2(p[j], p[j + 1])), y0, y1);
-                            const __half2 hs = __floats2half2_rn(y0, y1);
+                            const __half2 hs = ab_pack<TWICE>(y0, y1, rest);
                             half16[j >> 1] = *reinterpret_cast<const uint32_t*>(&hs);
                         }
                         tc_tmem_st16(slot + AB_N + 16 * h, half16);
@@ -624,6 +659,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             for (int j = 0; j < 32; ++j)
                                 if (32 * h + j < lo || 32 * h + j >= hi) s[j] = 0xff800000u;
                         }
+                        if (TWICE && a.kv_len <= AB_N) settle(of_keys, t, rows, h, row_d, near);
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
                             uint64_t nl2 = row_nl2, d2 = row_d2;
@@ -637,7 +673,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             const float p0 = at_ex2(x0), p1 = at_ex2(x1);
                             const uint64_t diff = at_add2(at_pack2(__uint_as_float(t[j]), __uint_as_float(t[j + 1])), d2);
                             at_unpack2(at_mul2(at_mul2(diff, shrink2), at_pack2(p0, p1)), y0, y1);
-                            const __half2 hp = __floats2half2_rn(p0, p1), hs = __floats2half2_rn(y0, y1);
+                            const __half2 hp = ab_pack<TWICE>(p0, p1, rest), hs = ab_pack<TWICE>(y0, y1, rest);
                             p16[j >> 1] = *reinterpret_cast<const uint32_t*>(&hp);
                             s16[j >> 1] = *reinterpret_cast<const uint32_t*>(&hs);
                         }
@@ -815,23 +851,29 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     if (!ab_map(&mq, a, a.q_off, a.q_len, a.heads, a.q_row, a.q_head) || !ab_map(&mg, a, a.do_off, a.q_len, a.heads, a.do_row, a.do_head) ||
         !ab_map(&mk, a, a.k_off, a.kv_len, kv_heads, a.k_row, a.k_head) || !ab_map(&mv, a, a.v_off, a.kv_len, kv_heads, a.v_row, a.v_head))
         return ktb_fail(ctx, KTB_E_CUDA, "attention_bwd", "cuTensorMapEncodeTiled failed");
+    const bool keys = (a.want & (KTB_ATTN_DK | KTB_ATTN_DV)) && a.dk_rows > 0 && a.dk_heads > 0;
+    const bool queries = (a.want & KTB_ATTN_DQ) && a.dq_rows > 0 && a.dq_heads > 0;
+    const bool join_q = queries && a.query_parts > 1, join_k = keys && a.key_parts > 1;
+    const int64_t nq = join_q ? (int64_t)a.dq_rows * a.dq_heads : 0, nk = join_k ? (int64_t)a.dk_rows * a.dk_heads : 0;
+    const int64_t blocks = ((nq > nk ? nq : nk) * (HD / 8) + 255) / 256;
+    if (blocks > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many rows in parts");
     ktb_attention_rows_kernel<HD><<<(unsigned)row_blocks, 256, 0, ctx->stream>>>(a, w);
     KTB_CHECK_LAUNCH(ctx, "ktb_attention_rows_kernel");
     static bool attr_set[KTB_MAX_DEVICES] = {};     // the attribute is per device
     if (!attr_set[ctx->device & (KTB_MAX_DEVICES - 1)]) {
-        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
-        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
+        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD, 0>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
+        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD, 1>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
+        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_bwd_kernel<HD, 2>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)ab_shape<HD>::SMEM));
         attr_set[ctx->device & (KTB_MAX_DEVICES - 1)] = true;
     }
     ab_work work;
-    const bool keys = (a.want & (KTB_ATTN_DK | KTB_ATTN_DV)) && a.dk_rows > 0 && a.dk_heads > 0;
-    const bool queries = (a.want & KTB_ATTN_DQ) && a.dq_rows > 0 && a.dq_heads > 0;
     work.key_tiles = keys ? (a.dk_rows + AB_M - 1) / AB_M : 0;
     work.key_heads = keys ? a.dk_heads : 0;
     work.query_tiles = queries ? (a.dq_rows + AB_M - 1) / AB_M : 0;
     work.query_heads = queries ? a.dq_heads : 0;
     work.key_parts = a.key_parts > 1 ? a.key_parts : 1;
     work.query_parts = a.query_parts > 1 ? a.query_parts : 1;
+    work.twice = a.twice;
     const long long items = (long long)work.key_tiles * work.key_heads * work.key_parts + (long long)work.query_tiles * work.query_heads * work.query_parts;
     uint8_t* parts = reinterpret_cast<uint8_t*>(a.dev_scratch) + ab_rows_bytes(a);
     work.part_q = reinterpret_cast<float*>(parts);
@@ -854,17 +896,13 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     config.attrs = &early;
     config.numAttrs = 1;
     // (not cutting is a kernel of its own: finding a part cost the others up to 9 %)
-    auto kernel = work.key_parts > 1 || work.query_parts > 1 ? ktb_attention_bwd_kernel<HD, true> : ktb_attention_bwd_kernel<HD, false>;
+    auto kernel = a.twice ? ktb_attention_bwd_kernel<HD, 2> : work.key_parts > 1 || work.query_parts > 1 ? ktb_attention_bwd_kernel<HD, 1> : ktb_attention_bwd_kernel<HD, 0>;
     KTB_CUDA(ctx, cudaLaunchKernelEx(&config, kernel, mq, mk, mv, mg, a, w, work, ctx->dev_status));
-    const bool join_q = queries && work.query_parts > 1, join_k = keys && work.key_parts > 1;
     if (join_q || join_k) {
         KTB_CHECK_LAUNCH(ctx, "ktb_attention_bwd_kernel");
         ab_joined q = {work.part_q, a.dq_off, a.dq_row, a.dq_head, a.dq_rows, a.dq_heads, a.dq_row0, a.dq_head0, join_q ? work.query_parts : 0};
         ab_joined k = {work.part_k, a.dk_off, a.dk_row, a.dk_head, a.dk_rows, a.dk_heads, a.dk_row0, a.dk_head0, join_k && (a.want & KTB_ATTN_DK) ? work.key_parts : 0};
         ab_joined v = {work.part_v, a.dv_off, a.dv_row, a.dv_head, a.dk_rows, a.dk_heads, a.dk_row0, a.dk_head0, join_k && (a.want & KTB_ATTN_DV) ? work.key_parts : 0};
-        const int64_t nq = join_q ? (int64_t)a.dq_rows * a.dq_heads : 0, nk = join_k ? (int64_t)a.dk_rows * a.dk_heads : 0;
-        const int64_t blocks = ((nq > nk ? nq : nk) * (HD / 8) + 255) / 256;
-        if (blocks > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many rows in parts");
         ktb_attention_join_kernel<HD><<<dim3((unsigned)blocks, 3), 256, 0, ctx->stream>>>(reinterpret_cast<__half*>(a.arena), q, k, v);
         KTB_CHECK_LAUNCH(ctx, "ktb_attention_join_kernel");
         return KTB_OK;
@@ -880,7 +918,7 @@ extern "C" int ktb_launch_attention_bwd(ktb_ctx* ctx, const ktb_attn_bwd_args* a
     if (a.head_dim != 64 && a.head_dim != 128) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "head_dim must be 64 or 128");
     if (a.q_len < 0 || a.kv_len < 0 || a.heads < 0 || a.kv_group < 1 || a.heads % a.kv_group)
         return ktb_fail(ctx, KTB_E_ARG, me, "lengths, heads or kv_group");
-    if (a.key_parts < 0 || a.key_parts > 64 || a.query_parts < 0 || a.query_parts > 64) return ktb_fail(ctx, KTB_E_ARG, me, "parts of a walk");
+    if (a.key_parts < 0 || a.key_parts > 64 || a.query_parts < 0 || a.query_parts > 64 || a.twice < 0 || a.twice > 1) return ktb_fail(ctx, KTB_E_ARG, me, "parts of a walk");
     if ((a.want & ~7) || a.want == 0) return ktb_fail(ctx, KTB_E_ARG, me, "which gradients are wanted");
     if (a.q_len == 0 || a.kv_len == 0 || a.heads == 0) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "no queries, keys or heads");
     if (a.q_len > (1 << 30) || a.kv_len > (1 << 30) || a.heads > 65535 * 32) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "lengths or heads");

@@ -69,10 +69,10 @@ static __device__ __forceinline__ float at_chunk_max(const uint32_t (&v)[CW], fl
 // P = exp2(s * sl - m) for CW scores -> CW/2 packed f16 pairs; the f32 values are added to acc2.
 // POLY of every 4 pairs take the polynomial instead of the exp unit.  A score of -inf (a masked
 // column) gives 0 on either path (the polynomial clamps it to 2^-125, which is 0 in f16 and
-// vanishes in the sum).
+// vanishes in the sum).  `rest`: what rounding P to f16 left out, instead of P.
 template <int CW, int POLY, bool FINE>
 static __device__ __forceinline__ void at_chunk_prob(const uint32_t (&v)[CW], float sl, float m, uint64_t& acc2,
-                                                     uint32_t (&packed)[CW / 2]) {
+                                                     uint32_t (&packed)[CW / 2], bool rest = false) {
     const uint64_t sl2 = at_pack2(sl, sl), nm2 = at_pack2(-m, -m);
 #pragma unroll
     for (int i = 0; i < CW; i += 2) {
@@ -86,7 +86,8 @@ static __device__ __forceinline__ void at_chunk_prob(const uint32_t (&v)[CW], fl
             p1 = at_ex2(x1);
         }
         acc2 = at_add2(acc2, at_pack2(p0, p1));
-        const __half2 h = __floats2half2_rn(p0, p1);
+        __half2 h = __floats2half2_rn(p0, p1);
+        if (rest) h = __floats2half2_rn(p0 - __low2float(h), p1 - __high2float(h));
         packed[i >> 1] = *reinterpret_cast<const uint32_t*>(&h);
     }
 }
@@ -112,14 +113,19 @@ enum { B_QFULL = 0, B_QFREE = 2, B_KVFULL = 4, B_KVEMPTY = B_KVFULL + AT_MAX_STA
 // store the output, so a tile pair no longer pays a start-up and a drain of its own.
 //
 // DENSE: keys and values are rows of one tensor instead of pages, a.num_tiles groups of BN of them of which d.kv_len exist;
-// rows that see nothing give 0, and the log-sum-exp of every row is kept.
+// rows that see nothing give 0, and the log-sum-exp of every row is kept.  PARTS: the keys of an item are cut into d.parts
+// ranges, an item of its own each, where whole items would leave most SMs idle; ktb_attention_join_fwd_kernel joins them.  With
+// d.twice every page comes twice: P as f16 times V, then what that rounding left out (up to 2^-12 of P) times V.  A result is
+// the sum of a few large P, so that over many rows their roundings are as large as the result's own, 2^-12, but over a few rows
+// one or another is off by twice that.
 struct at_dense {
     float* lse;                 // null: not wanted
     int64_t row, head;
-    int kv_len;
+    int kv_len, parts, twice;
+    float *part_o, *part_lse;   // [part][query][head][head_dim], [part][query][head]
 };
 
-template <int BN, int TPR, int POLY, int HD, bool DENSE>
+template <int BN, int TPR, int POLY, int HD, bool DENSE, bool PARTS>
 __global__ void __launch_bounds__(128 + 256 * TPR, 1)
 ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                          const __grid_constant__ CUtensorMap map_v, const ktb_attn_args a, const at_dense d,
@@ -146,10 +152,15 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // Sub-item s of this CTA: false when the CTA has run out of items.  n_of[i] = steps (SB kv rows each)
     // tile i can see (kv position p is visible to row R iff p <= R + delta), 0 for a tile that does
     // not exist; nmax = pages to stream.  An item whose two halves coincide has an empty second half.
-    auto sub_item = [&](int s, int& head, int& q0, int (&n_of)[2], int& nmax, bool& again) -> bool {
+    auto sub_item = [&](int s, int& head, int& q0, int (&n_of)[2], int& nmax, bool& again, int& page0, int& part) -> bool {
         const long long item64 = (long long)blockIdx.x + (long long)(s >> 1) * gridDim.x;
         if (item64 >= n_items) return false;
-        const int item = (int)item64;
+        int item = (int)item64;
+        part = page0 = 0;
+        if (PARTS) {
+            part = item % d.parts;
+            item /= d.parts;
+        }
         head = item / half_pairs;
         const int r = item % half_pairs;
         const int qp = (s & 1) ? r : q_pairs - 1 - r;
@@ -166,6 +177,17 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             n_of[i] = empty ? 0 : n;
         }
         nmax = ((n_of[0] > n_of[1] ? n_of[0] : n_of[1]) + NSUB - 1) / NSUB;
+        if (PARTS) {                                   // pages page0 .. end - 1 of these; whole ones where they come twice
+            page0 = (int)((long long)nmax * part / d.parts);
+            const int pages = (int)((long long)nmax * (part + 1) / d.parts) - page0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                n_of[i] -= page0 * NSUB;
+                n_of[i] = n_of[i] < 0 ? 0 : n_of[i] > pages * NSUB ? pages * NSUB : n_of[i];
+                if (d.twice) n_of[i] = (n_of[i] + NSUB - 1) / NSUB * 2 * NSUB;
+            }
+            nmax = ((n_of[0] > n_of[1] ? n_of[0] : n_of[1]) + NSUB - 1) / NSUB;
+        }
         return true;
     };
 
@@ -218,7 +240,8 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int s = 0; ok; ++s) {
                 int head, q0, n_of[2], nmax;
             bool again;
-                if (!sub_item(s, head, q0, n_of, nmax, again)) break;
+            int page0, part;
+                if (!sub_item(s, head, q0, n_of, nmax, again, page0, part)) break;
                 const int kv_head = head / kv_group;   // grouped-query attention: kv_group query heads per K/V head
                 for (int i = 0; i < 2 && ok; ++i) {
                     if (n_of[i] == 0) continue;
@@ -245,8 +268,8 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     tc_mbar_expect_tx(&bars[B_KVFULL + slot], KV_BYTES);
                     const CUtensorMap* map = (l & 1) ? &map_v : &map_k;
                     if (DENSE) {
-                        tc_tma_load_3d(sKV + slot * KV_BYTES, map, &bars[B_KVFULL + slot], 0, kv_head, j * BN);
-                        if (HD > 64) tc_tma_load_3d(sKV + slot * KV_BYTES + KV_BLK, map, &bars[B_KVFULL + slot], 64, kv_head, j * BN);
+                        tc_tma_load_3d(sKV + slot * KV_BYTES, map, &bars[B_KVFULL + slot], 0, kv_head, (page0 + (PARTS ? j >> d.twice : j)) * BN);
+                        if (HD > 64) tc_tma_load_3d(sKV + slot * KV_BYTES + KV_BLK, map, &bars[B_KVFULL + slot], 64, kv_head, (page0 + (PARTS ? j >> d.twice : j)) * BN);
                         continue;
                     }
                     at_tma_load_4d(sKV + slot * KV_BYTES, map, &bars[B_KVFULL + slot], 0, kv_head, 0, (int)page);
@@ -321,7 +344,8 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int s = 0; ok; ++s) {
                 int head, q0, n_of[2], nmax;
             bool again;
-                if (!sub_item(s, head, q0, n_of, nmax, again)) break;
+            int page0, part;
+                if (!sub_item(s, head, q0, n_of, nmax, again, page0, part)) break;
                 n = n_of[i];
                 if (n > 0) {
                     ok = __all_sync(0xffffffffu, tc_mbar_wait(&bars[B_QFULL + i], q_uses & 1, abort_flag, st, 21)) != 0;
@@ -408,11 +432,16 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         for (int s = 0; ok; ++s) {
         int head, q0, n_of[2], nmax;
             bool again;
-        if (!sub_item(s, head, q0, n_of, nmax, again)) break;
+            int page0, part;
+        if (!sub_item(s, head, q0, n_of, nmax, again, page0, part)) break;
         const int n = n_of[tile];
         const int R = q0 + tile * AT_BM + r;
         if (n == 0) {
-            if (DENSE && !again && R < a.seq_q) {               // a tile whose rows see nothing
+            if (PARTS && d.parts > 1 && !again && R < a.seq_q) {
+                const int64_t at = ((int64_t)part * a.seq_q + R) * a.heads + head;
+                for (int c = 0; c < OH; c += 4) *reinterpret_cast<float4*>(d.part_o + at * HD + half * OH + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (half == 0) d.part_lse[at] = -INFINITY;
+            } else if (DENSE && !again && R < a.seq_q) {        // a tile whose rows see nothing
                 __half* dst = reinterpret_cast<__half*>(a.arena) + a.o_off + (int64_t)R * a.o_row_stride + (int64_t)head * a.o_head_stride + half * OH;
                 for (int c = 0; c < OH; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
                 if (half == 0 && d.lse) d.lse[(int64_t)R * d.row + (int64_t)head * d.head] = -INFINITY;
@@ -433,8 +462,15 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             j_mask = jm > 0x7fffffff ? 0x7fffffff : (int)jm;
         }
         if (DENSE && d.kv_len / SB < j_mask) j_mask = d.kv_len / SB;      // the last keys do not fill a step
+        const int j0 = PARTS ? page0 * NSUB : 0;                // first step of the part
+        if (PARTS) {
+            j_mask -= j0;
+            limit -= (long long)j0 * SB;
+        }
         for (int j = 0; j < n && ok; ++j) {            // j counts steps of SB kv rows
             const int g = g0 + j;                      // step number of the tile across sub-items
+            const bool rest = PARTS && d.twice && ((j / NSUB) & 1);
+            const int js = PARTS && d.twice ? j / (2 * NSUB) * NSUB + j % NSUB : j;        // the step that its keys are
             const uint32_t slot_off = (g & 1) * 64;
             // the whole warp leaves together: the TMEM accesses below are warp-collective.
             // S(g) is issued after P V(g-2), which read the P columns of this slot.
@@ -454,10 +490,10 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             tc_tmem_ld_wait();
 
             // columns of this thread's range the row may see (all of them except on the diagonal pages)
-            const bool need_mask = j >= j_mask;          // same for the whole tile
+            const bool need_mask = js >= j_mask;          // same for the whole tile
             // hidden columns become -inf once (exp2 turns them into zeros), then every step takes the same path
             if (need_mask) {
-                const long long vis_ll = limit - ((long long)j * SB + half * HB) + 1;
+                const long long vis_ll = limit - ((long long)js * SB + half * HB) + 1;
                 const int vis = vis_ll > HB ? HB : (vis_ll < 0 ? 0 : (int)vis_ll);
 #pragma unroll
                 for (int c = 0; c < NCH; ++c)
@@ -505,12 +541,12 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
             for (int c = 0; c < NCH; ++c) {
                 uint32_t packed[CW / 2];
-                at_chunk_prob<CW, POLY, DENSE>(v[c], sl, m_exp, acc2, packed);
+                at_chunk_prob<CW, POLY, DENSE>(v[c], sl, m_exp, acc2, packed, rest);
                 tc_tmem_st<CW / 2>(p_addr + slot_off + c * (CW / 2), packed);
             }
             float s0, s1;
             at_unpack2(acc2, s0, s1);
-            l_run += s0 + s1;
+            if (!rest) l_run += s0 + s1;
             tc_tmem_st_wait();
             tc_fence_before_sync();          // P (and O) stores of this thread are complete
             __syncwarp();
@@ -524,12 +560,15 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             // total row sum = the two partial sums (same rescaling history on both threads)
             float l_other = 0.f;
             if (TPR == 1 || swap_with_partner(l_run, l_other)) {
-                // (the polynomial leaves 2^-125 of a hidden key: a row that sees none is known by its limit)
+                // (the polynomial leaves 2^-125 of a hidden key: a row that sees none, here, is known by its limit)
                 const float sum = DENSE && limit < 0 ? 0.f : l_run + l_other;
                 const float inv = DENSE && limit < 0 ? 0.f : 1.0f / sum;
                 const bool store = *abort_flag == 0 && R < a.seq_q;
                 // (m_ref in units of log 2; the logarithm of an empty sum is -inf)
-                if (DENSE && store && half == 0 && d.lse)
+                const int64_t at_part = ((int64_t)part * a.seq_q + R) * a.heads + head;
+                const bool part_of = PARTS && d.parts > 1;
+                if (part_of && store && half == 0) d.part_lse[at_part] = (m_ref + log2f(sum)) * 0.6931471805599453f;
+                if (DENSE && !part_of && store && half == 0 && d.lse)
                     d.lse[(int64_t)R * d.row + (int64_t)head * d.head] = (m_ref + log2f(sum)) * 0.6931471805599453f;
                 __half* dst = reinterpret_cast<__half*>(a.arena) + a.o_off + (int64_t)R * a.o_row_stride +
                               (int64_t)head * a.o_head_stride + half * OH;
@@ -538,7 +577,12 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     uint32_t o[32];
                     tc_tmem_ld32(o_addr + c0, o);
                     tc_tmem_ld_wait();
-                    if (store) {
+                    if (part_of && store) {
+#pragma unroll
+                        for (int c = 0; c < 32; c += 4)
+                            *reinterpret_cast<float4*>(d.part_o + at_part * HD + half * OH + c0 + c) =
+                                make_float4(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv, __uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
+                    } else if (store) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 8) {
                             uint4 w;
@@ -560,23 +604,56 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (warp == 1) tc_tmem_dealloc(tmem_base, 512);
 }
 
-template <int BN, int TPR, int POLY = 0, int HD = AT_D, bool DENSE = false>
+// Joins the parts of a row: their outputs weighted by exp(lse), in the order of the parts.  Eight columns to a thread.
+template <int HD>
+__global__ void __launch_bounds__(256) ktb_attention_join_fwd_kernel(const ktb_attn_args a, const at_dense d) {
+    const int64_t all = (int64_t)a.seq_q * a.heads, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / (HD / 8);
+    const int col = threadIdx.x % (HD / 8) * 8;
+    if (at >= all) return;
+    float m = -INFINITY;
+    for (int p = 0; p < d.parts; ++p) m = fmaxf(m, d.part_lse[p * all + at]);
+    float sum = 0.f, o[8] = {};
+    for (int p = 0; p < d.parts; ++p) {
+        const float l = d.part_lse[p * all + at], w = l == -INFINITY ? 0.f : expf(l - m);
+        sum += w;
+        const float4* from = reinterpret_cast<const float4*>(d.part_o + (p * all + at) * HD + col);
+        const float4 x = from[0], y = from[1];
+        o[0] = fmaf(w, x.x, o[0]), o[1] = fmaf(w, x.y, o[1]), o[2] = fmaf(w, x.z, o[2]), o[3] = fmaf(w, x.w, o[3]);
+        o[4] = fmaf(w, y.x, o[4]), o[5] = fmaf(w, y.y, o[5]), o[6] = fmaf(w, y.z, o[6]), o[7] = fmaf(w, y.w, o[7]);
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;          // (a NaN stays one)
+    const int64_t row = at / a.heads, head = at % a.heads;
+    uint4 w;
+    __half2* h = reinterpret_cast<__half2*>(&w);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(o[2 * i] * inv, o[2 * i + 1] * inv);
+    *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(a.arena) + a.o_off + row * a.o_row_stride + head * a.o_head_stride + col) = w;
+    if (col == 0 && d.lse) d.lse[row * d.row + head * d.head] = sum == 0.f ? -INFINITY : m + logf(sum);
+}
+
+template <int BN, int TPR, int POLY = 0, int HD = AT_D, bool DENSE = false, bool PARTS = false>
 static int launch_attn(ktb_ctx* ctx, const ktb_attn_args& a, const CUtensorMap& mq, const CUtensorMap& mk,
                        const CUtensorMap& mv, const at_dense& d = at_dense()) {
     constexpr int AT_STAGES = BN == 128 ? 4 : 8;
     constexpr size_t SMEM = 2 * AT_BM * HD * 2 + AT_STAGES * (size_t)(BN * HD * 2) + 2 * 2 * 2 * AT_BM * 4 + 1024 + 512;
     static bool attr_set[KTB_MAX_DEVICES] = {};     // the attribute is per device
     if (!attr_set[ctx->device & (KTB_MAX_DEVICES - 1)]) {
-        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_fwd_kernel<BN, TPR, POLY, HD, DENSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
+        KTB_CUDA(ctx, cudaFuncSetAttribute(ktb_attention_fwd_kernel<BN, TPR, POLY, HD, DENSE, PARTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)SMEM));
         attr_set[ctx->device & (KTB_MAX_DEVICES - 1)] = true;
     }
     const int q_pairs = (a.seq_q + 2 * AT_BM - 1) / (2 * AT_BM);
     // an item = the tile pairs (q_pairs - 1 - r, r) of one head; one persistent CTA per SM walks them
-    const long long items = (long long)((q_pairs + 1) / 2) * a.heads;
+    const long long items = (long long)((q_pairs + 1) / 2) * a.heads * (PARTS ? d.parts : 1);
     if (items > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_fwd", "too many query tiles");
+    const long long blocks = ((long long)a.seq_q * a.heads * (HD / 8) + 255) / 256;        // (of joining parts)
+    if (PARTS && blocks > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_dense", "too many rows in parts");
     const int grid = items < ctx->sm_count ? (int)items : ctx->sm_count;
-    ktb_attention_fwd_kernel<BN, TPR, POLY, HD, DENSE><<<grid, 128 + 256 * TPR, SMEM, ctx->stream>>>(mq, mk, mv, a, d, q_pairs, (int)items, ctx->dev_status);
+    ktb_attention_fwd_kernel<BN, TPR, POLY, HD, DENSE, PARTS><<<grid, 128 + 256 * TPR, SMEM, ctx->stream>>>(mq, mk, mv, a, d, q_pairs, (int)items, ctx->dev_status);
     KTB_CHECK_LAUNCH(ctx, "ktb_attention_fwd_kernel");
+    if (PARTS && d.parts > 1) {
+        ktb_attention_join_fwd_kernel<HD><<<(unsigned)blocks, 256, 0, ctx->stream>>>(a, d);
+        KTB_CHECK_LAUNCH(ctx, "ktb_attention_join_fwd_kernel");
+    }
     return KTB_OK;
 }
 
@@ -641,6 +718,10 @@ extern "C" int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_arg
     const int64_t all = b.q_off | b.k_off | b.v_off | b.o_off | b.q_row | b.q_head | b.k_row | b.k_head | b.v_row | b.v_head | b.o_row | b.o_head;
     if ((all & 7) || (reinterpret_cast<uintptr_t>(b.arena) & 15))
         return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "strides and offsets must be multiples of 8 elements");
+    if (b.parts < 0 || b.parts > 64 || b.twice < 0 || b.twice > 1) return ktb_fail(ctx, KTB_E_ARG, me, "parts of the keys, twice");
+    if (b.parts > 1 && (!b.dev_scratch || (reinterpret_cast<uintptr_t>(b.dev_scratch) & 15) ||
+                        b.scratch_bytes < (int64_t)b.parts * b.q_len * b.heads * (b.head_dim + 1) * 4))
+        return ktb_fail(ctx, KTB_E_ARG, me, "scratch too small for the parts");
     __half* base = reinterpret_cast<__half*>(b.arena);
     CUtensorMap mq, mk, mv;
     const uint32_t box[3] = {64, 1, 128};
@@ -674,5 +755,11 @@ extern "C" int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_arg
     d.row = b.lse_row;
     d.head = b.lse_head;
     d.kv_len = b.kv_len;
+    d.parts = b.parts > 1 ? b.parts : 1;
+    d.twice = b.twice;
+    d.part_o = reinterpret_cast<float*>(b.dev_scratch);
+    d.part_lse = d.part_o + (int64_t)b.parts * b.q_len * b.heads * b.head_dim;
+    if (b.parts > 1 || b.twice)
+        return b.head_dim == 64 ? launch_attn<128, 1, 1, 64, true, true>(ctx, a, mq, mk, mv, d) : launch_attn<128, 1, 1, 128, true, true>(ctx, a, mq, mk, mv, d);
     return b.head_dim == 64 ? launch_attn<128, 1, 1, 64, true>(ctx, a, mq, mk, mv, d) : launch_attn<128, 1, 1, 128, true>(ctx, a, mq, mk, mv, d);
 }

@@ -29,6 +29,9 @@ from .lower_mm import _is_zero_const, _unext
 from .trace import Access, LoopInfo, Node, Store, Unsupported, iv_full
 
 
+SMS, TILE, STEP = 148, 128, 64           # SMs; rows that a CTA owns, rows that it streams at a time
+
+
 # ---- pieces of the expressions ------------------------------------------------------------------------------------
 def _load(n: Node, dtype: str = "f16") -> Optional[Access]:
     """The direct f16 tile behind views and an extension to f32 (or a tile of another type as it is)."""
@@ -406,6 +409,32 @@ def _disjoint(arena: ArenaMap, reads, writes) -> bool:
     return not any(_runs_overlap(*a, *b) for i, a in enumerate(writes) for b in list(writes[i + 1:]) + spans)
 
 
+def dense_parts(q_len: int, kv_len: int, heads: int) -> int:
+    """Parts that the keys of the forward pass are cut into.
+
+    A CTA takes two pairs of 128-row tiles of a head, the last ones with the first ones.  Where these leave half of the SMs or
+    more without work, the keys are cut until they do not: one query of 32 heads over 8192 keys took 88 us, in four parts 33; 1024
+    queries of 32 heads over 16384 keys 445 us, in two 252; one query of 8 heads over 65536 keys 644 us, in sixteen 56.  A part and
+    joining it cost four microseconds, 512 keys five: smaller parts gain nothing (64 queries of 8 heads over 1024 keys 15.4 us, in
+    two 16.5; over 2048 keys 24.8, in four 16.6)."""
+    items = -(-(-(-q_len // 256)) // 2) * heads
+    return max(1, min(16, SMS // items, kv_len // 512)) if kv_len >= 1536 else 1
+
+
+# (An output's error stays below 1.5 of its rounding from some 20 rows on, a gradient's, three sums of which each may be off, from 200.)
+FEW_ROWS_FORWARD, FEW_ROWS_BACKWARD = 24, 256
+
+
+def few_rows(q_len: int, heads: int, causal: int, delta: int, most: int) -> bool:
+    """Whether at most ``most`` rows see a key.
+
+    P and dS are rounded to f16 before they are multiplied.  Every result is a sum of many products, so that over many rows these
+    roundings come to as much as the result's own and together to 1.41 of it.  Over a few rows they are a matter of luck: of sixty
+    draws of one query over 700 keys the error of an output was 1.42 of the rounding on average and 1.76 at most, of a gradient
+    over 2 x 2 positions 1.4 and 2.1.  There the kernels multiply what the rounding left out too."""
+    return (q_len + min(delta, 0) if causal else q_len) * heads <= most
+
+
 class AttentionDenseStatement(Statement):
     """The forward pass; the store of the rows' log-sum-exp behind it joins."""
     kind = "attention_dense"
@@ -460,7 +489,15 @@ class AttentionDenseStatement(Statement):
         seen = np.full(nr, k.rows) if not causal else np.clip(np.arange(nr) + 1 + a.causal_delta, 0, k.rows)
         self.flops = int(4 * nh * hd * seen.sum())
         self._bytes = 2 * hd * (2 * nr * nh + 2 * k.rows * (nh // grp)) + (4 * nr * nh if self.used == 2 else 0)
+        # (by the whole tensors: a rank that has some of the cores sums in the same parts)
+        a.parts = dense_parts(q.rows, k.rows, q.heads)
+        a.twice = few_rows(q.rows, q.heads, causal, delta, FEW_ROWS_FORWARD)
         self.device_arrays = []
+        if a.parts > 1:
+            a.scratch_bytes = 4 * a.parts * nr * nh * (hd + 1)
+            a.dev_scratch = dev.alloc(a.scratch_bytes)
+            self.device_arrays = [a.dev_scratch]
+            self.launches = 2
         self.fps = _footprints(arena, (q, k, v), writes, stmt_id)
 
     def launch(self, dev, arena_ptr):
@@ -472,9 +509,6 @@ class AttentionDenseStatement(Statement):
 
     def bytes_moved(self):
         return self._bytes
-
-
-SMS, TILE, STEP = 148, 128, 64           # rows that a CTA owns, rows that it streams at a time
 
 
 def grad_parts(q_len: int, kv_len: int, heads: int, kv_heads: int, causal: int, delta: int) -> Tuple[int, int]:
@@ -639,6 +673,8 @@ class AttentionGradStatement(Statement):
         for ptr in self.device_arrays:
             self.dev.free(ptr)
         self.device_arrays = []
+        # (of a single key, that same kernel keeps what two orders of a sum differ by from passing for a gradient)
+        a.twice = a.kv_len == 1 or few_rows(a.q_len, a.heads, a.causal, a.causal_delta, FEW_ROWS_BACKWARD)
         self._cut(self.dev, *grad_parts(a.q_len, a.kv_len, a.heads, k.heads, a.causal, a.causal_delta))
         self.fps = _footprints(self.arena, walks.values(), writes, self.id)
 

@@ -137,7 +137,8 @@ class AttnArgs(C.Structure):
 class AttnDenseArgs(C.Structure):
     _fields_ = [("arena", C.c_void_p)] + \
         [(n, C.c_int64) for n in "q_off k_off v_off o_off lse_off q_row q_head k_row k_head v_row v_head o_row o_head lse_row lse_head".split()] + \
-        [(n, C.c_int32) for n in "q_len kv_len heads kv_group head_dim causal causal_delta".split()] + [("scale", C.c_float)]
+        [(n, C.c_int32) for n in "q_len kv_len heads kv_group head_dim causal causal_delta".split()] + [("scale", C.c_float)] + \
+        [("parts", C.c_int32), ("twice", C.c_int32), ("dev_scratch", C.c_void_p), ("scratch_bytes", C.c_int64)]
 
 
 ATTN_DQ, ATTN_DK, ATTN_DV = 1, 2, 4
@@ -148,7 +149,7 @@ class AttnBwdArgs(C.Structure):
         [(n, C.c_int64) for n in ("q_off k_off v_off o_off do_off lse_off dq_off dk_off dv_off q_row q_head k_row k_head v_row v_head "
                                   "o_row o_head do_row do_head lse_row lse_head dq_row dq_head dk_row dk_head dv_row dv_head").split()] + \
         [(n, C.c_int32) for n in "q_len kv_len heads kv_group head_dim causal causal_delta".split()] + [("scale", C.c_float)] + \
-        [(n, C.c_int32) for n in "want dq_row0 dq_rows dq_head0 dq_heads dk_row0 dk_rows dk_head0 dk_heads key_parts query_parts reserved".split()] + \
+        [(n, C.c_int32) for n in "want dq_row0 dq_rows dq_head0 dq_heads dk_row0 dk_rows dk_head0 dk_heads key_parts query_parts twice".split()] + \
         [("dev_scratch", C.c_void_p), ("scratch_bytes", C.c_int64)]
 
 

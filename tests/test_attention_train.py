@@ -14,7 +14,7 @@ import pytest
 
 from ktir_cpu_b200 import HardwareConfig, KTIRInterpreter, kernels as K, runtime as R
 from ktir_cpu_b200.interpreter import Session
-from ktir_cpu_b200.lower_attn_train import grad_parts, grad_scratch_bytes
+from ktir_cpu_b200.lower_attn_train import FEW_ROWS_BACKWARD, FEW_ROWS_FORWARD, dense_parts, few_rows, grad_parts, grad_scratch_bytes
 from ktir_cpu_b200.parser import KTIRParser
 from oracle.numpy_interp import OracleInterpreter
 
@@ -38,8 +38,8 @@ def _seen(q_len, kv_len, causal):
     return j <= i + kv_len - q_len if causal else np.ones((q_len, kv_len), bool)
 
 
-def formulas(kw, do, causal, o=None, lse=None, scale=None):
-    """Outputs in 64 bits and, for each, a bound on what the kernels' roundings move: name -> (value, bound)."""
+def formulas(kw, do, causal, o=None, lse=None, scale=None, half=HALF):
+    """Outputs in 64 bits and, for each, a bound on what the kernels' roundings move: name -> (value, bound).  ``half``: of P and dS."""
     q, k, v = (kw[n].astype(np.float64).transpose(1, 0, 2) for n in ("query_ptr", "key_ptr", "value_ptr"))
     grp, (q_len, kv_len) = len(q) // len(k), (q.shape[1], k.shape[1])
     k, v = np.repeat(k, grp, 0), np.repeat(v, grp, 0)
@@ -54,7 +54,7 @@ def formulas(kw, do, causal, o=None, lse=None, scale=None):
         out = {}
         if do is None:
             res, spread = p @ v, p @ np.abs(v)
-            out["output_ptr"] = (res, (HALF + F32) * spread + HALF * np.abs(res) + 2.0 ** -25)
+            out["output_ptr"] = (res, (half + F32) * spread + HALF * np.abs(res) + 2.0 ** -25)
             l64 = (m + np.log(total))[..., 0]
             out["lse_ptr"] = (l64[..., None], 2.0 ** -19 * (1 + np.abs(np.where(np.isfinite(l64), l64, 0)))[..., None])
         else:
@@ -68,8 +68,8 @@ def formulas(kw, do, causal, o=None, lse=None, scale=None):
             floor = np.repeat(2.0 * big, grp)[:, None, None] * 2.0 ** -39      # half of f16's smallest step, shifted back
             # what f32 moves in dS: P from the scores, dO V^T and D from their own sums
             size = p * (np.abs(do) @ np.abs(v).transpose(0, 2, 1) + (np.abs(do) * np.abs(o)).sum(-1, keepdims=True))
-            eds = HALF * np.abs(ds) + F32 * size + np.where(seen, floor, 0)
-            ep = (HALF + F32) * p + np.where(seen, 2.0 ** -39, 0)
+            eds = half * np.abs(ds) + F32 * size + np.where(seen, floor, 0)
+            ep = (half + F32) * p + np.where(seen, 2.0 ** -39, 0)
             for name, val, err in (("query_grad_ptr", scale * (ds @ k), scale * (eds @ np.abs(k) + F32 * (np.abs(ds) @ np.abs(k)))),
                                    ("key_grad_ptr", scale * shared(ds.transpose(0, 2, 1) @ q), scale * shared(eds.transpose(0, 2, 1) @ np.abs(q) + F32 * (np.abs(ds).transpose(0, 2, 1) @ np.abs(q)))),
                                    ("value_grad_ptr", shared(p.transpose(0, 2, 1) @ do), shared(ep.transpose(0, 2, 1) @ np.abs(do)))):
@@ -256,10 +256,21 @@ def test_ranks_take_their_heads(world):
 
 @pytest.mark.parametrize("q_len,kv_len,heads,kv_heads,causal,parts", [
     (2048, 2048, 256, 256, True, (1, 1)), (197, 197, 12, 12, False, (1, 1)), (8192, 8192, 16, 4, True, (1, 1)),   # enough tiles
-    (1000, 1000, 8, 1, False, (13, 2)), (1, 8192, 32, 8, True, (1, 5)), (4096, 4096, 1, 1, False, (3, 3)), (1, 1, 1, 1, True, (1, 1)),
+    (1000, 1000, 8, 1, False, (11, 1)), (1, 8192, 32, 8, True, (1, 4)), (4096, 4096, 1, 1, False, (3, 3)), (1, 1, 1, 1, True, (1, 1)),
     (100, 20, 2, 2, True, (1, 1)), (4096, 64, 8, 1, False, (16, 1))])
 def test_long_walks_are_cut_where_there_are_few(q_len, kv_len, heads, kv_heads, causal, parts):
     assert grad_parts(q_len, kv_len, heads, kv_heads, int(causal), kv_len - q_len if causal else 0) == parts
+
+
+@pytest.mark.parametrize("q_len,kv_len,heads,parts", [(2048, 2048, 256, 1), (197, 197, 12, 1), (1, 1, 1, 1), (1, 511, 1, 1), (1, 1535, 4, 1), (1, 1536, 4, 3),
+                                                      (1, 8192, 4, 16), (1024, 65536, 32, 2), (1024, 65536, 37, 2), (1024, 65536, 38, 1), (4096, 4096, 2, 8)])
+def test_keys_are_cut_where_there_are_few_queries(q_len, kv_len, heads, parts):
+    assert dense_parts(q_len, kv_len, heads) == parts
+
+
+def test_few_rows_are_those_that_see_a_key():
+    assert few_rows(1, 256, 0, 0, 256) and not few_rows(1, 257, 0, 0, 256) and not few_rows(300, 1, 0, -299, 256)
+    assert few_rows(8000, 8, 1, 32 - 8000, 256) and not few_rows(33, 8, 1, 50, 256)
 
 
 @pytest.mark.parametrize("parts", [(1, 1), (3, 1), (1, 5), (8, 8), (0, 0)])
@@ -304,6 +315,45 @@ def test_forward(q_len, kv_len, heads, kv_heads, hd, causal, build_lib):
     src = K.attention_forward(q_len, kv_len, heads, kv_heads, hd, causal)
     got = _run(src, FWD, _kwargs(FWD, kw, q_len, heads, hd), "attention_dense", times=3)
     _check(got, formulas(kw, None, causal))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c,parts", [((2500, 1540, 2, 1, 128, True), 3), ((257, 2200, 3, 3, 64, True), 4), ((1, 16400, 1, 1, 128, True), 16),
+                                     ((300, 5000, 30, 2, 64, False), 4), ((700, 1601, 4, 4, 128, True), 3)])
+def test_forward_in_parts(c, parts, build_lib):
+    """Parts that rows see nothing of, rows that see nothing at all, a last part that fills no step."""
+    assert dense_parts(c[0], c[1], c[2]) == parts
+    kw, _ = _inputs(*c[:5], seed=c[1])
+    got = _run(K.attention_forward(*c), FWD, _kwargs(FWD, kw, c[0], c[2], c[4]), "attention_dense", times=3)
+    _check(got, formulas(kw, None, c[5]))
+
+
+FEW = [(2, 2, 4, 4, 128, True), (1, 1, 8, 8, 64, False), (6, 14, 8, 4, 64, False), (1, 700, 8, 8, 128, True), (20, 100, 2, 2, 64, False), (3, 5000, 8, 1, 64, True),
+       (7, 7, 4, 1, 128, True), (130, 65, 1, 1, 128, False), (100, 8, 4, 4, 64, True), (2, 129, 3, 1, 128, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", FEW)
+def test_few_rows_lose_nothing_to_f16_operands(c, build_lib):
+    """Where few rows see a key, what f16 leaves out of P and dS is multiplied too: 2^-11 of 2^-11 is all that stays out."""
+    kw, do = _inputs(*c[:5], seed=c[1])
+    got = _run(K.attention_forward(*c), FWD, _kwargs(FWD, kw, c[0], c[2], c[4]), "attention_dense", times=3)
+    delta = c[1] - c[0] if c[5] else 0
+    _check(got, formulas(kw, None, c[5], half=HALF * HALF if few_rows(c[0], c[2], c[5], delta, FEW_ROWS_FORWARD) else HALF))
+    o, lse = _forward_results(kw, c[5])
+    got = _run(K.attention_backward(*c), BWD, _kwargs(BWD, kw, c[0], c[2], c[4], do, o, lse), "attention_bwd", times=3)
+    assert few_rows(c[0], c[2], c[5], delta, FEW_ROWS_BACKWARD)
+    _check(got, formulas(kw, do, c[5], o, lse, half=HALF * HALF))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("q_len,heads,kv_heads,hd,causal", [(1, 4, 4, 64, False), (1, 8, 2, 128, True), (60, 8, 8, 128, False), (60, 4, 1, 64, True)])
+def test_one_key_has_no_gradient_of_its_scores(q_len, heads, kv_heads, hd, causal, build_lib):
+    """P is 1 whatever the scores are, and O is V: dQ and dK are nothing, not what two orders of a sum differ by."""
+    kw, do = _inputs(q_len, 1, heads, kv_heads, hd, seed=hd)
+    o, lse = _forward_results(kw, causal)
+    got = _run(K.attention_backward(q_len, 1, heads, kv_heads, hd, causal), BWD, _kwargs(BWD, kw, q_len, heads, hd, do, o, lse), "attention_bwd")
+    assert not got["query_grad_ptr"].any() and not got["key_grad_ptr"].any() and got["value_grad_ptr"].any()
 
 
 @pytest.mark.gpu
@@ -441,7 +491,7 @@ def test_a_training_step_of_an_attention_layer(build_lib):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("c", [(100, 200, 8, 4, 64, True), (400, 300, 8, 2, 128, False)])         # (the second one in parts)
+@pytest.mark.parametrize("c", [(100, 200, 8, 4, 64, True), (400, 300, 8, 2, 128, False), (48, 1600, 8, 2, 64, True)])   # (gradients, outputs in parts)
 def test_shards_add_up_to_the_whole(c, build_lib):
     kw, do = _inputs(*c[:5])
     o, lse = _forward_results(kw, c[5])
@@ -558,14 +608,15 @@ def test_launchers_refuse(build_lib):
                                ("dq_row0", -1, -2), ("dq_rows", 65, -2), ("dq_heads", 5, -2), ("dq_head0", 1, -2), ("dk_rows", 65, -2), ("dk_head0", 1, -2),
                                ("dk_row0", 64, -2), ("k_row", 12, -3), ("q_off", st.args.q_off + 4, -3), ("dv_head", 2, -3), ("dev_scratch", None, -2),
                                ("dev_scratch", st.args.dev_scratch + 16, -2), ("scratch_bytes", st.args.scratch_bytes - 1, -2),
-                               ("key_parts", -1, -2), ("query_parts", 65, -2), ("key_parts", 2, -2), ("query_parts", 2, -2)):
+                               ("key_parts", -1, -2), ("query_parts", 65, -2), ("key_parts", 2, -2), ("query_parts", 2, -2), ("twice", 2, -2), ("twice", -1, -2)):
         refused("ktb_launch_attention_bwd", st.args, field, value, code, "attention_bwd")
     assert dev.lib.ktb_attention_bwd_scratch_bytes(C.byref(st.args)) == st.args.scratch_bytes
     fwd = KTIRInterpreter()
     fwd.load(K.attention_forward(64, 64, 4, 2, 64, True))
     fs, _ = fwd.session(FWD, **_kwargs(FWD, kw, 64, 4, 64))
     for field, value, code in (("head_dim", 96, -3), ("kv_group", 0, -2), ("kv_group", 3, -2), ("q_len", -1, -2), ("kv_len", 0, -3), ("scale", 0.0, -3),
-                               ("scale", -1.0, -3), ("scale", float("nan"), -3), ("v_row", 12, -3), ("o_off", 4, -3)):
+                               ("scale", -1.0, -3), ("scale", float("nan"), -3), ("v_row", 12, -3), ("o_off", 4, -3), ("parts", -1, -2), ("parts", 65, -2), ("twice", 2, -2), ("twice", -1, -2),
+                               ("parts", 2, -2)):
         refused("ktb_launch_attention_dense", fs.plan.statements[0].args, field, value, code, "attention_dense")
     fwd.close()
     gpu.close()
