@@ -496,7 +496,7 @@ typedef struct {
     int32_t causal, causal_delta;
     float scale;
     /* few queries and heads: parts that the keys are cut into (0, 1: none; 64 at most), with dev_scratch (16-byte boundary) of
-       4 * parts * q_len * heads * (head_dim + 1) bytes to join them in.  The order of a sum depends on them; launches that share
+       4 * parts * (q_len up to a multiple of 32) * heads * (head_dim + 1) bytes to join them in.  The order of a sum depends on them; launches that share
        scratch must be ordered. */
     int32_t parts;
     int32_t twice;              /* 1: P is multiplied as f16 and once more as what that left out (half the rate; for few rows) */

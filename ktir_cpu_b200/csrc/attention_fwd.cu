@@ -122,8 +122,17 @@ struct at_dense {
     float* lse;                 // null: not wanted
     int64_t row, head;
     int kv_len, parts, twice;
-    float *part_o, *part_lse;   // [part][query][head][head_dim], [part][query][head]
+    float4* part_o;             // [part][head][query / 32][column / 4][query % 32]: a warp's rows side by side
+    float* part_lse;            // [part][head][query, up to a multiple of 32]
+    int rows32;                 // queries / 32, rounded up
 };
+
+// Where a part keeps row R: the index of its log-sum-exp; of its first four columns it is `at_part_o` (32 further for every next four).
+static __device__ __forceinline__ int64_t at_part_row(const at_dense& d, int heads, int part, int head, int R) {
+    return ((int64_t)part * heads + head) * d.rows32 * 32 + R;
+}
+template <int HD>
+static __device__ __forceinline__ int64_t at_part_o(int64_t row) { return (row >> 5) * (HD / 4 * 32) + (row & 31); }
 
 template <int BN, int TPR, int POLY, int HD, bool DENSE, bool PARTS>
 __global__ void __launch_bounds__(128 + 256 * TPR, 1)
@@ -438,8 +447,8 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const int R = q0 + tile * AT_BM + r;
         if (n == 0) {
             if (PARTS && d.parts > 1 && !again && R < a.seq_q) {
-                const int64_t at = ((int64_t)part * a.seq_q + R) * a.heads + head;
-                for (int c = 0; c < OH; c += 4) *reinterpret_cast<float4*>(d.part_o + at * HD + half * OH + c) = make_float4(0.f, 0.f, 0.f, 0.f);
+                const int64_t at = at_part_row(d, a.heads, part, head, R);
+                for (int c = 0; c < OH / 4; ++c) d.part_o[at_part_o<HD>(at) + (half * OH / 4 + c) * 32] = make_float4(0.f, 0.f, 0.f, 0.f);
                 if (half == 0) d.part_lse[at] = -INFINITY;
             } else if (DENSE && !again && R < a.seq_q) {        // a tile whose rows see nothing
                 __half* dst = reinterpret_cast<__half*>(a.arena) + a.o_off + (int64_t)R * a.o_row_stride + (int64_t)head * a.o_head_stride + half * OH;
@@ -565,7 +574,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 const float inv = DENSE && limit < 0 ? 0.f : 1.0f / sum;
                 const bool store = *abort_flag == 0 && R < a.seq_q;
                 // (m_ref in units of log 2; the logarithm of an empty sum is -inf)
-                const int64_t at_part = ((int64_t)part * a.seq_q + R) * a.heads + head;
+                const int64_t at_part = at_part_row(d, a.heads, part, head, R);
                 const bool part_of = PARTS && d.parts > 1;
                 if (part_of && store && half == 0) d.part_lse[at_part] = (m_ref + log2f(sum)) * 0.6931471805599453f;
                 if (DENSE && !part_of && store && half == 0 && d.lse)
@@ -580,7 +589,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     if (part_of && store) {
 #pragma unroll
                         for (int c = 0; c < 32; c += 4)
-                            *reinterpret_cast<float4*>(d.part_o + at_part * HD + half * OH + c0 + c) =
+                            d.part_o[at_part_o<HD>(at_part) + (half * OH + c0 + c) / 4 * 32] =
                                 make_float4(__uint_as_float(o[c]) * inv, __uint_as_float(o[c + 1]) * inv, __uint_as_float(o[c + 2]) * inv, __uint_as_float(o[c + 3]) * inv);
                     } else if (store) {
 #pragma unroll
@@ -604,31 +613,32 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     if (warp == 1) tc_tmem_dealloc(tmem_base, 512);
 }
 
-// Joins the parts of a row: their outputs weighted by exp(lse), in the order of the parts.  Eight columns to a thread.
+// Joins the parts of a row: their outputs weighted by exp(lse), in the order of the parts.  A warp takes 32 rows of a head, a
+// thread eight columns of one.
 template <int HD>
 __global__ void __launch_bounds__(256) ktb_attention_join_fwd_kernel(const ktb_attn_args a, const at_dense d) {
-    const int64_t all = (int64_t)a.seq_q * a.heads, at = ((int64_t)blockIdx.x * 256 + threadIdx.x) / (HD / 8);
-    const int col = threadIdx.x % (HD / 8) * 8;
-    if (at >= all) return;
+    const int64_t warp = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 5, group = warp / (HD / 8);        // 32 rows of a head
+    const int head = (int)(group / d.rows32), row = (int)(group % d.rows32) * 32 + (threadIdx.x & 31), col = (int)(warp % (HD / 8)) * 8;
+    if (head >= a.heads || row >= a.seq_q) return;
     float m = -INFINITY;
-    for (int p = 0; p < d.parts; ++p) m = fmaxf(m, d.part_lse[p * all + at]);
+    for (int p = 0; p < d.parts; ++p) m = fmaxf(m, d.part_lse[at_part_row(d, a.heads, p, head, row)]);
     float sum = 0.f, o[8] = {};
     for (int p = 0; p < d.parts; ++p) {
-        const float l = d.part_lse[p * all + at], w = l == -INFINITY ? 0.f : expf(l - m);
+        const int64_t at = at_part_row(d, a.heads, p, head, row);
+        const float l = d.part_lse[at], w = l == -INFINITY ? 0.f : expf(l - m);
         sum += w;
-        const float4* from = reinterpret_cast<const float4*>(d.part_o + (p * all + at) * HD + col);
-        const float4 x = from[0], y = from[1];
+        const float4* from = d.part_o + at_part_o<HD>(at) + col / 4 * 32;
+        const float4 x = from[0], y = from[32];
         o[0] = fmaf(w, x.x, o[0]), o[1] = fmaf(w, x.y, o[1]), o[2] = fmaf(w, x.z, o[2]), o[3] = fmaf(w, x.w, o[3]);
         o[4] = fmaf(w, y.x, o[4]), o[5] = fmaf(w, y.y, o[5]), o[6] = fmaf(w, y.z, o[6]), o[7] = fmaf(w, y.w, o[7]);
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;          // (a NaN stays one)
-    const int64_t row = at / a.heads, head = at % a.heads;
     uint4 w;
     __half2* h = reinterpret_cast<__half2*>(&w);
 #pragma unroll
     for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(o[2 * i] * inv, o[2 * i + 1] * inv);
-    *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(a.arena) + a.o_off + row * a.o_row_stride + head * a.o_head_stride + col) = w;
-    if (col == 0 && d.lse) d.lse[row * d.row + head * d.head] = sum == 0.f ? -INFINITY : m + logf(sum);
+    *reinterpret_cast<uint4*>(reinterpret_cast<__half*>(a.arena) + a.o_off + (int64_t)row * a.o_row_stride + (int64_t)head * a.o_head_stride + col) = w;
+    if (col == 0 && d.lse) d.lse[(int64_t)row * d.row + (int64_t)head * d.head] = sum == 0.f ? -INFINITY : m + logf(sum);
 }
 
 template <int BN, int TPR, int POLY = 0, int HD = AT_D, bool DENSE = false, bool PARTS = false>
@@ -645,7 +655,7 @@ static int launch_attn(ktb_ctx* ctx, const ktb_attn_args& a, const CUtensorMap& 
     // an item = the tile pairs (q_pairs - 1 - r, r) of one head; one persistent CTA per SM walks them
     const long long items = (long long)((q_pairs + 1) / 2) * a.heads * (PARTS ? d.parts : 1);
     if (items > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_fwd", "too many query tiles");
-    const long long blocks = ((long long)a.seq_q * a.heads * (HD / 8) + 255) / 256;        // (of joining parts)
+    const long long blocks = ((long long)d.rows32 * 32 * a.heads * (HD / 8) + 255) / 256;        // (of joining parts)
     if (PARTS && blocks > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_dense", "too many rows in parts");
     const int grid = items < ctx->sm_count ? (int)items : ctx->sm_count;
     ktb_attention_fwd_kernel<BN, TPR, POLY, HD, DENSE, PARTS><<<grid, 128 + 256 * TPR, SMEM, ctx->stream>>>(mq, mk, mv, a, d, q_pairs, (int)items, ctx->dev_status);
@@ -720,7 +730,7 @@ extern "C" int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_arg
         return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "strides and offsets must be multiples of 8 elements");
     if (b.parts < 0 || b.parts > 64 || b.twice < 0 || b.twice > 1) return ktb_fail(ctx, KTB_E_ARG, me, "parts of the keys, twice");
     if (b.parts > 1 && (!b.dev_scratch || (reinterpret_cast<uintptr_t>(b.dev_scratch) & 15) ||
-                        b.scratch_bytes < (int64_t)b.parts * b.q_len * b.heads * (b.head_dim + 1) * 4))
+                        b.scratch_bytes < (int64_t)b.parts * (((int64_t)b.q_len + 31) / 32 * 32) * b.heads * (b.head_dim + 1) * 4))
         return ktb_fail(ctx, KTB_E_ARG, me, "scratch too small for the parts");
     __half* base = reinterpret_cast<__half*>(b.arena);
     CUtensorMap mq, mk, mv;
@@ -757,8 +767,9 @@ extern "C" int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_arg
     d.kv_len = b.kv_len;
     d.parts = b.parts > 1 ? b.parts : 1;
     d.twice = b.twice;
-    d.part_o = reinterpret_cast<float*>(b.dev_scratch);
-    d.part_lse = d.part_o + (int64_t)b.parts * b.q_len * b.heads * b.head_dim;
+    d.rows32 = (b.q_len + 31) / 32;
+    d.part_o = reinterpret_cast<float4*>(b.dev_scratch);
+    d.part_lse = reinterpret_cast<float*>(b.dev_scratch) + (int64_t)d.parts * d.rows32 * 32 * b.heads * b.head_dim;
     if (b.parts > 1 || b.twice)
         return b.head_dim == 64 ? launch_attn<128, 1, 1, 64, true, true>(ctx, a, mq, mk, mv, d) : launch_attn<128, 1, 1, 128, true, true>(ctx, a, mq, mk, mv, d);
     return b.head_dim == 64 ? launch_attn<128, 1, 1, 64, true>(ctx, a, mq, mk, mv, d) : launch_attn<128, 1, 1, 128, true>(ctx, a, mq, mk, mv, d);

@@ -494,7 +494,7 @@ class AttentionDenseStatement(Statement):
         a.twice = few_rows(q.rows, q.heads, causal, delta, FEW_ROWS_FORWARD)
         self.device_arrays = []
         if a.parts > 1:
-            a.scratch_bytes = 4 * a.parts * nr * nh * (hd + 1)
+            a.scratch_bytes = 4 * a.parts * (-(-nr // 32) * 32) * nh * (hd + 1)
             a.dev_scratch = dev.alloc(a.scratch_bytes)
             self.device_arrays = [a.dev_scratch]
             self.launches = 2
