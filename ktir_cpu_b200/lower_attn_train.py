@@ -451,6 +451,8 @@ class AttentionDenseStatement(Statement):
         hd = int(m["q"].shape[-1])
         if hd not in (64, 128):
             raise Unsupported("attention over whole sequences supports head_dim 64 and 128")
+        if not 0 < np.float32(m["scale"]) < np.inf:
+            raise Unsupported("a score scale that is not positive or not finite")
         q = _walk(m["q"], store.axes, sel, None, hd, arena, "Read from")
         o = _walk(store.target, store.axes, sel, None, hd, arena, "Scatter to")
         k, v = (_walk(m[x], store.axes, sel, T, hd, arena, "Read from") for x in ("k", "v"))
@@ -489,7 +491,8 @@ class AttentionDenseStatement(Statement):
         seen = np.full(nr, k.rows) if not causal else np.clip(np.arange(nr) + 1 + a.causal_delta, 0, k.rows)
         self.flops = int(4 * nh * hd * seen.sum())
         self._bytes = 2 * hd * (2 * nr * nh + 2 * k.rows * (nh // grp)) + (4 * nr * nh if self.used == 2 else 0)
-        # (by the whole tensors: a rank that has some of the cores sums in the same parts)
+        # (by the whole tensors: a rank that has some of the heads sums in the same parts; one that has some of the rows cuts
+        # them at other keys, and may differ in the last bit)
         a.parts = dense_parts(q.rows, k.rows, q.heads)
         a.twice = few_rows(q.rows, q.heads, causal, delta, FEW_ROWS_FORWARD)
         self.device_arrays = []
@@ -574,6 +577,8 @@ class AttentionGradStatement(Statement):
         hd = int(m["q"].shape[-1])
         if hd not in (64, 128):
             raise Unsupported("attention gradient supports head_dim 64 and 128")
+        if not np.isfinite(np.float32(m["scale"])):
+            raise Unsupported("a score scale that is not finite")
         over_keys = name == "dq"
 
         def own(acc, what="Read from"):
@@ -679,8 +684,8 @@ class AttentionGradStatement(Statement):
         self.fps = _footprints(self.arena, walks.values(), writes, self.id)
 
     def _cut(self, dev, key_parts: int, query_parts: int):
-        """The parts of the walks, and scratch for them.  (They follow from the whole tensors: a rank that has some of the cores
-        sums in the same parts.)"""
+        """The parts of the walks, and scratch for them.  (They follow from the whole tensors: a rank that has some of the heads
+        sums in the same parts; one that has some of the rows cuts them elsewhere, and may differ in the last bit.)"""
         a = self.args
         for ptr in self.device_arrays:
             dev.free(ptr)

@@ -254,6 +254,16 @@ def test_ranks_take_their_heads(world):
     assert covered == [(r * per * 2, per * 2, r * per, per, 7) for r in range(world)]
 
 
+@pytest.mark.parametrize("scale,fwd,bwd", [(0.0, 0, 1), (-0.5, 0, 1), (float("nan"), 0, 0), (float("inf"), 0, 0), (1e-30, 1, 1)])
+def test_scales_that_the_kernels_do_not_take_run_step_by_step(scale, fwd, bwd):
+    kw, do = _inputs(64, 64, 4, 2, 64)
+    o, lse = _forward_results(kw, True)
+    for fn, make, kind, fused in ((FWD, K.attention_forward, "attention_dense", fwd), (BWD, K.attention_backward, "attention_bwd", bwd)):
+        sess = _session(make(64, 64, 4, 2, 64, True), fn, _kwargs(fn, kw, 64, 4, 64, do, o, lse, np.float32(scale)))
+        kinds = {s.kind for s in sess.plan.statements}
+        assert kinds == ({kind} if fused else {"generic"})
+
+
 @pytest.mark.parametrize("q_len,kv_len,heads,kv_heads,causal,parts", [
     (2048, 2048, 256, 256, True, (1, 1)), (197, 197, 12, 12, False, (1, 1)), (8192, 8192, 16, 4, True, (1, 1)),   # enough tiles
     (1000, 1000, 8, 1, False, (11, 1)), (1, 8192, 32, 8, True, (1, 4)), (4096, 4096, 1, 1, False, (3, 3)), (1, 1, 1, 1, True, (1, 1)),
@@ -456,6 +466,33 @@ def test_sessions_side_by_side_and_new_inputs(build_lib):
             _check(got, formulas(kw, do, c[5], o, lse))
     for gpu in interps:
         gpu.close()
+
+
+@pytest.mark.gpu
+def test_many_calls_in_flight(build_lib):
+    """Candidates of one text on inputs of their own, several under way at a time: one plan's scratch and parts serve them all."""
+    from ktir_cpu_b200.batch import Candidate, evaluate_many
+    cands = []
+    for seed in range(4):
+        for c in ((40, 1700, 8, 2, 64, False), (300, 300, 2, 1, 128, True)):
+            kw, do = _inputs(*c[:5], seed=seed)
+            o, lse = _forward_results(kw, c[5])
+            cands.append(Candidate(K.attention_forward(*c), FWD, _kwargs(FWD, kw, c[0], c[2], c[4])))
+            cands.append(Candidate(K.attention_backward(*c), BWD, _kwargs(BWD, kw, c[0], c[2], c[4], do, o, lse)))
+        x = _inputs(70, 70, 4, 2, 64, seed=seed)[0]
+        cos, sin = K.rotary_tables(200, 64)
+        at = np.random.default_rng(seed).integers(0, 200, 70).astype(np.int32)
+        cands.append(Candidate(K.rotary(70, 4, 2, 64, table_rows=200), "rotary_kernel", dict(
+            query_out_ptr=np.zeros((70, 4, 64), np.float16), key_out_ptr=np.zeros((70, 2, 64), np.float16), query_ptr=x["query_ptr"],
+            key_ptr=x["key_ptr"], positions_ptr=at, cos_ptr=cos, sin_ptr=sin)))
+    res = evaluate_many(cands)
+    assert not res.errors
+    for i, c in enumerate(cands):
+        gpu = KTIRInterpreter()
+        gpu.load(c.source)
+        want = gpu.execute_function(c.function, **c.kwargs)
+        gpu.close()
+        assert res.outputs[i].keys() and all(v.tobytes() == want[n].tobytes() for n, v in res.outputs[i].items()), (i, c.function)
 
 
 @pytest.mark.gpu
