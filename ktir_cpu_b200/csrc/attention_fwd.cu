@@ -113,7 +113,9 @@ enum { B_QFULL = 0, B_QFREE = 2, B_KVFULL = 4, B_KVEMPTY = B_KVFULL + AT_MAX_STA
 // store the output, so a tile pair no longer pays a start-up and a drain of its own.
 //
 // DENSE: keys and values are rows of one tensor instead of pages, a.num_tiles groups of BN of them of which d.kv_len exist;
-// rows that see nothing give 0, and the log-sum-exp of every row is kept.  PARTS: the keys of an item are cut into d.parts
+// rows that see nothing give 0, and the log-sum-exp of every row is kept (256 heads of 2048 positions, 128 wide, causal: 291 us,
+// 944 TFLOP/s, 344 once the power cap holds; 1531 queries of 32 heads over 4603 keys 118 us: 96 items on 148 SMs, and parts
+// cost what they spread, 117 in three).  PARTS: the keys of an item are cut into d.parts
 // ranges, an item of its own each, where whole items would leave most SMs idle; ktb_attention_join_fwd_kernel joins them.  With
 // d.twice every page comes twice: P as f16 times V, then what that rounding left out (up to 2^-12 of P) times V.  A result is
 // the sum of a few large P, so that over many rows their roundings are as large as the result's own, 2^-12, but over a few rows

@@ -5,7 +5,8 @@
 // sequence indirect ktdp.load of two table rows, arith.mulf / subf / addf on broadcast tiles, ktdp.store, which the
 // reference dispatches op by op (ktir_cpu/ops/memory_ops.py:867-915, ktir_cpu/dialects/arith_ops.py:49-59).
 //
-// HBM bounds it: every element is read and written once.  A thread owns VEC pairs (16 bytes of x and of y, or of
+// HBM bounds it: every element is read and written once (8192 tokens of 72 heads of 128, f16: 52 us, 5.9 TB/s; a token is a
+// launch, 4 us).  A thread owns VEC pairs (16 bytes of x and of y, or of
 // adjacent pairs), or as many bytes behind the pairs, of up to HEADS heads of one token, so that it reads its table entries
 // once for all of them and has their loads in flight together; the position -> table -> product chain is entered after they
 // have been issued (asked for first, the position holds them up: 8192 tokens of 72 heads, 128 wide, 52 us -> 66).  What turns

@@ -1464,8 +1464,8 @@ def _attention_tiles(q_len, kv_len, heads, kv_heads, block_q, block_kv):
 
 
 def _attention_scores(p, q, k, q0, k0, dims, causal, kv_len, ind):
-    """Scaled scores of a tile of query rows (position-major, ``grp`` heads each) and a tile of keys; %{p}hidden says what
-    stands where a query does not see a key: ``None`` returned as its condition if it sees all."""
+    """The text that makes %{p}sc, the scaled scores of a tile of query rows (position-major, ``grp`` heads each) and a tile of keys,
+    and the lines that make %keep, whether a query sees a key, in a ``linalg.generic`` over them (``None``: it sees all)."""
     bm, bn, hd, grp = dims
     f = lambda shp, dt="f32": f"tensor<{_xs(shp, dt)}>"   # noqa: E731
     s = (f"{ind}%{p}kt_e = tensor.empty() : {f([hd, bn], 'f16')}\n"
