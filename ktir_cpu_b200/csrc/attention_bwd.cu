@@ -39,8 +39,8 @@ static __device__ __forceinline__ void ab_wait_for_rows() { asm volatile("gridde
 
 // ---- what the rows bring: 14 - lse / ln 2, D, |dO| per row, and the largest norms of a block of rows ---------------
 // HBM bounds it (O, dO and V once; 256 heads of 2048 positions, 128 wide: 86 us, 4.7 TB/s).  A block takes
-// 256 rows of heads, 2^heads_log neighbouring heads of 256 >> heads_log positions (so that what it reads lies together), head_dim / 8
-// threads each, four of their loads ahead of the arithmetic.
+// w.block rows of heads, 2^heads_log neighbouring heads of w.block >> heads_log positions (so that what it reads lies together),
+// head_dim / 8 threads each, four of their loads ahead of the arithmetic.
 struct ab_scratch {
     unsigned* taken;               // items handed out beyond the first of every CTA
     float* neg_lse;                // [heads][padded queries]
@@ -51,6 +51,7 @@ struct ab_scratch {
     int64_t padded;
     int q_log, k_log;              // heads_log for queries, for keys
     int q_blocks, k_blocks;
+    int block;
 };
 
 // Dot product of eight f16 in f32.  (The fma takes f16 factors; converted first, 2048 positions of 256 heads took 92 us, not 86.)
@@ -76,7 +77,7 @@ __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_
     const bool keys = blockIdx.x >= (unsigned)q_wide * w.q_blocks;
     const int at = keys ? blockIdx.x - q_wide * w.q_blocks : blockIdx.x, wide = keys ? k_wide : q_wide, log = keys ? w.k_log : w.q_log;
     const int block = at / wide, head0 = (at % wide) << log, heads = keys ? kv_heads : a.heads;
-    const int64_t row0 = (int64_t)block * (256 >> log), rows = keys ? a.kv_len : a.q_len;
+    const int64_t row0 = (int64_t)block * (w.block >> log), rows = keys ? a.kv_len : a.q_len;
     const __half* from = base + (keys ? a.v_off : a.do_off) + lane * 8;
     const __half* from_o = base + a.o_off + lane * 8;
     const int64_t stride = keys ? a.v_row : a.do_row, head_stride = keys ? a.v_head : a.do_head;
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_
     const int head = head0 + (group & ((1 << log) - 1));
     float most = 0.f, most_d = 0.f;
 #pragma unroll 1
-    for (int i0 = 0; i0 < 256; i0 += BATCH * GROUPS) {
+    for (int i0 = 0; i0 < w.block; i0 += BATCH * GROUPS) {
         uint4 g[BATCH], o[BATCH];
         float lse[BATCH];
 #pragma unroll
@@ -92,7 +93,7 @@ __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_
             const int64_t row = row0 + ((i0 + i * GROUPS + group) >> log);
             g[i] = o[i] = make_uint4(0, 0, 0, 0);
             lse[i] = -INFINITY;
-            if (row < rows && head < heads) {
+            if (row < rows && head < heads && i0 + i * GROUPS + group < w.block) {
                 g[i] = *reinterpret_cast<const uint4*>(from + row * stride + head * head_stride);
                 if (!keys) {
                     o[i] = *reinterpret_cast<const uint4*>(from_o + row * a.o_row + head * a.o_head);
@@ -112,7 +113,7 @@ __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_
             g2 = g2 <= 3.0e38f ? g2 : 0.f;                              // (a row with an infinity has no say in the shift)
             most = fmaxf(most, g2);
             if (fabsf(d) <= 3.0e38f) most_d = fmaxf(most_d, fabsf(d));
-            if (!keys && lane == 0 && row < w.padded && head < heads) {
+            if (!keys && lane == 0 && row < w.padded && head < heads && i0 + i * GROUPS + group < w.block) {
                 const int64_t to = (int64_t)head * w.padded + row;
                 // (no probability: rows past the end, rows that see nothing)
                 w.neg_lse[to] = lse[i] == -INFINITY ? -INFINITY : fmaf(-lse[i], AB_LOG2E, AB_SHIFT);
@@ -153,7 +154,7 @@ struct ab_shape {
     static constexpr int OWN = AB_M * HD * 2;               // bytes of X, of Y
     static constexpr int STEP = AB_N * HD * 2;              // bytes of X', of Y'
     static constexpr int STAGES = HD == 64 ? 8 : 4;         // 128 KB of the stream on its way
-    static constexpr size_t SMEM = 2 * OWN + STAGES * (2 * STEP + 3 * AB_N * 4) + 1024 + 512;
+    static constexpr size_t SMEM = 2 * OWN + STAGES * (2 * STEP + 3 * AB_N * 4) + 8 * 2048 + 1024 + 512;
     // columns of TMEM: two accumulators (for queries X and Y as f16 pairs in place of the second), then the slots: S and T
     static constexpr int ACC1 = HD, X = HD, Y = HD + HD / 2, SLOT = 2 * HD;
     static constexpr int SLOTS = (512 - SLOT) / (2 * AB_N);
@@ -258,7 +259,8 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     uint8_t* sY = sX + Z::OWN;
     uint8_t* ring = sY + Z::OWN;                            // per stage X', then Y'
     float* sRow = reinterpret_cast<float*>(ring + Z::STAGES * 2 * Z::STEP);     // keys: per stage 64 x (14 - lse / ln 2), 64 x D, 64 x |dO| where steps come twice
-    uint64_t* full = reinterpret_cast<uint64_t*>(sRow + Z::STAGES * 3 * AB_N);
+    uint8_t* sOut = reinterpret_cast<uint8_t*>(sRow + Z::STAGES * 3 * AB_N);    // 2 KB a warp of the softmax
+    uint64_t* full = reinterpret_cast<uint64_t*>(sOut + 8 * 2048);
     uint64_t *empty = full + Z::STAGES, *own_full = empty + Z::STAGES, *own_free = own_full + 1, *a_ready = own_free + 1;
     uint64_t *acc_free = a_ready + 1, *done = acc_free + 1, *next_full = done + 1, *next_free = next_full + 2;
     uint64_t *s_full = next_free + 2, *t_full = s_full + Z::SLOTS, *p_full = t_full + Z::SLOTS;     // p_full: per slot and half of its columns
@@ -704,13 +706,15 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             // are read, so that its first scores are made meanwhile.
             if (!KEYS && index >= 0 && then.n > 0 && !own(c + (it.n > 0))) return false;
             // results: keys: the first warpgroup dK, the second dV; queries: half of the columns of dQ each
-            const bool store = row < (KEYS ? a.dk_row0 + a.dk_rows : a.dq_row0 + a.dq_rows) && *abort_flag == 0;
+            const int row_end = KEYS ? a.dk_row0 + a.dk_rows : a.dq_row0 + a.dq_rows, warp_row = it.row0 + (warp & 3) * 32;
+            const bool store = *abort_flag == 0;
             const float back = 0x1p-14f;
             const bool of_v = KEYS && group == 1;
             const int want = KEYS ? (of_v ? a.want & KTB_ATTN_DV : a.want & KTB_ATTN_DK) : a.want & KTB_ATTN_DQ;
-            const int64_t off = !KEYS ? a.dq_off + (int64_t)row * a.dq_row + (int64_t)it.head * a.dq_head
-                              : of_v  ? a.dv_off + (int64_t)row * a.dv_row + (int64_t)it.head * a.dv_head
-                                      : a.dk_off + (int64_t)row * a.dk_row + (int64_t)it.head * a.dk_head;
+            const int64_t row_stride = !KEYS ? a.dq_row : of_v ? a.dv_row : a.dk_row;
+            const int64_t off = (int64_t)warp_row * row_stride + (!KEYS ? a.dq_off + (int64_t)it.head * a.dq_head
+                                                                   : of_v ? a.dv_off + (int64_t)it.head * a.dv_head
+                                                                          : a.dk_off + (int64_t)it.head * a.dk_head);
             float* sum = nullptr;                               // a part's sums stay f32
             if (PARTS && (KEYS ? work.key_parts : work.query_parts) > 1) {
                 const int row_here = row - (KEYS ? a.dk_row0 : a.dq_row0), head_here = it.head - (KEYS ? a.dk_head0 : a.dq_head0);
@@ -737,21 +741,20 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
                     for (int j = 0; j < 32; ++j) v[j] = 0;
                 }
-                if (PARTS && store && want && sum) {
+                if (PARTS && sum) {
+                    if (!store || !want || row >= row_end) continue;
 #pragma unroll
                     for (int j = 0; j < 32; j += 4)
                         *reinterpret_cast<float4*>(sum + x + j) = make_float4(__uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor,
                                                                              __uint_as_float(v[j + 2]) * factor, __uint_as_float(v[j + 3]) * factor);
-                } else if (store && want) {
+                } else if (want) {                              // (the same for the whole warp)
+                    uint32_t o[16];
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8) {
-                        uint4 o;
-                        __half2* h = reinterpret_cast<__half2*>(&o);
-#pragma unroll
-                        for (int e = 0; e < 4; ++e)
-                            h[e] = __floats2half2_rn(__uint_as_float(v[j + 2 * e]) * factor, __uint_as_float(v[j + 2 * e + 1]) * factor);
-                        *reinterpret_cast<uint4*>(dst + x + j) = o;
+                    for (int j = 0; j < 16; ++j) {
+                        const __half2 h = __floats2half2_rn(__uint_as_float(v[2 * j]) * factor, __uint_as_float(v[2 * j + 1]) * factor);
+                        o[j] = *reinterpret_cast<const uint32_t*>(&h);
                     }
+                    tc_store_rows(sOut + (warp - 4) * 2048, o, dst + x, row_stride, store ? row_end - warp_row : 0);
                 }
             }
             return true;
@@ -812,13 +815,16 @@ static int64_t ab_padded(const ktb_attn_bwd_args& a) { return ((int64_t)a.q_len 
 
 // Neighbouring heads that a block of the rows kernel takes (a power of two, eight at most), and the rows of it.
 static int ab_heads_log(int heads) { return heads >= 8 ? 3 : heads >= 4 ? 2 : heads >= 2 ? 1 : 0; }
-static int64_t ab_row_blocks(int64_t rows, int heads) { return (rows + (256 >> ab_heads_log(heads)) - 1) / (256 >> ab_heads_log(heads)); }
+static int64_t ab_row_blocks(int64_t rows, int heads, int block) { return (rows + (block >> ab_heads_log(heads)) - 1) / (block >> ab_heads_log(heads)); }
+// Rows of heads to a block: few, where blocks of many would leave SMs idle (197 positions of 12 heads with their gradients 14.4 us,
+// with 64 rows to a block 12.6; 1000 queries over 2777 keys of 32 / 8 heads 114.7, 116.0).
+static int ab_block(const ktb_attn_bwd_args& a) { return (int64_t)a.q_len * a.heads + (int64_t)a.kv_len * (a.heads / a.kv_group) <= 16384 ? 64 : 256; }
 
 static int64_t ab_up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 // A counter; per query and head three floats; per block of queries and head two, per block of keys and key head one ...
 static int64_t ab_rows_bytes(const ktb_attn_bwd_args& a) {
     const int kv_heads = a.heads / a.kv_group;
-    return ab_up(256 + 4 * (int64_t)a.heads * (3 * ab_padded(a) + 2 * ab_row_blocks(ab_padded(a), a.heads)) + 4 * kv_heads * ab_row_blocks(a.kv_len, kv_heads));
+    return ab_up(256 + 4 * (int64_t)a.heads * (3 * ab_padded(a) + 2 * ab_row_blocks(ab_padded(a), a.heads, ab_block(a))) + 4 * kv_heads * ab_row_blocks(a.kv_len, kv_heads, ab_block(a)));
 }
 // ... and, of walks that are cut, the parts' sums.
 static int64_t ab_part_bytes(const ktb_attn_bwd_args& a, bool keys) {
@@ -841,8 +847,9 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     w.padded = ab_padded(a);
     w.q_log = ab_heads_log(a.heads);
     w.k_log = ab_heads_log(kv_heads);
-    w.q_blocks = (int)ab_row_blocks(w.padded, a.heads);
-    w.k_blocks = (int)ab_row_blocks(a.kv_len, kv_heads);
+    w.block = ab_block(a);
+    w.q_blocks = (int)ab_row_blocks(w.padded, a.heads, w.block);
+    w.k_blocks = (int)ab_row_blocks(a.kv_len, kv_heads, w.block);
     const int64_t row_blocks = (int64_t)w.q_blocks * ((a.heads + (1 << w.q_log) - 1) >> w.q_log) + (int64_t)w.k_blocks * ((kv_heads + (1 << w.k_log) - 1) >> w.k_log);
     if (row_blocks > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many rows");
     w.taken = reinterpret_cast<unsigned*>(a.dev_scratch);

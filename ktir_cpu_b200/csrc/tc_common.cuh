@@ -104,6 +104,22 @@ static __device__ __forceinline__ void tc_tma_store_2d(const CUtensorMap* map, c
                  ::"l"(map), "r"(tc_smem_u32(smem_src)), "r"(x), "r"(y)
                  : "memory");
 }
+// 32 rows x 32 columns of f16, a row of them in a lane's registers, to `to` (row 0 of the warp) through 2 KB of shared memory that
+// is the warp's own, so that an instruction writes 8 rows' 64 bytes instead of 32 rows' 16; rows from `rows` on are left out.
+static __device__ __forceinline__ void tc_store_rows(uint8_t* stage, const uint32_t (&h)[16], __half* to, int64_t row_stride, int rows) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+        *reinterpret_cast<uint4*>(stage + lane * 64 + ((u ^ ((lane >> 1) & 3)) << 4)) = make_uint4(h[4 * u], h[4 * u + 1], h[4 * u + 2], h[4 * u + 3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = i * 8 + (lane >> 2), u = lane & 3;
+        if (row < rows)
+            *reinterpret_cast<uint4*>(to + row * row_stride + u * 8) = *reinterpret_cast<const uint4*>(stage + row * 64 + ((u ^ ((row >> 1) & 3)) << 4));
+    }
+    __syncwarp();
+}
 static __device__ __forceinline__ void tc_bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // At most N of this thread's bulk groups may still be READING their shared-memory source.
 template <int N>
