@@ -500,6 +500,8 @@ typedef struct {
        scratch must be ordered. */
     int32_t parts;
     int32_t twice;              /* 1: P is multiplied as f16 and once more as what that left out (half the rate; for few rows) */
+    int32_t single;             /* 1: a CTA takes one pair of 128-row tiles at a time instead of a late and an early one */
+    int32_t reserved;
     void* dev_scratch;
     int64_t scratch_bytes;
 } ktb_attn_dense_args;

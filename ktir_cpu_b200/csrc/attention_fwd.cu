@@ -114,8 +114,8 @@ enum { B_QFULL = 0, B_QFREE = 2, B_KVFULL = 4, B_KVEMPTY = B_KVFULL + AT_MAX_STA
 //
 // DENSE: keys and values are rows of one tensor instead of pages, a.num_tiles groups of BN of them of which d.kv_len exist;
 // rows that see nothing give 0, and the log-sum-exp of every row is kept (256 heads of 2048 positions, 128 wide, causal: 291 us,
-// 944 TFLOP/s, 344 once the power cap holds; 1531 queries of 32 heads over 4603 keys 118 us: 96 items on 148 SMs, and parts
-// cost what they spread, 117 in three).  PARTS: the keys of an item are cut into d.parts
+// 944 TFLOP/s, 344 once the power cap holds; 1531 queries of 32 heads over 4603 keys 107 us: 192 pairs of tiles on 148
+// SMs).  d.single: an item is one pair of tiles.  PARTS: the keys of an item are cut into d.parts
 // ranges, an item of its own each, where whole items would leave most SMs idle; ktb_attention_join_fwd_kernel joins them.  With
 // d.twice every page comes twice: P as f16 times V, then what that rounding left out (up to 2^-12 of P) times V.  A result is
 // the sum of a few large P, so that over many rows their roundings are as large as the result's own, 2^-12, but over a few rows
@@ -124,6 +124,7 @@ struct at_dense {
     float* lse;                 // null: not wanted
     int64_t row, head;
     int kv_len, parts, twice;
+    int single;                 // items are single tile pairs, late ones first, dealt out to and fro
     float4* part_o;             // [part][head][query / 32][column / 4][query % 32]: a warp's rows side by side
     float* part_lse;            // [part][head][query, up to a multiple of 32]
     int rows32;                 // queries / 32, rounded up
@@ -164,7 +165,9 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     // tile i can see (kv position p is visible to row R iff p <= R + delta), 0 for a tile that does
     // not exist; nmax = pages to stream.  An item whose two halves coincide has an empty second half.
     auto sub_item = [&](int s, int& head, int& q0, int (&n_of)[2], int& nmax, bool& again, int& page0, int& part) -> bool {
-        const long long item64 = (long long)blockIdx.x + (long long)(s >> 1) * gridDim.x;
+        const bool single = DENSE && d.single;
+        const int round = single ? s : s >> 1;
+        const long long item64 = (long long)(single && (round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x) + (long long)round * gridDim.x;
         if (item64 >= n_items) return false;
         int item = (int)item64;
         part = page0 = 0;
@@ -172,11 +175,11 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             part = item % d.parts;
             item /= d.parts;
         }
-        head = item / half_pairs;
+        head = single ? item % a.heads : item / half_pairs;
         const int r = item % half_pairs;
-        const int qp = (s & 1) ? r : q_pairs - 1 - r;
+        const int qp = single ? q_pairs - 1 - item / a.heads : (s & 1) ? r : q_pairs - 1 - r;
         q0 = qp * 2 * AT_BM;
-        const bool empty = (s & 1) && r == q_pairs - 1 - r;
+        const bool empty = !single && (s & 1) && r == q_pairs - 1 - r;
         again = empty;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
@@ -655,7 +658,7 @@ static int launch_attn(ktb_ctx* ctx, const ktb_attn_args& a, const CUtensorMap& 
     }
     const int q_pairs = (a.seq_q + 2 * AT_BM - 1) / (2 * AT_BM);
     // an item = the tile pairs (q_pairs - 1 - r, r) of one head; one persistent CTA per SM walks them
-    const long long items = (long long)((q_pairs + 1) / 2) * a.heads * (PARTS ? d.parts : 1);
+    const long long items = (long long)(DENSE && d.single ? q_pairs : (q_pairs + 1) / 2) * a.heads * (PARTS ? d.parts : 1);
     if (items > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_fwd", "too many query tiles");
     const long long blocks = ((long long)d.rows32 * 32 * a.heads * (HD / 8) + 255) / 256;        // (of joining parts)
     if (PARTS && blocks > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_dense", "too many rows in parts");
@@ -730,7 +733,8 @@ extern "C" int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_arg
     const int64_t all = b.q_off | b.k_off | b.v_off | b.o_off | b.q_row | b.q_head | b.k_row | b.k_head | b.v_row | b.v_head | b.o_row | b.o_head;
     if ((all & 7) || (reinterpret_cast<uintptr_t>(b.arena) & 15))
         return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "strides and offsets must be multiples of 8 elements");
-    if (b.parts < 0 || b.parts > 64 || b.twice < 0 || b.twice > 1) return ktb_fail(ctx, KTB_E_ARG, me, "parts of the keys, twice");
+    if (b.parts < 0 || b.parts > 64 || b.twice < 0 || b.twice > 1 || b.single < 0 || b.single > 1)
+        return ktb_fail(ctx, KTB_E_ARG, me, "parts of the keys, twice, single");
     if (b.parts > 1 && (!b.dev_scratch || (reinterpret_cast<uintptr_t>(b.dev_scratch) & 15) ||
                         b.scratch_bytes < (int64_t)b.parts * (((int64_t)b.q_len + 31) / 32 * 32) * b.heads * (b.head_dim + 1) * 4))
         return ktb_fail(ctx, KTB_E_ARG, me, "scratch too small for the parts");
@@ -769,6 +773,7 @@ extern "C" int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_arg
     d.kv_len = b.kv_len;
     d.parts = b.parts > 1 ? b.parts : 1;
     d.twice = b.twice;
+    d.single = b.single;
     d.rows32 = (b.q_len + 31) / 32;
     d.part_o = reinterpret_cast<float4*>(b.dev_scratch);
     d.part_lse = reinterpret_cast<float*>(b.dev_scratch) + (int64_t)d.parts * d.rows32 * 32 * b.heads * b.head_dim;

@@ -409,16 +409,47 @@ def _disjoint(arena: ArenaMap, reads, writes) -> bool:
     return not any(_runs_overlap(*a, *b) for i, a in enumerate(writes) for b in list(writes[i + 1:]) + spans)
 
 
-def dense_parts(q_len: int, kv_len: int, heads: int) -> int:
-    """Parts that the keys of the forward pass are cut into.
+def dense_plan(q_len: int, kv_len: int, heads: int, head_dim: int, causal: int, delta: int, twice: bool) -> Tuple[int, int]:
+    """How the forward pass deals out its work: (whether a CTA takes single pairs of 128-row tiles, parts that the keys are cut into).
 
-    A CTA takes two pairs of 128-row tiles of a head, the last ones with the first ones.  Where these leave half of the SMs or
-    more without work, the keys are cut until they do not: one query of 32 heads over 8192 keys took 88 us, in four parts 33; 1024
-    queries of 32 heads over 16384 keys 445 us, in two 252; one query of 8 heads over 65536 keys 644 us, in sixteen 56.  A part and
-    joining it cost four microseconds, 512 keys five: smaller parts gain nothing (64 queries of 8 heads over 1024 keys 15.4 us, in
-    two 16.5; over 2048 keys 24.8, in four 16.6)."""
-    items = -(-(-(-q_len // 256)) // 2) * heads
-    return max(1, min(16, SMS // items, kv_len // 512)) if kv_len >= 1536 else 1
+    Either an item is a late pair of tiles of a head and an early one, so that all items cost the same and neighbours read the same
+    keys, or a single pair, late ones first and dealt out to and fro, which is half as coarse.  Keys cut into parts make more items
+    of few.  The way that an estimate in microseconds of the busiest CTA finds best is taken: 1.73 a page of 128 keys (1.55, 64
+    wide; 1.27 for one tile alone), 3 to start and end a pair, 2 more and a share of joining for a part.  It is within 6 % of what 21
+    shapes took as pairs, single or not, within 15 in parts.  Measured, items of two pairs / single ones / the best parts: 842
+    positions of 8 heads 31.0 / 18.6 / 16.8; 1531 queries of 32 heads over 4603 keys 117.0 / 107.4 / 113.9; 1024 over 16384 keys 442.6
+    / 226.6 / 249.8; one query over 8192 keys 88.3 / 88.3 / 32.9; 2048 positions of 128 heads 148.9 / 134.9, of 256 heads, whose keys
+    L2 does not hold, 254.8 / 268.1."""
+    q0 = np.arange(0, q_len, 256, dtype=np.int64)
+    two = q0 + 128 < q_len
+    seen = np.clip(np.where(two, q0 + 256, q0 + 128) + delta, 0, kv_len) if causal else np.full(len(q0), kv_len)
+    pages, page = -(-seen // 128), np.where(two, 1.73 if head_dim == 128 else 1.55, 1.27) * (2 if twice else 1)
+    n, best = len(pages), (0, 1)
+    if n * heads > 16 * SMS:                     # (many items: no order of them is far from the others)
+        return best
+
+    def busiest(single, parts):
+        own = 3.0 + (2.0 if parts > 1 else 0.0) + -(-pages // parts) * page
+        if single:
+            cost = np.repeat(own[::-1], heads * parts)
+        else:
+            pairs = own[::-1][:(n + 1) // 2].copy()
+            pairs[:n // 2] += own[:n // 2]
+            cost = np.tile(np.repeat(pairs, parts), heads)
+        rounds = -(-len(cost) // SMS)
+        cost = np.pad(cost, (0, rounds * SMS - len(cost))).reshape(rounds, SMS)
+        if single:
+            cost[1::2] = cost[1::2, ::-1]
+        return cost.sum(0).max() + (5.0 if parts == 1 else 8.0 + 8.0 * parts * q_len * heads * head_dim / 8e6)
+    least = busiest(0, 1)
+    for parts in (1, 2, 3, 4, 5, 6, 8, 12, 16):
+        if parts > 1 and (n * heads * parts > 4 * SMS or parts * 192 > kv_len):
+            break
+        for single in (0, 1):
+            t = busiest(single, parts)
+            if t < 0.97 * least:
+                best, least = (single, parts), t
+    return best
 
 
 # (An output's error stays below 1.5 of its rounding from some 20 rows on, a gradient's, three sums of which each may be off, from 200.)
@@ -493,8 +524,8 @@ class AttentionDenseStatement(Statement):
         self._bytes = 2 * hd * (2 * nr * nh + 2 * k.rows * (nh // grp)) + (4 * nr * nh if self.used == 2 else 0)
         # (by the whole tensors: a rank that has some of the heads sums in the same parts; one that has some of the rows cuts
         # them at other keys, and may differ in the last bit)
-        a.parts = dense_parts(q.rows, k.rows, q.heads)
         a.twice = few_rows(q.rows, q.heads, causal, delta, FEW_ROWS_FORWARD)
+        a.single, a.parts = dense_plan(q.rows, k.rows, q.heads, hd, causal, delta, bool(a.twice))
         self.device_arrays = []
         if a.parts > 1:
             a.scratch_bytes = 4 * a.parts * (-(-nr // 32) * 32) * nh * (hd + 1)

@@ -138,7 +138,7 @@ class AttnDenseArgs(C.Structure):
     _fields_ = [("arena", C.c_void_p)] + \
         [(n, C.c_int64) for n in "q_off k_off v_off o_off lse_off q_row q_head k_row k_head v_row v_head o_row o_head lse_row lse_head".split()] + \
         [(n, C.c_int32) for n in "q_len kv_len heads kv_group head_dim causal causal_delta".split()] + [("scale", C.c_float)] + \
-        [("parts", C.c_int32), ("twice", C.c_int32), ("dev_scratch", C.c_void_p), ("scratch_bytes", C.c_int64)]
+        [("parts", C.c_int32), ("twice", C.c_int32), ("single", C.c_int32), ("reserved", C.c_int32), ("dev_scratch", C.c_void_p), ("scratch_bytes", C.c_int64)]
 
 
 ATTN_DQ, ATTN_DK, ATTN_DV = 1, 2, 4

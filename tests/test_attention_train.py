@@ -14,7 +14,7 @@ import pytest
 
 from ktir_cpu_b200 import HardwareConfig, KTIRInterpreter, kernels as K, runtime as R
 from ktir_cpu_b200.interpreter import Session
-from ktir_cpu_b200.lower_attn_train import FEW_ROWS_BACKWARD, FEW_ROWS_FORWARD, dense_parts, few_rows, grad_parts, grad_scratch_bytes
+from ktir_cpu_b200.lower_attn_train import FEW_ROWS_BACKWARD, FEW_ROWS_FORWARD, dense_plan, few_rows, grad_parts, grad_scratch_bytes
 from ktir_cpu_b200.parser import KTIRParser
 from oracle.numpy_interp import OracleInterpreter
 
@@ -272,10 +272,12 @@ def test_long_walks_are_cut_where_there_are_few(q_len, kv_len, heads, kv_heads, 
     assert grad_parts(q_len, kv_len, heads, kv_heads, int(causal), kv_len - q_len if causal else 0) == parts
 
 
-@pytest.mark.parametrize("q_len,kv_len,heads,parts", [(2048, 2048, 256, 1), (197, 197, 12, 1), (1, 1, 1, 1), (1, 511, 1, 1), (1, 1535, 4, 1), (1, 1536, 4, 3),
-                                                      (1, 8192, 4, 16), (1024, 65536, 32, 2), (1024, 65536, 37, 2), (1024, 65536, 38, 1), (4096, 4096, 2, 8)])
-def test_keys_are_cut_where_there_are_few_queries(q_len, kv_len, heads, parts):
-    assert dense_parts(q_len, kv_len, heads) == parts
+@pytest.mark.parametrize("q_len,kv_len,heads,hd,causal,plan", [
+    (2048, 2048, 256, 128, 1, (0, 1)), (197, 197, 12, 64, 0, (0, 1)), (1, 1, 1, 128, 1, (0, 1)), (842, 842, 8, 64, 0, (1, 4)), (1024, 1024, 8, 128, 1, (1, 4)),
+    (1531, 4603, 32, 128, 1, (1, 1)), (1, 8192, 32, 128, 1, (0, 4)), (1024, 65536, 37, 128, 0, (1, 1)), (8192, 8192, 512, 64, 1, (0, 1)), (100, 7, 3, 64, 1, (0, 1)),
+    (4096, 4096, 16, 128, 1, (1, 1)), (1, 65536, 4, 64, 0, (0, 16))])
+def test_few_items_are_single_or_in_parts(q_len, kv_len, heads, hd, causal, plan):
+    assert dense_plan(q_len, kv_len, heads, hd, causal, kv_len - q_len if causal else 0, False) == plan
 
 
 def test_few_rows_are_those_that_see_a_key():
@@ -328,11 +330,14 @@ def test_forward(q_len, kv_len, heads, kv_heads, hd, causal, build_lib):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("c,parts", [((2500, 1540, 2, 1, 128, True), 3), ((257, 2200, 3, 3, 64, True), 4), ((1, 16400, 1, 1, 128, True), 16),
-                                     ((300, 5000, 30, 2, 64, False), 4), ((700, 1601, 4, 4, 128, True), 3)])
-def test_forward_in_parts(c, parts, build_lib):
-    """Parts that rows see nothing of, rows that see nothing at all, a last part that fills no step."""
-    assert dense_parts(c[0], c[1], c[2]) == parts
+@pytest.mark.parametrize("plan", [(0, 1), (1, 1), (0, 3), (1, 2), (1, 7)])
+@pytest.mark.parametrize("c", [(2500, 1540, 2, 1, 128, True), (257, 2200, 3, 3, 64, True), (1, 4400, 1, 1, 128, True), (300, 2000, 30, 2, 64, False), (700, 1601, 4, 4, 128, True),
+                               (513, 70, 120, 4, 64, False), (90, 33, 5, 1, 128, True), (1100, 1100, 70, 7, 64, True)])
+def test_forward_however_it_is_dealt_out(c, plan, build_lib, monkeypatch):
+    """Parts that rows see nothing of, rows that see nothing at all, a last part that fills no step, more parts than pages, more items
+    than SMs."""
+    from ktir_cpu_b200 import lower_attn_train
+    monkeypatch.setattr(lower_attn_train, "dense_plan", lambda *a: plan)
     kw, _ = _inputs(*c[:5], seed=c[1])
     got = _run(K.attention_forward(*c), FWD, _kwargs(FWD, kw, c[0], c[2], c[4]), "attention_dense", times=3)
     _check(got, formulas(kw, None, c[5]))
@@ -652,7 +657,7 @@ def test_launchers_refuse(build_lib):
     fwd.load(K.attention_forward(64, 64, 4, 2, 64, True))
     fs, _ = fwd.session(FWD, **_kwargs(FWD, kw, 64, 4, 64))
     for field, value, code in (("head_dim", 96, -3), ("kv_group", 0, -2), ("kv_group", 3, -2), ("q_len", -1, -2), ("kv_len", 0, -3), ("scale", 0.0, -3),
-                               ("scale", -1.0, -3), ("scale", float("nan"), -3), ("v_row", 12, -3), ("o_off", 4, -3), ("parts", -1, -2), ("parts", 65, -2), ("twice", 2, -2), ("twice", -1, -2),
+                               ("scale", -1.0, -3), ("scale", float("nan"), -3), ("v_row", 12, -3), ("o_off", 4, -3), ("parts", -1, -2), ("parts", 65, -2), ("twice", 2, -2), ("twice", -1, -2), ("single", 2, -2),
                                ("parts", 2, -2)):
         refused("ktb_launch_attention_dense", fs.plan.statements[0].args, field, value, code, "attention_dense")
     fwd.close()
