@@ -12,7 +12,7 @@
 // have been issued (asked for first, the position holds them up: 8192 tokens of 72 heads, 128 wide, 52 us -> 66).  What turns
 // and what is copied is loaded by the same instructions, since lanes of one warp do either (f32, 4001 tokens of 40 heads, 96
 // wide, half of it turned: 36 us in branches of their own, 27 together).
-#include "common.cuh"
+#include "tc_common.cuh"
 
 template <typename T> static __device__ __forceinline__ float ro_up(T v);
 template <> __device__ __forceinline__ float ro_up<__half>(__half v) { return __half2float(v); }
@@ -136,8 +136,8 @@ ktb_rotary_kernel(const ktb_rotary_args a, int64_t token0, uint32_t n_threads, u
 // pairs of f16, say): a thread owns 16 bytes of a head, wherever they fall.  What they are turned with is in the same bytes
 // (adjacent pairs) or n elements on or back: two neighbouring vectors, shifted into one; a vector that holds the end of the first
 // half needs both.  Table values are kept for several heads of the token, whose own bytes are on their way together; the rest
-// of a head comes from L1.  4096 tokens of 40 heads, 128 wide, 54 turned: halves 61 us element by element, 43 so; adjacent pairs
-// 45 in 4-byte vectors, 24 so.
+// of a head comes from L1.  4096 tokens of 40 heads, 128 wide, 54 turned: halves 61 us element by element, 39 so; adjacent pairs
+// 45 in 4-byte vectors, 23 so.  Instructions bound it (f32, with half as many elements to 16 bytes, moves twice the bytes).
 // VEC elements from `shift` on in the 2 * VEC of lo and hi.
 template <typename T, typename V>
 static __device__ __forceinline__ V ro_shift(const V& lo, const V& hi, int shift) {
@@ -159,6 +159,10 @@ static __device__ __forceinline__ V ro_shift(const V& lo, const V& hi, int shift
     return y;
 }
 
+// (nothing that is read is written: later loads need not wait for earlier stores)
+template <typename V>
+static __device__ __forceinline__ V ro_ldg(const void* p) { const uint4 q = __ldg(reinterpret_cast<const uint4*>(p)); return *reinterpret_cast<const V*>(&q); }
+
 template <typename T, bool ADJ>
 __global__ void __launch_bounds__(256, 4)
 ktb_rotary_rows_kernel(const ktb_rotary_args a, int64_t token0, uint32_t n_threads, uint32_t slots, int row_vecs, int heads_total, ktb_status* st) {
@@ -177,9 +181,9 @@ ktb_rotary_rows_kernel(const ktb_rotary_args a, int64_t token0, uint32_t n_threa
     // !ADJ: the other half's elements start at `other`; `split`: those of this vector's later elements n back, in front of the head
     const bool split = !ADJ && e0 < n && e0 + VEC > n;
     const int other = e0 < n ? e0 + n : e0 - n, shift = other % VEC, end = (row_vecs - 1) * VEC;
-    float cs[PAIRS], sn[PAIRS];
+    uint64_t cs[VEC / 2], sn[VEC / 2];                   // factors of elements 2i and 2i + 1, and of their partners
 #pragma unroll
-    for (int i = 0; i < PAIRS; ++i) cs[i] = 1.f, sn[i] = 0.f;
+    for (int i = 0; i < VEC / 2; ++i) cs[i] = sn[i] = 0;
     bool asked = false;
 #pragma unroll 1
     for (int first = (int)(r % slots); first < heads_total; first += HEADS * (int)slots) {
@@ -207,13 +211,23 @@ ktb_rotary_rows_kernel(const ktb_rotary_args a, int64_t token0, uint32_t n_threa
             }
             const float* table = reinterpret_cast<const float*>(a.arena);
             const int64_t row = pos < (int64_t)1 << 40 ? pos * a.table_stride : (int64_t)1 << 61;
+            // entries of pair j0 + i, or, from the other half on, of e - n (a row past the table's end is zeros, one across it in part)
+            const int j0 = ADJ ? e0 / 2 : e0 < n ? e0 : e0 - n, wrap = ADJ || e0 >= n ? VEC : n - e0;
+            const int64_t in_cos = a.cos_end - a.cos_off - row, in_sin = a.sin_end - a.sin_off - row;
+            const float *cr = table + (in_cos > 0 ? a.cos_off + row : 0), *sr = table + (in_sin > 0 ? a.sin_off + row : 0);
+            const int nc = in_cos < n ? in_cos < 0 ? 0 : (int)in_cos : n, ns = in_sin < n ? in_sin < 0 ? 0 : (int)in_sin : n;
+            float c[PAIRS], s[PAIRS];
 #pragma unroll
             for (int i = 0; i < PAIRS; ++i) {
-                const int e = ADJ ? e0 / 2 + i : e0 + i, j = ADJ || e < n ? e : e - n;
-                if (j >= n) continue;
-                cs[i] = a.cos_off + row + j < a.cos_end ? table[a.cos_off + row + j] : 0.f;
-                sn[i] = a.sin_off + row + j < a.sin_end ? table[a.sin_off + row + j] : 0.f;
-                if (a.inverse) sn[i] = -sn[i];
+                const int j = i < wrap ? j0 + i : i - wrap;
+                c[i] = j < nc ? cr[j] : 0.f;
+                s[i] = j < ns ? sr[j] : 0.f;
+                if (a.inverse != (!ADJ && e0 + i < n)) s[i] = -s[i];         // (x' = x cos + y (-sin))
+            }
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) {
+                cs[i] = ADJ ? at_pack2(c[i], c[i]) : at_pack2(c[2 * i], c[2 * i + 1]);
+                sn[i] = ADJ ? at_pack2(-s[i], s[i]) : at_pack2(s[2 * i], s[2 * i + 1]);
             }
         }
 #pragma unroll
@@ -223,21 +237,25 @@ ktb_rotary_rows_kernel(const ktb_rotary_args a, int64_t token0, uint32_t n_threa
             if (!ADJ && turn) {
                 // (other lanes have loaded these; a second vector past the head holds nothing that is wanted)
                 const int at = other - shift;
-                const V lo = *reinterpret_cast<const V*>(src[k] + at);
-                y = shift ? ro_shift<T>(lo, at < end ? *reinterpret_cast<const V*>(src[k] + at + VEC) : lo, shift) : lo;
+                const V lo = ro_ldg<V>(src[k] + at);
+                y = shift ? ro_shift<T>(lo, at < end ? ro_ldg<V>(src[k] + at + VEC) : lo, shift) : lo;
                 if (split) {
-                    const V head = *reinterpret_cast<const V*>(src[k]), back = ro_shift<T>(head, head, VEC - (n - e0));
+                    const V head = ro_ldg<V>(src[k]), back = ro_shift<T>(head, head, VEC - (n - e0));
 #pragma unroll
                     for (int i = 0; i < VEC; ++i)
                         if (e0 + i >= n) y.e[i] = back.e[i];
                 }
             }
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const int e = e0 + i;
-                const bool upper = ADJ ? i & 1 : e >= n;
-                const float mc = __fmul_rn(ro_up<T>(x[k].e[i]), cs[ADJ ? i / 2 : i]), os = __fmul_rn(ro_up<T>(ADJ ? x[k].e[i ^ 1] : y.e[i]), sn[ADJ ? i / 2 : i]);
-                if (e < 2 * n) v.e[i] = ro_down<T>(upper ? __fadd_rn(mc, os) : __fsub_rn(mc, os));      // (behind the pairs: copied)
+            for (int i = 0; i < VEC / 2; ++i) {
+                // (two products at a time; their sums one by one, since a pair of them becomes an fma, which does not round the product)
+                const uint64_t own = at_pack2(ro_up<T>(x[k].e[2 * i]), ro_up<T>(x[k].e[2 * i + 1]));
+                const uint64_t partner = ADJ ? at_pack2(ro_up<T>(x[k].e[2 * i + 1]), ro_up<T>(x[k].e[2 * i])) : at_pack2(ro_up<T>(y.e[2 * i]), ro_up<T>(y.e[2 * i + 1]));
+                float mc0, mc1, os0, os1;
+                at_unpack2(at_mul2(own, cs[i]), mc0, mc1);
+                at_unpack2(at_mul2(partner, sn[i]), os0, os1);
+                if (e0 + 2 * i < 2 * n)                      // (behind the pairs: copied)
+                    v.e[2 * i] = ro_down<T>(__fadd_rn(mc0, os0)), v.e[2 * i + 1] = ro_down<T>(__fadd_rn(mc1, os1));
             }
             *reinterpret_cast<V*>(dst[k]) = v;
         }
