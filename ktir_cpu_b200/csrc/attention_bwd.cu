@@ -22,8 +22,8 @@
 // whose sums run over rows).  Sums, D and the statistics are f32.  Where few rows see a key these roundings are multiplied too
 // (MODE 2).
 //
-// 256 heads of 2048 positions, 128 wide, causal: 1.06 ms, 650 TFLOP/s of the five products (900 of the seven), 1.25 ms once
-// the power cap holds; 16 / 4 heads of 8192 positions 0.76 ms, 903 (not capped).
+// 256 heads of 2048 positions, 128 wide, causal: 1.04 ms, 660 TFLOP/s of the five products (925 of the seven), 1.20 ms once
+// the power cap holds; 16 / 4 heads of 8192 positions 0.76 ms, 906, capped 0.87.
 #include <type_traits>
 
 #include "tc_common.cuh"
@@ -39,7 +39,7 @@ static __device__ __forceinline__ void ab_wait_for_rows() { asm volatile("gridde
 
 // ---- what the rows bring: 14 - lse / ln 2, D, |dO| per row, and the largest norms of a block of rows ---------------
 // HBM bounds it (O, dO and V once; 256 heads of 2048 positions, 128 wide: 86 us, 4.7 TB/s).  A block takes
-// w.block rows of heads, 2^heads_log neighbouring heads of w.block >> heads_log positions (so that what it reads lies together),
+// BLOCK rows of heads, 2^heads_log neighbouring heads of BLOCK >> heads_log positions (so that what it reads lies together),
 // head_dim / 8 threads each, four of their loads ahead of the arithmetic.
 struct ab_scratch {
     unsigned* taken;               // items handed out beyond the first of every CTA
@@ -65,7 +65,7 @@ static __device__ __forceinline__ float ab_dot8(uint4 a, uint4 b) {
     return s;
 }
 
-template <int HD>
+template <int HD, int BLOCK>
 __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_bwd_args a, const ab_scratch w) {
     constexpr int LANES = HD / 8, GROUPS = 256 / LANES, BATCH = 4;
     ab_follow();
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_
     const bool keys = blockIdx.x >= (unsigned)q_wide * w.q_blocks;
     const int at = keys ? blockIdx.x - q_wide * w.q_blocks : blockIdx.x, wide = keys ? k_wide : q_wide, log = keys ? w.k_log : w.q_log;
     const int block = at / wide, head0 = (at % wide) << log, heads = keys ? kv_heads : a.heads;
-    const int64_t row0 = (int64_t)block * (w.block >> log), rows = keys ? a.kv_len : a.q_len;
+    const int64_t row0 = (int64_t)block * (BLOCK >> log), rows = keys ? a.kv_len : a.q_len;
     const __half* from = base + (keys ? a.v_off : a.do_off) + lane * 8;
     const __half* from_o = base + a.o_off + lane * 8;
     const int64_t stride = keys ? a.v_row : a.do_row, head_stride = keys ? a.v_head : a.do_head;
@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_
     const int head = head0 + (group & ((1 << log) - 1));
     float most = 0.f, most_d = 0.f;
 #pragma unroll 1
-    for (int i0 = 0; i0 < w.block; i0 += BATCH * GROUPS) {
+    for (int i0 = 0; i0 < BLOCK; i0 += BATCH * GROUPS) {
         uint4 g[BATCH], o[BATCH];
         float lse[BATCH];
 #pragma unroll
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_
             const int64_t row = row0 + ((i0 + i * GROUPS + group) >> log);
             g[i] = o[i] = make_uint4(0, 0, 0, 0);
             lse[i] = -INFINITY;
-            if (row < rows && head < heads && i0 + i * GROUPS + group < w.block) {
+            if (row < rows && head < heads && i0 + i * GROUPS + group < BLOCK) {
                 g[i] = *reinterpret_cast<const uint4*>(from + row * stride + head * head_stride);
                 if (!keys) {
                     o[i] = *reinterpret_cast<const uint4*>(from_o + row * a.o_row + head * a.o_head);
@@ -113,7 +113,7 @@ __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_
             g2 = g2 <= 3.0e38f ? g2 : 0.f;                              // (a row with an infinity has no say in the shift)
             most = fmaxf(most, g2);
             if (fabsf(d) <= 3.0e38f) most_d = fmaxf(most_d, fabsf(d));
-            if (!keys && lane == 0 && row < w.padded && head < heads && i0 + i * GROUPS + group < w.block) {
+            if (!keys && lane == 0 && row < w.padded && head < heads && i0 + i * GROUPS + group < BLOCK) {
                 const int64_t to = (int64_t)head * w.padded + row;
                 // (no probability: rows past the end, rows that see nothing)
                 w.neg_lse[to] = lse[i] == -INFINITY ? -INFINITY : fmaf(-lse[i], AB_LOG2E, AB_SHIFT);
@@ -868,7 +868,7 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     const int64_t nq = join_q ? (int64_t)a.dq_rows * a.dq_heads : 0, nk = join_k ? (int64_t)a.dk_rows * a.dk_heads : 0;
     const int64_t blocks = ((nq > nk ? nq : nk) * (HD / 8) + 255) / 256;
     if (blocks > 0x7fffffff) return ktb_fail(ctx, KTB_E_UNSUPPORTED, "attention_bwd", "too many rows in parts");
-    ktb_attention_rows_kernel<HD><<<(unsigned)row_blocks, 256, 0, ctx->stream>>>(a, w);
+    (w.block == 64 ? ktb_attention_rows_kernel<HD, 64> : ktb_attention_rows_kernel<HD, 256>)<<<(unsigned)row_blocks, 256, 0, ctx->stream>>>(a, w);
     KTB_CHECK_LAUNCH(ctx, "ktb_attention_rows_kernel");
     static bool attr_set[KTB_MAX_DEVICES] = {};     // the attribute is per device
     if (!attr_set[ctx->device & (KTB_MAX_DEVICES - 1)]) {
