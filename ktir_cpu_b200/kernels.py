@@ -1369,7 +1369,7 @@ def rotary(tokens: int = 64, heads: int = 8, kv_heads: int = 2, head_dim: int = 
     assert layout in ("half", "interleaved") and dtype in ("f16", "f32") and 0 < rot <= head_dim and rot % 2 == 0
     n, T = rot // 2, tokens
     if block is None:
-        most = max(1, 16384 // (max(heads, kv_heads) * n))
+        most = max(1, 16384 // (max(heads, kv_heads) * max(n, (head_dim - rot) // 4)))     # (the rest is one tile, a pair several)
         block = max(b for b in range(1, min(most, T) + 1) if T % b == 0)
     assert T % block == 0
     bt = block

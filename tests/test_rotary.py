@@ -121,6 +121,14 @@ def test_tables_are_those_of_64_bits():
     np.testing.assert_allclose(slow[1][:, 3], np.sin(np.arange(64) / 4.0 * 10000.0 ** -0.75), rtol=0, atol=2.0 ** -24)
 
 
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim,part,layout", [
+    (944, 8, 0, 104, 4, "half"), (266, 9, 2, 256, 8, "half"), (816, 10, 0, 64, 4, "half"), (442, 11, 1, 256, 8, "interleaved"), (4096, 64, 8, 256, 6, "half")])
+def test_small_parts_of_long_heads_fit_the_scratchpad(tokens, heads, kv_heads, dim, part, layout):
+    """A core's tokens are as many as fit with what is behind the pairs, too."""
+    src, kw = _case(tokens, heads, kv_heads, dim, part, layout, False, "f32", None)
+    assert [s.kind for s in _session(src, kw).plan.statements] == ["rotary"]
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("case", CASES)
 def test_kernel_has_the_oracles_bits(case, build_lib):
