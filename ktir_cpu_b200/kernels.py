@@ -1364,7 +1364,8 @@ def rotary(tokens: int = 64, heads: int = 8, kv_heads: int = 2, head_dim: int = 
     (a, b) -> (a cos - b sin, b cos + a sin), in f32, rounded once; the elements behind are copied.  ``layout`` says which
     elements are pair j: "half" j and j + rotary_dim / 2, "interleaved" 2j and 2j + 1.  ``inverse`` turns back: the
     gradient of the rotation.  ``kv_heads = 0`` leaves the keys out.  The tables hold whatever frequencies a model uses
-    (``rotary_tables``).  A core owns ``block`` tokens, a divisor of ``tokens``."""
+    (``rotary_tables``).  A core owns ``block`` tokens, a divisor of ``tokens``; one token's heads have to fit its scratchpad
+    (``heads * rotary_dim`` up to 65536)."""
     rot = head_dim if rotary_dim is None else rotary_dim
     assert layout in ("half", "interleaved") and dtype in ("f16", "f32") and 0 < rot <= head_dim and rot % 2 == 0
     n, T = rot // 2, tokens
