@@ -470,7 +470,10 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const int group = (warp - 4) >> 2;                      // two warpgroups take the steps in turn
         const int r = (warp & 3) * 32 + lane;                   // row of the tile == TMEM lane
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const float sl = a.scale * AB_LOG2E;
+        // A hidden column's score is the infinity that the scale turns into -infinity, so that exp2 makes it a zero.  (A scale of
+        // zero, times that, would be NaN: 2^-120 in its place moves no exponent, since f16 operands' scores are below 2^40.)
+        const float sl = a.scale == 0.f ? 0x1p-120f : a.scale * AB_LOG2E;
+        const uint32_t hidden = sl < 0.f ? 0x7f800000u : 0xff800000u;
         const uint64_t sl2 = at_pack2(sl, sl);
         ab_wait_for_rows();
         int g0 = 0, c = 0;
@@ -610,7 +613,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         if (masked) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                if (32 * h + j < lo || 32 * h + j >= hi) s[j] = 0xff800000u;        // exp2 makes it a zero
+                                if (32 * h + j < lo || 32 * h + j >= hi) s[j] = hidden;
                         }
                         float p[32];
 #pragma unroll
@@ -663,7 +666,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         if (masked) {
 #pragma unroll
                             for (int j = 0; j < 32; ++j)
-                                if (32 * h + j < lo || 32 * h + j >= hi) s[j] = 0xff800000u;
+                                if (32 * h + j < lo || 32 * h + j >= hi) s[j] = hidden;
                         }
                         if (TWICE && a.kv_len <= AB_N) settle(of_keys, t, rows, h, row_d, near);
 #pragma unroll

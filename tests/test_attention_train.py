@@ -678,3 +678,18 @@ def test_other_head_sizes_run_step_by_step(case, build_lib):
         assert {s.kind for sess in gpu._sessions.values() for s in sess.plan.statements} == {"generic"}
         gpu.close()
         _check(got, formulas(kw, None, causal) if fn == FWD else formulas(kw, do, causal, o, lse))
+
+
+# ---- ranges of the inputs ------------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [-0.25, -0.5, 0.0, -0.0])
+@pytest.mark.parametrize("c", [(150, 150, 2, 2, 128, True), (100, 197, 6, 2, 64, False), (70, 90, 3, 1, 128, False), (300, 111, 8, 4, 64, True), (9, 30, 2, 1, 64, True)])
+def test_gradients_with_a_score_scale_of_zero_or_below(c, scale, build_lib):
+    """A hidden key has no probability whatever sign the scale has.  (scale Q) K^T = |scale| Q (-K)^T, so that the formulas with -K
+    give dQ, dV and -dK.)"""
+    kw, do = _inputs(*c[:5], seed=c[1])
+    mirrored = dict(kw, key_ptr=-kw["key_ptr"])
+    o, lse = _forward_results(mirrored, c[5], scale=abs(scale))
+    got = _run(K.attention_backward(*c), BWD, _kwargs(BWD, kw, c[0], c[2], c[4], do, o, lse, np.float32(scale)), "attention_bwd")
+    got["key_grad_ptr"] = -got["key_grad_ptr"]
+    _check(got, formulas(mirrored, do, c[5], o, lse, scale=abs(scale)))
