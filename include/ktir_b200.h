@@ -487,7 +487,7 @@ int ktb_launch_attention_fwd(ktb_ctx* ctx, const ktb_attn_args* args);
  * scaled scores, in f32; a row that sees none gives 0 and -inf.  The loop of ktb_launch_attention_fwd (running maximum, sum and
  * accumulator per tile of keys, P rounded to f16) over keys and values that are tensors [kv_len][heads / kv_group][head_dim],
  * of any length, instead of pages.  Offsets and strides in elements (f16: multiples of 8; lse f32 [queries][heads],
- * lse_off < 0: not stored); head_dim 64 or 128. */
+ * lse_off < 0: not stored); head_dim 64 or 128.  scale > 0, and scale * head_dim * 65504^2 (what scores may be) 10^30 at most. */
 typedef struct {
     void* arena;
     int64_t q_off, k_off, v_off, o_off, lse_off;
@@ -513,7 +513,7 @@ int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_args* args);
  * query heads that share a key head.  What a KTIR program computes that walks tiles of keys and of queries with
  * linalg.matmul, exp and linalg.reduce (ktir_cpu/ops/arith_ops.py:323-340, ktir_cpu/dialects/linalg_ops.py:136-347).
  * Tensors are [positions][heads][head_dim] f16 (lse f32 [queries][heads]) in the arena, by offset and strides in elements,
- * the f16 ones multiples of 8; head_dim 64 or 128.  lse is the forward pass's (ktb_launch_attention_dense); where it is -inf
+ * the f16 ones multiples of 8; head_dim 64 or 128; scale of any sign, |scale| * head_dim * 65504^2 10^38 at most.  lse is the forward pass's (ktb_launch_attention_dense); where it is -inf
  * the row has no probabilities.  P and dS are rounded to f16 before they are multiplied; the order of every sum is fixed.
  * `want` says which gradients are stored; the dq_* ranges are of query rows and query heads, the dk_* ranges of key rows and
  * key heads, and the rest of the outputs is left as it is.  dev_scratch (256-byte boundary) holds

@@ -936,7 +936,8 @@ extern "C" int ktb_launch_attention_bwd(ktb_ctx* ctx, const ktb_attn_bwd_args* a
     if ((a.want & ~7) || a.want == 0) return ktb_fail(ctx, KTB_E_ARG, me, "which gradients are wanted");
     if (a.q_len == 0 || a.kv_len == 0 || a.heads == 0) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "no queries, keys or heads");
     if (a.q_len > (1 << 30) || a.kv_len > (1 << 30) || a.heads > 65535 * 32) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "lengths or heads");
-    if (!(fabsf(a.scale) <= 3.0e38f)) return ktb_fail(ctx, KTB_E_ARG, me, "score scale must be finite");
+    if (!(fabs((double)a.scale) * a.head_dim * 65504.0 * 65504.0 <= 1.0e38))     // (scores of f16 operands, times 1 / ln 2)
+        return ktb_fail(ctx, KTB_E_ARG, me, "scores must be finite");
     const int kv_heads = a.heads / a.kv_group;
     if (a.want & KTB_ATTN_DQ)
         if (a.dq_row0 < 0 || a.dq_rows < 0 || a.dq_rows > a.q_len - a.dq_row0 || a.dq_head0 < 0 || a.dq_heads < 0 || a.dq_heads > a.heads - a.dq_head0)

@@ -729,7 +729,8 @@ extern "C" int ktb_launch_attention_dense(ktb_ctx* ctx, const ktb_attn_dense_arg
         return ktb_fail(ctx, KTB_E_ARG, me, "lengths, heads or kv_group");
     if (b.q_len == 0 || b.heads == 0) return KTB_OK;
     if (b.kv_len == 0 || b.q_len > (1 << 30) || b.kv_len > (1 << 30)) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "lengths");
-    if (!(b.scale > 0.f && b.scale <= 3.0e38f)) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "score scale must be positive");
+    if (!(b.scale > 0.f && (double)b.scale * b.head_dim * 65504.0 * 65504.0 <= 1.0e30))    // (scores of f16 operands, next to the initial maximum)
+        return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "score scale must be positive, scores below 10^30");
     const int64_t all = b.q_off | b.k_off | b.v_off | b.o_off | b.q_row | b.q_head | b.k_row | b.k_head | b.v_row | b.v_head | b.o_row | b.o_head;
     if ((all & 7) || (reinterpret_cast<uintptr_t>(b.arena) & 15))
         return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "strides and offsets must be multiples of 8 elements");

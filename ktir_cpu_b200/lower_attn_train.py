@@ -30,6 +30,13 @@ from .trace import Access, LoopInfo, Node, Store, Unsupported, iv_full
 
 
 SMS, TILE, STEP = 148, 128, 64           # SMs; rows that a CTA owns, rows that it streams at a time
+# What scores may be at most, by the scale: the forward kernel starts from a maximum of -10^30, the backward one multiplies by 1 / ln 2.
+FORWARD_SCORES, BACKWARD_SCORES = 1.0e30, 1.0e38
+
+
+def _scores_below(scale: float, head_dim: int, bound: float) -> bool:
+    """Whether all scores that f16 operands can have are below ``bound`` in magnitude."""
+    return abs(float(np.float32(scale))) * head_dim * 65504.0 ** 2 <= bound       # (false for a NaN)
 
 
 # ---- pieces of the expressions ------------------------------------------------------------------------------------
@@ -240,10 +247,10 @@ def match_forward(value: Node):
             not _iter_of(lmul.args[0], loop, il) or not is_alpha(lmul.args[1]):
         return None
     m_init, l_init, acc_init = (_const_value(loop.inits[i]) for i in (im, il, ia))
-    # (scores of f16 operands are above -10^13; the maximum of a row that sees nothing has to stay finite)
+    # (the initial maximum has to be below every score, so that its value does not matter, and finite, for rows that see nothing)
     if m_init is None or not -3.0e38 < m_init <= -1.0e20 or l_init != 0.0 or acc_init != 0.0 or not m["scale"] > 0.0:
         return None
-    return dict(m, v=v, cond=cond, loop=loop, im=im, il=il, tile=tuple(masked.shape))
+    return dict(m, v=v, cond=cond, loop=loop, im=im, il=il, m_init=m_init, tile=tuple(masked.shape))
 
 
 def _is_lse(value: Node, m: dict) -> bool:
@@ -482,8 +489,8 @@ class AttentionDenseStatement(Statement):
         hd = int(m["q"].shape[-1])
         if hd not in (64, 128):
             raise Unsupported("attention over whole sequences supports head_dim 64 and 128")
-        if not 0 < np.float32(m["scale"]) < np.inf:
-            raise Unsupported("a score scale that is not positive or not finite")
+        if not np.float32(m["scale"]) > 0.0 or not _scores_below(m["scale"], hd, min(-m["m_init"], FORWARD_SCORES)):
+            raise Unsupported("a score scale that is not positive, or scores that may reach the initial maximum")
         q = _walk(m["q"], store.axes, sel, None, hd, arena, "Read from")
         o = _walk(store.target, store.axes, sel, None, hd, arena, "Scatter to")
         k, v = (_walk(m[x], store.axes, sel, T, hd, arena, "Read from") for x in ("k", "v"))
@@ -609,8 +616,8 @@ class AttentionGradStatement(Statement):
         hd = int(m["q"].shape[-1])
         if hd not in (64, 128):
             raise Unsupported("attention gradient supports head_dim 64 and 128")
-        if not np.isfinite(np.float32(m["scale"])):
-            raise Unsupported("a score scale that is not finite")
+        if not _scores_below(m["scale"], hd, BACKWARD_SCORES):
+            raise Unsupported("a score scale that is not finite, or scores that may not be")
         over_keys = name == "dq"
 
         def own(acc, what="Read from"):

@@ -693,3 +693,34 @@ def test_gradients_with_a_score_scale_of_zero_or_below(c, scale, build_lib):
     got = _run(K.attention_backward(*c), BWD, _kwargs(BWD, kw, c[0], c[2], c[4], do, o, lse, np.float32(scale)), "attention_bwd")
     got["key_grad_ptr"] = -got["key_grad_ptr"]
     _check(got, formulas(mirrored, do, c[5], o, lse, scale=abs(scale)))
+
+
+@pytest.mark.parametrize("scale,low,fwd,bwd", [(1e15, "-1.0e30", 1, 1), (1e22, "-1.0e30", 0, 1), (1e10, "-1.0e20", 0, 1), (1e6, "-1.0e20", 1, 1),
+                                               (3e27, "-1.0e30", 0, 0), (-3e27, "-1.0e30", 0, 0), (3e38, "-2.0e38", 0, 0)])
+def test_scores_that_may_reach_the_initial_maximum_or_infinity_run_step_by_step(scale, low, fwd, bwd):
+    """64 products of f16 are up to 2.7e11: times the scale, they stay above the initial maximum, or their row would not get its
+    own, and times 1 / ln 2 they are finite."""
+    kw, do = _inputs(64, 64, 4, 2, 64)
+    lse = np.zeros((64, 4), np.float32)
+    for fn, make, kind, fused in ((FWD, K.attention_forward, "attention_dense", fwd), (BWD, K.attention_backward, "attention_bwd", bwd)):
+        src = make(64, 64, 4, 2, 64, True).replace("%low = arith.constant -1.0e30", f"%low = arith.constant {low}")
+        assert set(_kinds(src, fn, _kwargs(fn, kw, 64, 4, 64, do, do, lse, np.float32(scale)))) == ({kind} if fused else {"generic"})
+
+
+@pytest.mark.gpu
+def test_launchers_refuse_scores_without_bounds(build_lib):
+    kw, do = _inputs(64, 64, 4, 2, 64)
+    for fn, make, launch, bad, good, code in ((FWD, K.attention_forward, "ktb_launch_attention_dense", (4e18, 3e38, float("inf")), 3e18, -3),
+                                              (BWD, K.attention_backward, "ktb_launch_attention_bwd", (4e26, -4e26, 3e38, float("-inf")), -3e26, -2)):
+        gpu = KTIRInterpreter()
+        gpu.load(make(64, 64, 4, 2, 64, True))
+        sess, _ = gpu.session(fn, **_kwargs(fn, kw, 64, 4, 64, do, do, np.zeros((64, 4), np.float32)))
+        a = sess.plan.statements[0].args
+        a.arena = sess.arena
+        for scale in bad + (good,):
+            a.scale = scale
+            before = gpu.device.launch_count()
+            rc = getattr(gpu.device.lib, launch)(gpu.device.h, C.byref(a))
+            assert rc == (0 if scale == good else code) and (gpu.device.launch_count() == before) == (scale != good), scale
+        gpu.device.sync()
+        gpu.close()
