@@ -18,8 +18,9 @@
 //
 // f16 operands.  P is at most 1 but mostly near 1 / keys, dS is as small as the gradient: both are rounded to f16 (2^-12 of the
 // value on average, the only roundings before the results') after a shift by powers of two that keeps them in range: P by
-// 2^14, dS by 2^14 / B with B >= |dO V^T - D| a power of two from the norms of dO and V (per row for dQ, per key head for dK,
-// whose sums run over rows).  Sums, D and the statistics are f32.  Where few rows see a key these roundings are multiplied too
+// 2^14, dS by 2^14 / B with B >= |dO V^T - D| a power of two from the norms of dO and V (per query for dQ; for dK, whose sums
+// run over queries, per key and from the queries that see it: one for all keys lost dK of those behind a query 10^6 times as
+// loud as the others 2 % of their value).  Sums, D and the statistics are f32.  Where few rows see a key these roundings are multiplied too
 // (MODE 2).
 //
 // 256 heads of 2048 positions, 128 wide, causal: 1.04 ms, 660 TFLOP/s of the five products (925 of the seven), 1.20 ms once
@@ -503,17 +504,54 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (lane == 0) tc_mbar_arrive(a_ready);
             return true;
         };
-        // What an item needs of its rows, asked for while the item before it ends: the largest |dO|, |D| and |V| of its key head
-        // (this lane's share of them), and of a query row 14 - lse / ln 2, D and |dO|.
-        struct ab_known { float most_g, most_d, most_v, nl, d, norm; };
+        // What an item needs of its rows, asked for while the item before it ends.  A key's shift follows from the largest |dO| and |D| of
+        // the queries that see it: this lane's share of those that all keys of its warp see, and those of the first query that its
+        // own key sees; the largest |V| of the key head (this lane's share); of a query row 14 - lse / ln 2, D and |dO|.
+        struct ab_known { float most_g, most_d, most_v, g, nl, d, norm; };
         auto ask = [&](const ab_item& it) {
-            ab_known v = {0.f, 0.f, 0.f, -INFINITY, 0.f, 0.f};
+            ab_known v = {0.f, 0.f, 0.f, 0.f, -INFINITY, 0.f, 0.f};
             const int kvh = it.keys ? it.head : it.head / grp;
             if (it.keys) {
-                for (int i = lane; i < w.q_blocks * grp; i += 32) {
-                    const float2 m = w.most_q[(int64_t)kvh * grp * w.q_blocks + i];
-                    v.most_g = fmaxf(v.most_g, m.x);
-                    v.most_d = fmaxf(v.most_d, m.y);
+                // Per head: queries own, own + 32, ... up to a block's end (own: the first that this lane's key sees), then whole
+                // blocks; 32 of either at a time, four loads ahead of the arithmetic.
+                const int rows = w.block >> w.q_log;
+                long long own = 0, edge = 0;                    // (unmasked: all blocks)
+                int block = 0, singles = 0;
+                if (a.causal) {
+                    const long long behind = (long long)it.row0 + (warp & 3) * 32 + 32 - a.causal_delta;      // queries from here on: all keys of the warp
+                    const int from = behind < 0 ? 0 : behind > a.q_len ? a.q_len : (int)behind;
+                    block = (from + rows - 1) / rows;
+                    edge = block * rows < a.q_len ? block * rows : a.q_len;
+                    singles = 1 + (int)((edge - from + 31) / 32);
+                    own = behind - 32 + lane;
+                }
+                const int per_head = singles + (w.q_blocks - block + 31) / 32;
+                int64_t head = (int64_t)kvh * grp;
+                const int64_t head_end = head + grp;
+                int c = 0;
+#pragma unroll 1
+                while (head < head_end) {
+                    float2 m[4];
+                    bool of_own[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        m[k] = make_float2(0.f, 0.f);
+                        of_own[k] = c == 0 && singles;
+                        if (head >= head_end) continue;
+                        if (c < singles) {
+                            const long long q = own + 32 * c;
+                            if (q >= 0 && q < edge) m[k] = make_float2(w.norm[head * w.padded + q], w.d[head * w.padded + q]);
+                        } else if (block + (c - singles) * 32 + lane < w.q_blocks) {
+                            m[k] = w.most_q[head * w.q_blocks + block + (c - singles) * 32 + lane];
+                        }
+                        if (++c == per_head) c = 0, ++head;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float d = fabsf(m[k].y) <= 3.0e38f ? fabsf(m[k].y) : 0.f;
+                        if (of_own[k]) v.g = fmaxf(v.g, m[k].x), v.d = fmaxf(v.d, d);
+                        else v.most_g = fmaxf(v.most_g, m[k].x), v.most_d = fmaxf(v.most_d, d);
+                    }
                 }
             } else if (it.row0 + r < a.q_len) {
                 const int64_t at = (int64_t)it.head * w.padded + it.row0 + r;
@@ -527,6 +565,12 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         auto of_warp = [&](float x) {
 #pragma unroll
             for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+            return x;
+        };
+        // Of this lane's value and those of the lanes behind it.
+        auto of_later = [&](float x) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) x = fmaxf(x, __shfl_down_sync(0xffffffffu, x, o));
             return x;
         };
         // Columns [32 h, 32 h + 32) of T: a difference of T and D within the rounding of their sums, 2^-22 of |dO| |V|, is none: a
@@ -551,7 +595,8 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             const int row = it.row0 + r;
             const float most_v = of_warp(known.most_v);
             const float row_nl = known.nl, row_d = known.d;
-            const float shrink = KEYS ? ab_shrink(of_warp(known.most_g) * most_v + of_warp(known.most_d)) : ab_shrink(known.norm * most_v + fabsf(row_d));
+            const float shrink = KEYS ? ab_shrink(fmaxf(of_warp(known.most_g), of_later(known.g)) * most_v + fmaxf(of_warp(known.most_d), of_later(known.d)))
+                                      : ab_shrink(known.norm * most_v + fabsf(row_d));
             const float near = (KEYS ? most_v : known.norm * most_v) * 0x1p-22f;
             const uint64_t shrink2 = at_pack2(shrink, shrink);
             const uint64_t row_nl2 = at_pack2(row_nl, row_nl), row_d2 = at_pack2(-row_d, -row_d);

@@ -724,3 +724,34 @@ def test_launchers_refuse_scores_without_bounds(build_lib):
             assert rc == (0 if scale == good else code) and (gpu.device.launch_count() == before) == (scale != good), scale
         gpu.device.sync()
         gpu.close()
+
+
+def _close(got, want, what):
+    """Rounding errors, in 2-norms: of P or dS and of the result, each 2^-11 of a value at most and less than two thirds of that on
+    average, are together below 2^-10.5."""
+    off = np.linalg.norm(got.astype(np.float64) - want) / np.linalg.norm(want)
+    assert off <= 2 ** -10.5, (what, float(off))
+
+
+LOUD = [(700, 700, 2, 2, 128, True), (700, 700, 8, 1, 64, True), (500, 700, 1, 1, 128, True), (600, 430, 12, 4, 64, True), (300, 2000, 2, 1, 128, True)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("loud", [1e5, 1e6])
+@pytest.mark.parametrize("c", LOUD)
+def test_a_loud_query_costs_keys_that_it_does_not_see_nothing(c, loud, build_lib):
+    q_len, kv_len, heads, _, hd, _ = c
+    kw, do = _inputs(*c[:5], seed=q_len, grad=0.01)
+    quiet = do.copy()
+    at = max(20, q_len - kv_len + 20)
+    do[at] = np.clip(do[at].astype(np.float32) * loud, -6e4, 6e4).astype(np.float16)
+    o, lse = _forward_results(kw, True)
+    got = _run(K.attention_backward(*c), BWD, _kwargs(BWD, kw, q_len, heads, hd, do, o, lse), "attention_bwd")
+    quiet[at] = 0
+    want = formulas(kw, quiet, True, o, lse)
+    behind = at + kv_len - q_len + 1                             # the first key that the loud query does not see
+    _close(got["key_grad_ptr"][behind:], want["key_grad_ptr"][0][behind:], "dK")
+    _close(got["key_grad_ptr"][behind:behind + 20], want["key_grad_ptr"][0][behind:behind + 20], "dK right behind")
+    _close(got["value_grad_ptr"][behind:], want["value_grad_ptr"][0][behind:], "dV")
+    rest = np.arange(q_len) != at
+    _close(got["query_grad_ptr"][rest], want["query_grad_ptr"][0][rest], "dQ")
