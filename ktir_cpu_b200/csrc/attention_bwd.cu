@@ -18,9 +18,9 @@
 //
 // f16 operands.  P is at most 1 but mostly near 1 / keys, dS is as small as the gradient: both are rounded to f16 (2^-12 of the
 // value on average, the only roundings before the results') after a shift by powers of two that keeps them in range: P by
-// 2^14, dS by 2^14 / B with B >= |dO V^T - D| a power of two from the norms of dO and V (per query for dQ; for dK, whose sums
-// run over queries, per key and from the queries that see it: one for all keys lost dK of those behind a query 10^6 times as
-// loud as the others 2 % of their value).  Sums, D and the statistics are f32.  Where few rows see a key these roundings are multiplied too
+// 2^14, dS by 2^14 / B with B >= |dO V^T - D| a power of two from the norms of dO and V: for dQ, whose sums run over keys, per
+// query and from the keys that it sees, for dK per key and from the queries that see it.  (From all of a head, dK of the keys
+// behind a query 10^6 times as loud as the others lost 2 % of its value, dQ of the queries before such a value likewise.)  Sums, D and the statistics are f32.  Where few rows see a key these roundings are multiplied too
 // (MODE 2).
 //
 // 256 heads of 2048 positions, 128 wide, causal: 1.04 ms, 660 TFLOP/s of the five products (925 of the seven), 1.20 ms once
@@ -49,6 +49,7 @@ struct ab_scratch {
     float* norm;
     float2* most_q;                // [heads][q_blocks]: largest |dO| and |D| of a block of queries
     float* most_v;                 // [key heads][k_blocks]: largest |V| of a block of keys
+    float* norm_v;                 // [key heads][keys]: |V|
     int64_t padded;
     int q_log, k_log;              // heads_log for queries, for keys
     int q_blocks, k_blocks;
@@ -121,6 +122,7 @@ __global__ void __launch_bounds__(256) ktb_attention_rows_kernel(const ktb_attn_
                 w.d[to] = d;
                 w.norm[to] = sqrtf(g2);
             }
+            if (keys && lane == 0 && row < rows && head < heads && i0 + i * GROUPS + group < BLOCK) w.norm_v[head * rows + row] = sqrtf(g2);
         }
     }
     __shared__ float sa[GROUPS], sd[GROUPS];
@@ -504,12 +506,13 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (lane == 0) tc_mbar_arrive(a_ready);
             return true;
         };
-        // What an item needs of its rows, asked for while the item before it ends.  A key's shift follows from the largest |dO| and |D| of
-        // the queries that see it: this lane's share of those that all keys of its warp see, and those of the first query that its
-        // own key sees; the largest |V| of the key head (this lane's share); of a query row 14 - lse / ln 2, D and |dO|.
-        struct ab_known { float most_g, most_d, most_v, g, nl, d, norm; };
+        // What an item needs of its rows, asked for while the item before it ends.  A key's shift follows from its |V| and the largest
+        // |dO| and |D| of the queries that see it: this lane's share of those that all keys of its warp see, and those of the first
+        // query that its own key sees.  A query's follows from its |dO| and |D| and the largest |V| of the keys that it sees: this lane's
+        // share of those that all queries of its warp see, and that of the last key that its own query sees.  And of a query 14 - lse / ln 2.
+        struct ab_known { float most_g, most_d, most_v, g, d, v, nl; };
         auto ask = [&](const ab_item& it) {
-            ab_known v = {0.f, 0.f, 0.f, 0.f, -INFINITY, 0.f, 0.f};
+            ab_known v = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, -INFINITY};
             const int kvh = it.keys ? it.head : it.head / grp;
             if (it.keys) {
                 // Per head: queries own, own + 32, ... up to a block's end (own: the first that this lane's key sees), then whole
@@ -553,13 +556,31 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                         else v.most_g = fmaxf(v.most_g, m[k].x), v.most_d = fmaxf(v.most_d, d);
                     }
                 }
-            } else if (it.row0 + r < a.q_len) {
-                const int64_t at = (int64_t)it.head * w.padded + it.row0 + r;
-                v.nl = w.neg_lse[at];
-                v.d = w.d[at];
-                v.norm = w.norm[at];
+                if (it.row0 + r < a.kv_len) v.v = w.norm_v[(int64_t)kvh * a.kv_len + it.row0 + r];
+            } else {
+                const float *norms = w.norm_v + (int64_t)kvh * a.kv_len, *of_blocks = w.most_v + (int64_t)kvh * w.k_blocks;
+                if (it.row0 + r < a.q_len) {
+                    const int64_t at = (int64_t)it.head * w.padded + it.row0 + r;
+                    v.nl = w.neg_lse[at];
+                    v.d = w.d[at];
+                    v.g = w.norm[at];
+                }
+                int blocks = w.k_blocks, edge = 0, single = 0;  // whole blocks that all queries of the warp see, then single keys
+                if (a.causal) {
+                    const long long first = (long long)it.row0 + (warp & 3) * 32 + 1 + a.causal_delta, own = first - 1 + lane;
+                    if (own >= 0 && own < a.kv_len) v.v = norms[own];
+                    if (first < a.kv_len) {
+                        edge = first < 0 ? 0 : (int)first;
+                        blocks = edge / (w.block >> w.k_log);
+                        single = blocks * (w.block >> w.k_log);
+                    }
+                }
+#pragma unroll 2
+                for (int i = lane; i < blocks || single + i < edge; i += 32) {
+                    const float x = i < blocks ? of_blocks[i] : 0.f, y = single + i < edge ? norms[single + i] : 0.f;
+                    v.most_v = fmaxf(v.most_v, fmaxf(x, y));
+                }
             }
-            for (int i = lane; i < w.k_blocks; i += 32) v.most_v = fmaxf(v.most_v, w.most_v[(int64_t)kvh * w.k_blocks + i]);
             return v;
         };
         auto of_warp = [&](float x) {
@@ -571,6 +592,12 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         auto of_later = [&](float x) {
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) x = fmaxf(x, __shfl_down_sync(0xffffffffu, x, o));
+            return x;
+        };
+        // ... and those of the lanes before it.
+        auto of_earlier = [&](float x) {
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) x = fmaxf(x, __shfl_up_sync(0xffffffffu, x, o));
             return x;
         };
         // Columns [32 h, 32 h + 32) of T: a difference of T and D within the rounding of their sums, 2^-22 of |dO| |V|, is none: a
@@ -593,11 +620,12 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         auto walk = [&](auto of_keys, const ab_item& it, int k, int& index) -> bool {
             constexpr bool KEYS = decltype(of_keys)::value;
             const int row = it.row0 + r;
-            const float most_v = of_warp(known.most_v);
             const float row_nl = known.nl, row_d = known.d;
-            const float shrink = KEYS ? ab_shrink(fmaxf(of_warp(known.most_g), of_later(known.g)) * most_v + fmaxf(of_warp(known.most_d), of_later(known.d)))
-                                      : ab_shrink(known.norm * most_v + fabsf(row_d));
-            const float near = (KEYS ? most_v : known.norm * most_v) * 0x1p-22f;
+            float most_g = known.g, most_v = known.v, most_d = fabsf(row_d);
+            if (KEYS) most_g = fmaxf(of_warp(known.most_g), of_later(known.g)), most_d = fmaxf(of_warp(known.most_d), of_later(known.d));
+            else most_v = fmaxf(of_warp(known.most_v), of_earlier(known.v));
+            const float shrink = ab_shrink(most_g * most_v + most_d);
+            const float near = (KEYS ? most_v : most_g * most_v) * 0x1p-22f;
             const uint64_t shrink2 = at_pack2(shrink, shrink);
             const uint64_t row_nl2 = at_pack2(row_nl, row_nl), row_d2 = at_pack2(-row_d, -row_d);
             const int last = it.first + it.per_head;
@@ -869,10 +897,12 @@ static int64_t ab_row_blocks(int64_t rows, int heads, int block) { return (rows 
 static int ab_block(const ktb_attn_bwd_args& a) { return (int64_t)a.q_len * a.heads + (int64_t)a.kv_len * (a.heads / a.kv_group) <= 16384 ? 64 : 256; }
 
 static int64_t ab_up(int64_t bytes) { return (bytes + 255) / 256 * 256; }
-// A counter; per query and head three floats; per block of queries and head two, per block of keys and key head one ...
+// A counter; per query and head three floats, per key and key head one; per block of queries and head two, per block of keys and key
+// head one ...
 static int64_t ab_rows_bytes(const ktb_attn_bwd_args& a) {
     const int kv_heads = a.heads / a.kv_group;
-    return ab_up(256 + 4 * (int64_t)a.heads * (3 * ab_padded(a) + 2 * ab_row_blocks(ab_padded(a), a.heads, ab_block(a))) + 4 * kv_heads * ab_row_blocks(a.kv_len, kv_heads, ab_block(a)));
+    return ab_up(256 + 4 * (int64_t)a.heads * (3 * ab_padded(a) + 2 * ab_row_blocks(ab_padded(a), a.heads, ab_block(a))) +
+                 4 * (int64_t)kv_heads * (ab_row_blocks(a.kv_len, kv_heads, ab_block(a)) + a.kv_len));
 }
 // ... and, of walks that are cut, the parts' sums.
 static int64_t ab_part_bytes(const ktb_attn_bwd_args& a, bool keys) {
@@ -906,6 +936,7 @@ static int ab_run(ktb_ctx* ctx, const ktb_attn_bwd_args& a) {
     w.norm = w.d + (int64_t)a.heads * w.padded;
     w.most_q = reinterpret_cast<float2*>(w.norm + (int64_t)a.heads * w.padded);
     w.most_v = reinterpret_cast<float*>(w.most_q + (int64_t)a.heads * w.q_blocks);
+    w.norm_v = w.most_v + (int64_t)kv_heads * w.k_blocks;
     CUtensorMap mq, mk, mv, mg;
     if (!ab_map(&mq, a, a.q_off, a.q_len, a.heads, a.q_row, a.q_head) || !ab_map(&mg, a, a.do_off, a.q_len, a.heads, a.do_row, a.do_head) ||
         !ab_map(&mk, a, a.k_off, a.kv_len, kv_heads, a.k_row, a.k_head) || !ab_map(&mv, a, a.v_off, a.kv_len, kv_heads, a.v_row, a.v_head))

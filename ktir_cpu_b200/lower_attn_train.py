@@ -572,8 +572,8 @@ def grad_parts(q_len: int, kv_len: int, heads: int, kv_heads: int, causal: int, 
 
 
 def grad_scratch_bytes(a: "R.AttnBwdArgs") -> int:
-    """``ktb_attention_bwd_scratch_bytes``: a counter, three floats per query (in tiles of 64) and head, two per block of queries
-    and head and one per block of keys and key head, where a block is 64 or 256 rows of a head or as many of up to eight heads; and the
+    """``ktb_attention_bwd_scratch_bytes``: a counter, three floats per query (in tiles of 64) and head, one per key and key head,
+    two per block of queries and head and one per block of keys and key head, where a block is 64 or 256 rows of a head or as many of up to eight heads; and the
     f32 sums of the parts of cut walks."""
     def up(n):
         return -(-n // 256) * 256
@@ -582,7 +582,7 @@ def grad_scratch_bytes(a: "R.AttnBwdArgs") -> int:
         return -(-rows // (block >> min(3, n.bit_length() - 1)))
     padded, kv_heads = -(-a.q_len // 64) * 64, a.heads // a.kv_group
     block = 64 if a.q_len * a.heads + a.kv_len * kv_heads <= 16384 else 256
-    total = up(256 + 4 * a.heads * (3 * padded + 2 * blocks(padded, a.heads)) + 4 * kv_heads * blocks(a.kv_len, kv_heads))
+    total = up(256 + 4 * a.heads * (3 * padded + 2 * blocks(padded, a.heads)) + 4 * kv_heads * (blocks(a.kv_len, kv_heads) + a.kv_len))
     if a.want & R.ATTN_DQ and a.query_parts > 1:
         total += up(4 * a.query_parts * a.head_dim * a.dq_rows * a.dq_heads)
     if a.want & (R.ATTN_DK | R.ATTN_DV) and a.key_parts > 1:

@@ -755,3 +755,21 @@ def test_a_loud_query_costs_keys_that_it_does_not_see_nothing(c, loud, build_lib
     _close(got["value_grad_ptr"][behind:], want["value_grad_ptr"][0][behind:], "dV")
     rest = np.arange(q_len) != at
     _close(got["query_grad_ptr"][rest], want["query_grad_ptr"][0][rest], "dQ")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("loud", [1e5, 1e6])
+@pytest.mark.parametrize("c", LOUD)
+def test_a_loud_value_costs_queries_that_do_not_see_it_nothing(c, loud, build_lib):
+    q_len, kv_len, heads, _, hd, _ = c
+    kw, do = _inputs(*c[:5], seed=q_len)
+    kw["value_ptr"] = (kw["value_ptr"] * np.float16(0.01)).astype(np.float16)
+    at = kv_len - 30
+    kw["value_ptr"][at] = np.clip(kw["value_ptr"][at].astype(np.float32) * loud, -6e4, 6e4).astype(np.float16)
+    o, lse = _forward_results(kw, True)
+    got = _run(K.attention_backward(*c), BWD, _kwargs(BWD, kw, q_len, heads, hd, do, o, lse), "attention_bwd")
+    want = formulas(kw, do, True, o, lse)
+    before = q_len - 30                                          # the first query that sees the loud value
+    _close(got["query_grad_ptr"][:before], want["query_grad_ptr"][0][:before], "dQ")
+    _close(got["query_grad_ptr"][before - 20:before], want["query_grad_ptr"][0][before - 20:before], "dQ right before")
+    _check(got, want)
