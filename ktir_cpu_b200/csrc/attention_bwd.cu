@@ -600,19 +600,16 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             for (int o = 1; o < 32; o <<= 1) x = fmaxf(x, __shfl_up_sync(0xffffffffu, x, o));
             return x;
         };
-        // Columns [32 h, 32 h + 32) of T: a difference of T and D within the rounding of their sums, 2^-22 of |dO| |V|, is none: a
-        // query that sees one key has no gradient.  (Where there are more keys than a step's, others' gradients are far above that.)
-        auto settle = [&](auto of_keys, uint32_t (&t)[32], const float4* rows, int h, float d, float near) {
+        // Columns [32 h, 32 h + 32) of T: a difference of T and D within the rounding of their sums, 2^-22 of |dO| |V| of that query and
+        // that key, is none: a query that sees one key has no gradient.  (Where there are more keys than a step's, others' gradients are far
+        // above that.)  `near`: 2^-22 of this row's norm; `norms_v`: |V| of the keys, where the columns are keys.
+        auto settle = [&](auto of_keys, uint32_t (&t)[32], const float4* rows, const float* norms_v, int h, float d, float near) {
             constexpr bool KEYS = decltype(of_keys)::value;
+            const float* of_row = reinterpret_cast<const float*>(rows) + 32 * h;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
-                float dj = d, most = near;
-                if (KEYS) {
-                    const float* of_row = reinterpret_cast<const float*>(rows) + 32 * h + j;
-                    dj = of_row[AB_N];
-                    most = near * of_row[2 * AB_N];
-                }
-                if (fabsf(__uint_as_float(t[j]) - dj) <= most) t[j] = __float_as_uint(dj);
+                const float dj = KEYS ? of_row[AB_N + j] : d, norm = KEYS ? of_row[2 * AB_N + j] : 32 * h + j < a.kv_len ? norms_v[32 * h + j] : 0.f;
+                if (fabsf(__uint_as_float(t[j]) - dj) <= near * norm) t[j] = __float_as_uint(dj);
             }
         };
         ab_known known = {};
@@ -625,7 +622,8 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             if (KEYS) most_g = fmaxf(of_warp(known.most_g), of_later(known.g)), most_d = fmaxf(of_warp(known.most_d), of_later(known.d));
             else most_v = fmaxf(of_warp(known.most_v), of_earlier(known.v));
             const float shrink = ab_shrink(most_g * most_v + most_d);
-            const float near = (KEYS ? most_v : most_g * most_v) * 0x1p-22f;
+            const float near = (KEYS ? most_v : most_g) * 0x1p-22f;
+            const float* norms_v = w.norm_v + (int64_t)(KEYS ? it.head : it.head / grp) * a.kv_len;
             const uint64_t shrink2 = at_pack2(shrink, shrink);
             const uint64_t row_nl2 = at_pack2(row_nl, row_nl), row_d2 = at_pack2(-row_d, -row_d);
             const int last = it.first + it.per_head;
@@ -712,7 +710,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             for (int j = 0; j < 8; ++j) nl[j] = rows[8 + j];
                         }
                         tc_tmem_ld_wait();
-                        if (TWICE && a.kv_len <= AB_N) settle(of_keys, t, rows, h, row_d, near);
+                        if (TWICE && a.kv_len <= AB_N) settle(of_keys, t, rows, norms_v, h, row_d, near);
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
                             uint64_t d2 = row_d2;
@@ -741,7 +739,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                             for (int j = 0; j < 32; ++j)
                                 if (32 * h + j < lo || 32 * h + j >= hi) s[j] = hidden;
                         }
-                        if (TWICE && a.kv_len <= AB_N) settle(of_keys, t, rows, h, row_d, near);
+                        if (TWICE && a.kv_len <= AB_N) settle(of_keys, t, rows, norms_v, h, row_d, near);
 #pragma unroll
                         for (int j = 0; j < 32; j += 2) {
                             uint64_t nl2 = row_nl2, d2 = row_d2;

@@ -773,3 +773,20 @@ def test_a_loud_value_costs_queries_that_do_not_see_it_nothing(c, loud, build_li
     _close(got["query_grad_ptr"][:before], want["query_grad_ptr"][0][:before], "dQ")
     _close(got["query_grad_ptr"][before - 20:before], want["query_grad_ptr"][0][before - 20:before], "dQ right before")
     _check(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hidden", [True, False])
+@pytest.mark.parametrize("c", [(16, 16, 2, 2, 64, True), (12, 40, 4, 2, 128, True), (20, 20, 3, 3, 64, False)])
+def test_few_keys_of_very_different_values(c, hidden, build_lib):
+    """A small difference of dO V^T and D is a gradient unless it is small next to that key's own value.  The large value is seen by
+    the last query only, or has next to no probability: a score of -16 and less next to the others'."""
+    kw, do = _inputs(*c[:5], seed=c[1])
+    at = -1 if hidden else 0
+    kw["value_ptr"][at] = np.clip(kw["value_ptr"][at].astype(np.float32) * 1e4, -6e4, 6e4).astype(np.float16)
+    if not hidden:
+        kw["query_ptr"][..., 0], kw["key_ptr"][..., 0], kw["key_ptr"][0] = 8, 2, 0
+        kw["key_ptr"][0, :, 0] = 2 - 2 * math.sqrt(c[4])
+    o, lse = _forward_results(kw, c[5])
+    got = _run(K.attention_backward(*c), BWD, _kwargs(BWD, kw, c[0], c[2], c[4], do, o, lse), "attention_bwd")
+    _check(got, formulas(kw, do, c[5], o, lse, half=HALF * HALF))
