@@ -385,7 +385,7 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         if (lane == 0 && *abort_flag && c > 0) ab_drain(own_full, (c - 1) & 1);
     } else if (warp == 1) {
         if (tc_elect_one()) {
-        // the warp runs this converged; one elected lane issues the tcgen05 instructions
+        // (one elected lane waits and issues)
         const uint32_t idesc_s = tc_idesc_f16(AB_M, AB_N, 0, 0), idesc_a = tc_idesc_f16(AB_M, HD, 0, 1);
         const uint64_t xd = tc_smem_desc(tc_smem_u32(sX), 16, 1024), yd = tc_smem_desc(tc_smem_u32(sY), 16, 1024);
         const uint32_t ring_at = tc_smem_u32(ring);
@@ -816,11 +816,13 @@ ktb_attention_bwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                     for (int j = 0; j < 32; ++j) v[j] = 0;
                 }
                 if (PARTS && sum) {
-                    if (!store || !want || row >= row_end) continue;
+                    if (store && want && row < row_end) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<float4*>(sum + x + j) = make_float4(__uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor,
-                                                                             __uint_as_float(v[j + 2]) * factor, __uint_as_float(v[j + 3]) * factor);
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<float4*>(sum + x + j) = make_float4(__uint_as_float(v[j]) * factor, __uint_as_float(v[j + 1]) * factor,
+                                                                                 __uint_as_float(v[j + 2]) * factor, __uint_as_float(v[j + 3]) * factor);
+                    }
+                    __syncwarp();                               // (the next load takes the whole warp)
                 } else if (want) {                              // (the same for the whole warp)
                     uint32_t o[16];
 #pragma unroll

@@ -460,6 +460,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
                 for (int c = 0; c < OH; c += 8) *reinterpret_cast<uint4*>(dst + c) = make_uint4(0, 0, 0, 0);
                 if (half == 0 && d.lse) d.lse[(int64_t)R * d.row + (int64_t)head * d.head] = -INFINITY;
             }
+            __syncwarp();
             continue;
         }
         float m_ref = a.m_init * 1.4426950408889634f;           // exponent reference, log2 domain
@@ -589,6 +590,7 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
 #pragma unroll
                 for (int c0 = 0; c0 < OH; c0 += 32) {
                     uint32_t o[32];
+                    __syncwarp();                               // (some rows store, the load takes the whole warp)
                     tc_tmem_ld32(o_addr + c0, o);
                     tc_tmem_ld_wait();
                     if (part_of && store) {
