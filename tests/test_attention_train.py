@@ -790,3 +790,19 @@ def test_few_keys_of_very_different_values(c, hidden, build_lib):
     o, lse = _forward_results(kw, c[5])
     got = _run(K.attention_backward(*c), BWD, _kwargs(BWD, kw, c[0], c[2], c[4], do, o, lse), "attention_bwd")
     _check(got, formulas(kw, do, c[5], o, lse, half=HALF * HALF))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [(200, 4000, 2, 2, 64, False), (600, 3000, 1, 1, 128, False), (30, 5000, 8, 1, 128, False), (3000, 3000, 1, 1, 64, True)])
+def test_keys_far_below_the_largest_score_keep_their_precision(c, build_lib):
+    """The first key has 13 more than the others, and a value of 0: what is left are probabilities of 2 * 10^-6, below the normal numbers of f16."""
+    q_len, kv_len, heads, _, hd, causal = c
+    kw, _ = _inputs(*c[:5], seed=hd)
+    kw["query_ptr"][..., 0], kw["key_ptr"][..., 0], kw["value_ptr"][0] = 8, 0, 0
+    kw["key_ptr"][0] = 0
+    kw["key_ptr"][0, :, 0] = 13 / 8 * math.sqrt(hd)
+    got = _run(K.attention_forward(*c), FWD, _kwargs(FWD, kw, q_len, heads, hd), "attention_dense")
+    want = formulas(kw, None, causal)
+    _check(got, want)
+    far = 500 if causal else 0
+    _close(got["output_ptr"][far:], want["output_ptr"][0][far:], "O")
