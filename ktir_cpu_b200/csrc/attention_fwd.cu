@@ -46,27 +46,30 @@ static __device__ __forceinline__ void at_tma_load_4d(void* smem_dst, const CUte
         : "memory");
 }
 
+// Of three; NAN_TOO: a NaN among them is the result.
+template <bool NAN_TOO>
 static __device__ __forceinline__ float at_max3(float a, float b, float c) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    if (NAN_TOO) asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    else asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 // Maximum of CW raw scores.
-template <int CW>
+template <int CW, bool NAN_TOO>
 static __device__ __forceinline__ float at_chunk_max(const uint32_t (&v)[CW], float mx) {
     if (CW % 8 == 0) {                 // four independent chains: the latency of max is not hidden otherwise
         float m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
         for (int i = 0; i < CW; i += 8) {
-            mx = at_max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-            m1 = at_max3(m1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
-            m2 = at_max3(m2, __uint_as_float(v[i + 4]), __uint_as_float(v[i + 5]));
-            m3 = at_max3(m3, __uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
+            mx = at_max3<NAN_TOO>(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+            m1 = at_max3<NAN_TOO>(m1, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+            m2 = at_max3<NAN_TOO>(m2, __uint_as_float(v[i + 4]), __uint_as_float(v[i + 5]));
+            m3 = at_max3<NAN_TOO>(m3, __uint_as_float(v[i + 6]), __uint_as_float(v[i + 7]));
         }
-        return at_max3(mx, m1, fmaxf(m2, m3));
+        return at_max3<NAN_TOO>(at_max3<NAN_TOO>(mx, m1, m2), m3, m3);
     }
 #pragma unroll
-    for (int i = 0; i < CW; i += 2) mx = at_max3(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+    for (int i = 0; i < CW; i += 2) mx = at_max3<NAN_TOO>(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
     return mx;
 }
 
@@ -523,11 +526,13 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             // row maximum of the raw scores (the scale is positive, so it commutes with max)
             float mx = -INFINITY;
 #pragma unroll
-            for (int c = 0; c < NCH; ++c) mx = at_chunk_max<CW>(v[c], mx);
+            for (int c = 0; c < NCH; ++c) mx = at_chunk_max<CW, DENSE>(v[c], mx);
             float mx_other = mx;
             // after the swap both threads of the row have their scores in registers: P may go over them
             if (TPR == 2 && !swap_with_partner(mx, mx_other)) { ok = false; break; }
             m_run = fmaxf(m_run, fmaxf(mx, mx_other) * sl);
+            // (a score that is NaN or infinite makes its row NaN: the polynomial would make a probability of 2^-125 of a NaN)
+            if (DENSE && !(mx < INFINITY)) m_ref = __uint_as_float(0x7fffffffu);
             // move the exponent reference only when the maximum has outgrown it by 2^8
             // (m_run and m_ref are the same on both threads of a row, so they move together)
             const bool move = m_run > m_ref + AT_RESCALE_GAP;

@@ -806,3 +806,18 @@ def test_keys_far_below_the_largest_score_keep_their_precision(c, build_lib):
     _check(got, want)
     far = 500 if causal else 0
     _close(got["output_ptr"][far:], want["output_ptr"][0][far:], "O")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [(150, 150, 2, 2, 128, True), (300, 333, 2, 1, 64, False), (90, 90, 40, 40, 64, True), (3, 2000, 2, 2, 128, False)])
+@pytest.mark.parametrize("what", [np.nan, np.inf, -np.inf])
+def test_special_values_in_keys(c, what, build_lib):
+    """A NaN score, or one of infinity, makes its row NaN; one of -infinity has no probability; a hidden one does nothing."""
+    kw, _ = _inputs(*c[:5])
+    n = c[1] - c[0] if c[5] else 0
+    for j in range(8):
+        x = {k: v.copy() for k, v in kw.items()}
+        x["key_ptr"][c[1] // 2 + j, 0, 5] = what
+        x["query_ptr"][:, 0, 5] = np.abs(x["query_ptr"][:, 0, 5])
+        got = _run(K.attention_forward(*c), FWD, _kwargs(FWD, x, c[0], c[2], c[4]), "attention_dense")
+        _check(got, formulas(x, None, c[5]))
