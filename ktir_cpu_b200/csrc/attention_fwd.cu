@@ -584,9 +584,9 @@ ktb_attention_fwd_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             // total row sum = the two partial sums (same rescaling history on both threads)
             float l_other = 0.f;
             if (TPR == 1 || swap_with_partner(l_run, l_other)) {
-                // (the polynomial leaves 2^-125 of a hidden key: a row that sees none, here, is known by its limit)
-                const float sum = DENSE && limit < 0 ? 0.f : l_run + l_other;
-                const float inv = DENSE && limit < 0 ? 0.f : 1.0f / sum;
+                // (the largest score that is seen has added 2^7, by the shift; one that is hidden, or -infinity, is nothing, though the polynomial makes 2^-125 of it.  A NaN stays one.)
+                const float total = l_run + l_other, sum = DENSE && total < 0x1p-40f ? 0.f : total;
+                const float inv = DENSE && sum == 0.f ? 0.f : 1.0f / sum;
                 const bool store = *abort_flag == 0 && R < a.seq_q;
                 // (m_ref in units of log 2; the logarithm of an empty sum is -inf)
                 const int64_t at_part = at_part_row(d, a.heads, part, head, R);

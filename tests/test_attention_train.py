@@ -821,3 +821,15 @@ def test_special_values_in_keys(c, what, build_lib):
         x["query_ptr"][:, 0, 5] = np.abs(x["query_ptr"][:, 0, 5])
         got = _run(K.attention_forward(*c), FWD, _kwargs(FWD, x, c[0], c[2], c[4]), "attention_dense")
         _check(got, formulas(x, None, c[5]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", [(150, 150, 2, 2, 128, True), (1, 1, 2, 2, 64, False), (40, 2000, 2, 2, 128, True)])
+def test_a_row_whose_scores_are_all_minus_infinity(c, build_lib):
+    kw, _ = _inputs(*c[:5])
+    first = c[1] - c[0]
+    kw["key_ptr"][:first + 1, :, 3] = -np.inf
+    kw["query_ptr"][..., 3] = 1
+    got = _run(K.attention_forward(*c), FWD, _kwargs(FWD, kw, c[0], c[2], c[4]), "attention_dense")
+    assert (got["output_ptr"][0] == 0).all() and (got["lse_ptr"][0] == -np.inf).all()
+    _check(got, formulas(kw, None, c[5]))
