@@ -550,8 +550,8 @@ int ktb_launch_attention_bwd(ktb_ctx* ctx, const ktb_attn_bwd_args* args);
  * its entry of the item table is the offset of its first position (idx_dtype units), then per tensor the offsets, in and
  * out, of the first element of its first pair.  Element j of a pair's first half is at j * pair_stride, its partner
  * in_partner / out_partner (> 0) behind; `rest` elements from in_rest on are copied to out_rest.  Outputs and inputs are
- * apart.  A position whose row is past a table's end (cos_end, sin_end: elements of the arena)
- * reads zeros there; a negative one is recorded in the status word. */
+ * apart.  The arena lies on a boundary of 4 bytes (8 for i64 positions).  A position whose row is past a table's end (cos_end,
+ * sin_end: elements of the arena) reads zeros there; a negative one is recorded in the status word. */
 #define KTB_ROTARY_TENSORS 4
 typedef struct {
     int32_t heads, rest;

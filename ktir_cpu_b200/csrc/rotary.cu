@@ -314,6 +314,7 @@ extern "C" int ktb_launch_rotary(ktb_ctx* ctx, const ktb_rotary_args* args) {
     if (a.pairs <= 0 || a.pair_stride < 1 || a.tokens < 0 || a.n_items < 0 || a.table_stride < 0)
         return ktb_fail(ctx, KTB_E_ARG, "rotary", "pairs, strides and counts");
     if (a.align < 1 || (a.align & (a.align - 1))) return ktb_fail(ctx, KTB_E_ARG, "rotary", "align must be a power of two");
+    if ((uintptr_t)a.arena & (a.idx_dtype == KTB_I64 ? 7 : 3)) return ktb_fail(ctx, KTB_E_ARG, "rotary", "arena off the boundaries of tables and positions");
     const int size = a.dtype == KTB_F16 ? 2 : 4;
     // the lowest set bit of `bits` divides every distance between the vectors of pairs, that of `rest_bits` those behind them
     const int64_t start = (int64_t)a.align | (int64_t)((uintptr_t)a.arena / size);
@@ -356,7 +357,7 @@ extern "C" int ktb_launch_rotary(ktb_ctx* ctx, const ktb_rotary_args* args) {
         if (a.dtype == KTB_F16) return adjacent ? launch_rotary_rows<__half, true>(ctx, a, H, row_vecs) : launch_rotary_rows<__half, false>(ctx, a, H, row_vecs);
         return adjacent ? launch_rotary_rows<float, true>(ctx, a, H, row_vecs) : launch_rotary_rows<float, false>(ctx, a, H, row_vecs);
     }
-    const int table_vec = ((a.table_stride | a.cos_off | a.sin_off) & 3) == 0;
+    const int table_vec = ((a.table_stride | a.cos_off | a.sin_off | (int64_t)((uintptr_t)a.arena / 4)) & 3) == 0;
     const int H = (int)heads_total;
     if (a.dtype == KTB_F16) {
         if (adjacent)

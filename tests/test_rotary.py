@@ -237,3 +237,43 @@ def test_launcher_refuses(build_lib):
     a.arena, a.n_items = sess.arena, 0
     assert dev.lib.ktb_launch_rotary(dev.h, C.byref(a)) == 0
     gpu.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("case", [(33, 9, 2, 64, 64, "half", False, "f16", 11), (33, 9, 2, 64, 64, "interleaved", False, "f16", 11), (16, 4, 4, 96, 48, "half", True, "f32", 4),
+                                  (21, 5, 1, 72, 50, "half", False, "f16", 3)])
+def test_arena_on_any_boundary_of_its_types(case, wide, build_lib):
+    """All tensors moved by 4, 8, ... bytes: vectors are as long as the addresses allow, those of the tables too."""
+    src, kw = _case(*case)
+    if wide:                                        # positions of 64 bits
+        src = src.replace(f"memref<{case[0]}xi32>", f"memref<{case[0]}xi64>")
+        kw["positions_ptr"] = kw["positions_ptr"].astype(np.int64)
+    want = _oracle(src, kw)
+    gpu = KTIRInterpreter()
+    gpu.load(src)
+    sess, _ = gpu.session("rotary_kernel", **kw)
+    st, = sess.plan.statements
+    assert st.kind == "rotary" and st.args.idx_dtype == R.DTYPE_CODE["i64" if wide else "i32"]
+    dev = gpu.device
+    offs = {n: sess.device_ptr(n) - sess.arena for n in kw}
+    room = dev.alloc(max(o + kw[n].nbytes for n, o in offs.items()) + 64)
+    for shift in (4, 8, 12, 16, 24, 2, 1):
+        a = R.RotaryArgs.from_buffer_copy(st.args)
+        a.arena = room + shift
+        refused = shift % (8 if wide else 4) != 0
+        if not refused:
+            for n, x in kw.items():
+                dev.h2d(room + shift + offs[n], x)
+            dev.sync()
+        assert dev.lib.ktb_launch_rotary(dev.h, C.byref(a)) == (-2 if refused else 0), shift
+        if refused:
+            assert b"arena" in dev.lib.ktb_last_error(dev.h)
+            continue
+        for n, x in want.items():
+            got = np.empty_like(x)
+            dev.d2h(got, room + shift + offs[n])
+            dev.sync()
+            np.testing.assert_array_equal(got, x, err_msg=f"{n} {shift}")
+    dev.free(room)
+    gpu.close()
