@@ -512,6 +512,12 @@ def _runs_overlap(s0, e0, s1, e1) -> bool:
     return bool((e1[k[ok]] > s0[ok]).any())
 
 
+def _runs_meet(starts, ends) -> bool:
+    """True if two of the runs have a byte in common."""
+    order = np.argsort(starts, kind="stable")
+    return bool((starts[order][1:] < np.maximum.accumulate(ends[order])[:-1]).any())
+
+
 # ---------------------------------------------------------------------------
 # Row softmax idiom
 # ---------------------------------------------------------------------------

@@ -23,7 +23,7 @@ import numpy as np
 
 from . import runtime as R
 from .dtypes import bytes_per_elem
-from .lower import ArenaMap, Footprint, Statement, _points, _row_broadcast, _row_reduce, _runs_overlap, _skip, strip_views
+from .lower import ArenaMap, Footprint, Statement, _points, _row_broadcast, _row_reduce, _runs_meet, _runs_overlap, _skip, strip_views
 from .lower_attn import _const_value, _ew, _int_affine
 from .lower_mm import _is_zero_const, _unext
 from .trace import Access, LoopInfo, Node, Store, Unsupported, iv_full
@@ -411,7 +411,9 @@ def _footprints(arena: ArenaMap, reads, writes, stmt_id: int) -> List[Footprint]
 
 
 def _disjoint(arena: ArenaMap, reads, writes) -> bool:
-    """No written run overlaps a tensor that is read, or another written run."""
+    """No written run overlaps a tensor that is read, or another written run, of its own tensor either."""
+    if any(_runs_meet(*w) for w in writes):
+        return False
     spans = [(f.starts, f.ends) for f in _footprints(arena, reads, [], 0)]
     return not any(_runs_overlap(*a, *b) for i, a in enumerate(writes) for b in list(writes[i + 1:]) + spans)
 

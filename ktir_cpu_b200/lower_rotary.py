@@ -15,7 +15,7 @@ import numpy as np
 
 from . import runtime as R
 from .dtypes import bytes_per_elem
-from .lower import ArenaMap, Footprint, Statement, _access_offsets, _points, _runs_overlap, strip_views
+from .lower import ArenaMap, Footprint, Statement, _access_offsets, _points, _runs_meet, _runs_overlap, strip_views
 from .lower_scatter import row_form
 from .trace import Access, IndirectAccess, Node, Store, Unsupported
 
@@ -244,6 +244,8 @@ class RotaryStatement(Statement):
         # Everything is read before anything is stored: nothing that is written may be read by another part of the launch.
         writes = [f for f in self.fps if f.write]
         for k, w in enumerate(writes):
+            if _runs_meet(w.starts, w.ends):
+                raise Unsupported("a rotary launch that stores an element twice")
             for f in self.fps:
                 if f is not w and _runs_overlap(w.starts, w.ends, f.starts, f.ends):
                     raise Unsupported("a rotary launch that reads what it writes")

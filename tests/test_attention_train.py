@@ -833,3 +833,23 @@ def test_a_row_whose_scores_are_all_minus_infinity(c, build_lib):
     got = _run(K.attention_forward(*c), FWD, _kwargs(FWD, kw, c[0], c[2], c[4]), "attention_dense")
     assert (got["output_ptr"][0] == 0).all() and (got["lse_ptr"][0] == -np.inf).all()
     _check(got, formulas(kw, None, c[5]))
+
+
+@pytest.mark.parametrize("block", [16, 64])
+@pytest.mark.parametrize("strides", ["[64, 64, 1]", "[8, 256, 1]", "[256, 8, 1]", "[64, 8, 1]", "[256, 56, 1]"])
+def test_an_element_stored_twice_is_not_one_launch(strides, block):
+    """Rows or heads of a tile's result over one another: the last one stays, which CTAs in no order do not promise."""
+    kw, do = _inputs(64, 64, 4, 1, 64)
+    rows = strides.split(",")[0] + ", 64, 1]"
+    for fn, make, ptr, bit, old, new in ((FWD, K.attention_forward, "output", 0, "[256, 64, 1]", strides), (BWD, K.attention_backward, "query_grad", R.ATTN_DQ, "[256, 64, 1]", strides),
+                                         (BWD, K.attention_backward, "key_grad", R.ATTN_DK, "[64, 64, 1]", rows), (BWD, K.attention_backward, "value_grad", R.ATTN_DV, "[64, 64, 1]", rows)):
+        src = make(64, 64, 4, 1, 64, True, block, block)
+        full = _kwargs(fn, kw, 64, 4, 64, do, do, np.zeros((64, 4), np.float32))
+        i = src.index(f"construct_memory_view %{ptr}_ptr")
+        assert "strides: " + old in src[i:]
+        try:
+            plan = _session(src[:i] + src[i:].replace("strides: " + old, "strides: " + new, 1), fn, full).plan.statements
+        except NotImplementedError:
+            continue
+        if ptr in ("output", "query_grad") or new.startswith("[8,"):
+            assert not any(s.kind == "attention_dense" or s.kind == "attention_bwd" and s.args.want & bit for s in plan), ptr

@@ -277,3 +277,15 @@ def test_arena_on_any_boundary_of_its_types(case, wide, build_lib):
             np.testing.assert_array_equal(got, x, err_msg=f"{n} {shift}")
     dev.free(room)
     gpu.close()
+
+
+@pytest.mark.parametrize("tokens,block", [(8, 2), (2, 2)])
+@pytest.mark.parametrize("strides", ["[64, 0, 1]", "[0, 16, 1]", "[64, 8, 1]", "[16, 16, 1]"])
+def test_an_element_stored_twice_is_not_one_launch(strides, tokens, block):
+    """Heads or tokens over one another: the last one stays, which threads in no order do not promise."""
+    src, kw = _case(tokens, 4, 0, 16, 16, "half", False, "f16", block)
+    i = src.index("construct_memory_view %query_out_ptr")
+    assert "strides: [64, 16, 1]" in src[i:]
+    assert [s.kind for s in _session(src, kw).plan.statements] == ["rotary"]
+    src = src[:i] + src[i:].replace("strides: [64, 16, 1]", "strides: " + strides, 1)
+    assert "rotary" not in [s.kind for s in _session(src, kw).plan.statements]
