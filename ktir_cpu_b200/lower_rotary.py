@@ -19,6 +19,8 @@ from .lower import ArenaMap, Footprint, Statement, _access_offsets, _points, _ru
 from .lower_scatter import row_form
 from .trace import Access, IndirectAccess, Node, Store, Unsupported
 
+MOST_TOKENS = 2 ** 31 - 1                # of an item, whose tokens 32 bits count
+
 
 def _term(n: Node) -> Optional[Tuple[Access, IndirectAccess]]:
     """x * (a table row spread over the heads) -> (tile of x, table access)."""
@@ -204,7 +206,7 @@ class RotaryStatement(Statement):
         tokens = p0.tokens
         if tokens == 1 and len(table) > 1:         # (a tile of one token does not say how far the next one is)
             steps = [int(s) for s in table[1] - table[0]]
-        if len(table) > 1 and (np.diff(table, axis=0) == np.array(steps)[None, :] * tokens).all():
+        if 1 < len(table) <= MOST_TOKENS // tokens and (np.diff(table, axis=0) == np.array(steps)[None, :] * tokens).all():
             tokens, table = tokens * len(table), table[:1]     # the tiles follow one another: one run of tokens
         a.n_items, a.tokens, a.pairs = len(table), tokens, p0.pairs
         a.dtype, a.idx_dtype = R.DTYPE_CODE[p0.i.dtype], R.DTYPE_CODE[p0.cos.idx_dtype]

@@ -289,3 +289,11 @@ def test_an_element_stored_twice_is_not_one_launch(strides, tokens, block):
     assert [s.kind for s in _session(src, kw).plan.statements] == ["rotary"]
     src = src[:i] + src[i:].replace("strides: [64, 16, 1]", "strides: " + strides, 1)
     assert "rotary" not in [s.kind for s in _session(src, kw).plan.statements]
+
+
+@pytest.mark.parametrize("most,items", [(2 ** 31 - 1, 1), (12, 1), (11, 3), (1, 3)])
+def test_tokens_that_an_item_cannot_count_stay_items(most, items, monkeypatch):
+    from ktir_cpu_b200 import lower_rotary
+    monkeypatch.setattr(lower_rotary, "MOST_TOKENS", most)
+    st, = _session(*_case(12, 2, 0, 16, 16, "half", False, "f16", 4)).plan.statements
+    assert st.kind == "rotary" and (st.args.n_items, st.args.tokens) == (items, 12 // items)
