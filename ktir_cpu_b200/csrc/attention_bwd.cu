@@ -1012,6 +1012,7 @@ extern "C" int ktb_launch_attention_bwd(ktb_ctx* ctx, const ktb_attn_bwd_args* a
     if ((a.want & ~7) || a.want == 0) return ktb_fail(ctx, KTB_E_ARG, me, "which gradients are wanted");
     if (a.q_len == 0 || a.kv_len == 0 || a.heads == 0) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "no queries, keys or heads");
     if (a.q_len > (1 << 30) || a.kv_len > (1 << 30) || a.heads > 65535 * 32) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "lengths or heads");
+    if (((int64_t)a.q_len + AB_N - 1) / AB_N * a.kv_group > (1 << 28)) return ktb_fail(ctx, KTB_E_UNSUPPORTED, me, "too many steps of a tile of keys");
     if (!(fabs((double)a.scale) * a.head_dim * 65504.0 * 65504.0 <= 1.0e38))     // (scores of f16 operands, times 1 / ln 2)
         return ktb_fail(ctx, KTB_E_ARG, me, "scores must be finite");
     const int kv_heads = a.heads / a.kv_group;

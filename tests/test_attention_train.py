@@ -853,3 +853,18 @@ def test_an_element_stored_twice_is_not_one_launch(strides, block):
             continue
         if ptr in ("output", "query_grad") or new.startswith("[8,"):
             assert not any(s.kind == "attention_dense" or s.kind == "attention_bwd" and s.args.want & bit for s in plan), ptr
+
+
+@pytest.mark.gpu
+def test_launcher_refuses_more_steps_than_it_counts(build_lib):
+    """Heads may lie over one another in what is read, so that few bytes are many steps."""
+    gpu = KTIRInterpreter()
+    kw, do = _inputs(64, 64, 4, 2, 64)
+    gpu.load(K.attention_backward(64, 64, 4, 2, 64, True))
+    sess, _ = gpu.session(BWD, **_kwargs(BWD, kw, 64, 4, 64, do, do, np.zeros((64, 4), np.float32)))
+    a = sess.plan.statements[0].args
+    a.arena, a.q_len, a.heads, a.kv_group, a.scratch_bytes = sess.arena, 1 << 20, 1 << 15, 1 << 15, 1 << 60
+    before = gpu.device.launch_count()
+    assert gpu.device.lib.ktb_launch_attention_bwd(gpu.device.h, C.byref(a)) == -3 and gpu.device.launch_count() == before
+    assert b"steps" in gpu.device.lib.ktb_last_error(gpu.device.h)
+    gpu.close()
