@@ -868,3 +868,35 @@ def test_launcher_refuses_more_steps_than_it_counts(build_lib):
     assert gpu.device.lib.ktb_launch_attention_bwd(gpu.device.h, C.byref(a)) == -3 and gpu.device.launch_count() == before
     assert b"steps" in gpu.device.lib.ktb_last_error(gpu.device.h)
     gpu.close()
+
+
+# More items than SMs, so that a CTA takes one after the other: walks of keys, of queries, and empty ones (queries that see nothing) in
+# every order; the last two with more than sixteen items an SM, which are handed out head by head.
+MANY = [(300, 300, 60, 60, 128, True), (500, 500, 48, 48, 64, True), (700, 300, 40, 40, 128, True), (300, 700, 48, 12, 128, False), (257, 197, 64, 64, 64, False),
+        (450, 130, 60, 30, 64, True), (130, 130, 620, 620, 64, True), (200, 150, 640, 640, 128, False)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("c", MANY)
+def test_ctas_that_take_many_items(c, build_lib):
+    kw, do = _inputs(*c[:5], seed=c[1])
+    items = -(-c[1] // 128) * c[3] + -(-c[0] // 128) * c[2]
+    assert items > 148 and (c[2] < 600 or items > 16 * 148)
+    assert grad_parts(*c[:4], int(c[5]), c[1] - c[0] if c[5] else 0) == (1, 1) and not few_rows(c[0], c[2], c[5], c[1] - c[0], FEW_ROWS_BACKWARD)
+    o, lse = _forward_results(kw, c[5])
+    got = _run(K.attention_backward(*c), BWD, _kwargs(BWD, kw, c[0], c[2], c[4], do, o, lse), "attention_bwd", times=3)
+    _check(got, formulas(kw, do, c[5], o, lse))
+    got = _run(K.attention_forward(*c), FWD, _kwargs(FWD, kw, c[0], c[2], c[4]), "attention_dense", times=3)
+    _check(got, formulas(kw, None, c[5]))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("parts", [(2, 3), (5, 1)])
+@pytest.mark.parametrize("c", [(300, 300, 40, 40, 128, True), (450, 430, 30, 10, 128, False), (500, 130, 40, 20, 64, True)])
+def test_ctas_that_take_many_parts(c, parts, build_lib, monkeypatch):
+    from ktir_cpu_b200 import lower_attn_train
+    monkeypatch.setattr(lower_attn_train, "grad_parts", lambda *a: parts)
+    kw, do = _inputs(*c[:5], seed=c[1])
+    o, lse = _forward_results(kw, c[5])
+    got = _run(K.attention_backward(*c), BWD, _kwargs(BWD, kw, c[0], c[2], c[4], do, o, lse), "attention_bwd", times=3)
+    _check(got, formulas(kw, do, c[5], o, lse))

@@ -297,3 +297,52 @@ def test_tokens_that_an_item_cannot_count_stay_items(most, items, monkeypatch):
     monkeypatch.setattr(lower_rotary, "MOST_TOKENS", most)
     st, = _session(*_case(12, 2, 0, 16, 16, "half", False, "f16", 4)).plan.statements
     assert st.kind == "rotary" and (st.args.n_items, st.args.tokens) == (items, 12 // items)
+
+
+# (tokens, heads, key heads, head size, turned part, layout, backwards, type, tokens per core, cores in reverse): where four heads go to
+# a thread (148 x 4096 of its vectors and more; half as many for rows of 16 bytes), head counts that are no multiple of four, heads of one
+# thread in both tensors, rests, several items
+LARGE = [(27000, 9, 1, 128, 128, "half", False, "f16", None, False), (27000, 9, 1, 128, 128, "interleaved", True, "f16", None, False),
+         (9000, 13, 2, 128, 64, "half", False, "f32", 36, True), (16000, 10, 3, 96, 48, "interleaved", True, "f32", None, False),
+         (40000, 5, 2, 96, 64, "half", True, "f16", 100, True), (60000, 3, 2, 64, 32, "interleaved", False, "f16", None, False),
+         (16384, 9, 1, 128, 54, "half", False, "f16", None, False), (16384, 9, 1, 128, 54, "interleaved", True, "f16", 64, True),
+         (9000, 13, 2, 96, 50, "half", True, "f32", 45, True), (9000, 6, 5, 96, 26, "interleaved", False, "f32", None, False),
+         (30000, 2, 1, 62, 22, "half", False, "f16", None, False), (8000, 6, 1, 61, 18, "interleaved", True, "f16", None, False)]
+
+
+def _restated(x, kw, part, layout, inverse):
+    """In f32, products and sums rounded one by one."""
+    n = part // 2
+    cos, sin = kw["cos_ptr"][kw["positions_ptr"]][:, None], kw["sin_ptr"][kw["positions_ptr"]][:, None]
+    j = np.arange(n)
+    a, b = (j, j + n) if layout == "half" else (2 * j, 2 * j + 1)
+    y, u, v = x.copy(), x[..., a].astype(np.float32), x[..., b].astype(np.float32)
+    sin = -sin if inverse else sin
+    y[..., a], y[..., b] = u * cos - v * sin, v * cos + u * sin
+    return y
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("case", LARGE)
+def test_four_heads_to_a_thread(case, build_lib):
+    src, kw = _case(*case[:9])
+    if case[9]:
+        cores = case[0] // case[8]
+        src = src.replace("    %t0 = arith.muli %pid, %c_bt : index\n", f"    %c_last = arith.constant {cores - 1} : index\n    %rev = arith.subi %c_last, %pid : index\n"
+                                                                         f"    %t0 = arith.muli %rev, %c_bt : index\n")
+    gpu = KTIRInterpreter()
+    gpu.load(src)
+    got = gpu.execute_function("rotary_kernel", **kw)
+    st, = [s for sess in gpu._sessions.values() for s in sess.plan.statements]
+    assert st.kind == "rotary" and st.args.n_items == (case[0] // case[8] if case[9] else 1)
+    gpu.close()
+    for name in ("query", "key"):
+        np.testing.assert_array_equal(got[name + "_out_ptr"], _restated(kw[name + "_ptr"], kw, *case[4:7]), err_msg=name)
+
+
+@pytest.mark.parametrize("case", CASES)
+def test_restatement_has_the_oracles_bits(case):
+    src, kw = _case(*case)
+    want = _oracle(src, kw)
+    for name in ("query", "key") if case[2] else ("query",):
+        np.testing.assert_array_equal(want[name + "_out_ptr"], _restated(kw[name + "_ptr"], kw, *case[4:7]))
