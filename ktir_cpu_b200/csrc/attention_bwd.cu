@@ -11,20 +11,20 @@
 //
 // Both kinds of tile are the same loop.  A CTA holds two tiles of 128 rows X and Y (K and V, or Q and dO) in shared memory and
 // streams pairs of 64-row tiles X', Y' (Q and dO, or K and V) through a ring by TMA.  Per step one warp issues
-// S = X X'^T and T = Y Y'^T into one of two slots of TMEM (three for queries, which have one accumulator less); two threads
-// a row read them, 32 columns each, and write P and dS as f16 over the same columns; the next products take them from there
+// S = X X'^T and T = Y Y'^T into a slot of TMEM (there are two at 128 columns a head, three at 64); a warpgroup reads them, a thread
+// a row (two take the steps in turn), and writes P and dS as f16 over the same columns; the next products take them from there
 // as their A operand: acc0 += dS X' and, for keys, acc1 += P Y'.  While one step is in the softmax, the tensor core has the
 // other slots'.
 //
 // f16 operands.  P is at most 1 but mostly near 1 / keys, dS is as small as the gradient: both are rounded to f16 (2^-12 of the
-// value on average, the only roundings before the results') after a shift by powers of two that keeps them in range: P by
-// 2^14, dS by 2^14 / B with B >= |dO V^T - D| a power of two from the norms of dO and V: for dQ, whose sums run over keys, per
-// query and from the keys that it sees, for dK per key and from the queries that see it.  (From all of a head, dK of the keys
-// behind a query 10^6 times as loud as the others lost 2 % of its value, dQ of the queries before such a value likewise.)  Sums, D and the statistics are f32.  Where few rows see a key these roundings are multiplied too
-// (MODE 2).
+// value on average; exp2 is approximate to 2^-22, all else before the results is f32) after a shift by powers of two that keeps
+// them in range: P by 2^14, dS by 2^14 / B with B >= |dO V^T - D| a power of two from the norms of dO and V: for dQ, whose sums
+// run over keys, per query and from the keys that it sees, for dK per key and from the queries that see it.  (From all of a head,
+// dK of the keys behind a query 10^6 times as loud as the others lost 2 % of its value, dQ of the queries before such a value
+// likewise.)  Sums, D and the statistics are f32.  Where few rows see a key these roundings are multiplied too (MODE 2).
 //
-// 256 heads of 2048 positions, 128 wide, causal: 1.04 ms, 660 TFLOP/s of the five products (925 of the seven), 1.20 ms once
-// the power cap holds; 16 / 4 heads of 8192 positions 0.76 ms, 906, capped 0.87.
+// 256 heads of 2048 positions, 128 wide, causal: 1.03 ms, 667 TFLOP/s of the five products (933 of the seven), 1.20 ms once
+// the power cap holds; 16 / 4 heads of 8192 positions 0.76 ms, 906, capped 0.88.
 #include <type_traits>
 
 #include "tc_common.cuh"
@@ -38,8 +38,8 @@
 static __device__ __forceinline__ void ab_follow() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 static __device__ __forceinline__ void ab_wait_for_rows() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
-// ---- what the rows bring: 14 - lse / ln 2, D, |dO| per row, and the largest norms of a block of rows ---------------
-// HBM bounds it (O, dO and V once; 256 heads of 2048 positions, 128 wide: 86 us, 4.7 TB/s).  A block takes
+// ---- what the rows bring: 14 - lse / ln 2, D and |dO| per query, |V| per key, and the largest norms of a block of rows --
+// HBM bounds it (O, dO and V once; 256 heads of 2048 positions, 128 wide: 81 us, 5.0 TB/s).  A block takes
 // BLOCK rows of heads, 2^heads_log neighbouring heads of BLOCK >> heads_log positions (so that what it reads lies together),
 // head_dim / 8 threads each, four of their loads ahead of the arithmetic.
 struct ab_scratch {

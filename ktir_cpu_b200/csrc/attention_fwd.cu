@@ -119,9 +119,9 @@ enum { B_QFULL = 0, B_QFREE = 2, B_KVFULL = 4, B_KVEMPTY = B_KVFULL + AT_MAX_STA
 // of the current one run, and its first scores are computed while the softmax warps normalise and
 // store the output, so a tile pair no longer pays a start-up and a drain of its own.
 //
-// DENSE: keys and values are rows of one tensor instead of pages, a.num_tiles groups of BN of them of which d.kv_len exist;
-// rows that see nothing give 0, and the log-sum-exp of every row is kept (256 heads of 2048 positions, 128 wide, causal: 291 us,
-// 944 TFLOP/s, 344 once the power cap holds; 1531 queries of 32 heads over 4603 keys 107 us: 192 pairs of tiles on 148
+// DENSE: keys and values are the d.kv_len rows of one tensor, BN at a time, instead of pages;
+// rows that see nothing give 0, and the log-sum-exp of every row is kept (256 heads of 2048 positions, 128 wide, causal: 286 us,
+// 962 TFLOP/s, 339 once the power cap holds; 1531 queries of 32 heads over 4603 keys 109 us: 192 pairs of tiles on 148
 // SMs).  d.single: an item is one pair of tiles.  PARTS: the keys of an item are cut into d.parts
 // ranges, an item of its own each, where whole items would leave most SMs idle; ktb_attention_join_fwd_kernel joins them.  With
 // d.twice every page comes twice: P as f16 times V, then what that rounding left out (up to 2^-12 of P) times V.  A result is

@@ -1363,7 +1363,7 @@ def rotary(tokens: int = 64, heads: int = 8, kv_heads: int = 2, head_dim: int = 
     [table_rows, rotary_dim / 2].  Pair j of a head's first ``rotary_dim`` elements is turned by that angle,
     (a, b) -> (a cos - b sin, b cos + a sin), in f32, rounded once; the elements behind are copied.  ``layout`` says which
     elements are pair j: "half" j and j + rotary_dim / 2, "interleaved" 2j and 2j + 1.  ``inverse`` turns back: the
-    gradient of the rotation.  ``kv_heads = 0`` leaves the keys out.  The tables hold whatever frequencies a model uses
+    gradient of the rotation.  The results are tensors of their own.  ``kv_heads = 0`` leaves the keys out.  The tables hold whatever frequencies a model uses
     (``rotary_tables``).  A core owns ``block`` tokens, a divisor of ``tokens``; one token's heads have to fit its scratchpad
     (``heads * rotary_dim`` up to 65536)."""
     rot = head_dim if rotary_dim is None else rotary_dim
